@@ -52,7 +52,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     cu, cpp = _sources()
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    headers.append(os.path.join(ROOT, "include", "hoard_moe.h"))
+    headers += [os.path.join(ROOT, "include", h) for h in ("hoard_moe.h", "hoard_harness.h", "hoard_cache.h")]
     objs, jobs = [], []
     cxx = shutil.which("g++") or "g++"
     for f in cu:

@@ -165,6 +165,12 @@ cudaError_t launch_rmsnorm_q8(const float* x, int H, float eps, const float* w, 
 cudaError_t launch_qgemv_set(int n, const int* types, const uint8_t* const* w, const int* N, int K,
                              const float* const* resid, float* const* y, const int8_t* xq, const float* xd,
                              const int* xbs, cudaStream_t s);
+cudaError_t launch_qknorm_rope_store_rows(const float* q, int64_t q_ts, int64_t q_hs, const float* k, const float* v,
+                                          const float* qn, const float* kn, int mode, float eps, int n_head, int n_kv,
+                                          int hd, int rope_dim, const int32_t* pos, int m, int row0,
+                                          const int32_t* row0_dev, int max_rows, float freq_base, float* q_out, void* kc,
+                                          void* vc, int64_t rs, int64_t hs, bool kv_bf16, float* acc, int32_t* row_pos,
+                                          cudaStream_t s);
 cudaError_t launch_qknorm_rope_store(const float* q, const float* k, const float* v, const float* qn, const float* kn,
                                      int mode, float eps, int n_head, int n_kv, int hd, int q_stride, int rope_dim,
                                      int pos, const int32_t* pos_dev, int max_ctx, float freq_base, float* q_out,

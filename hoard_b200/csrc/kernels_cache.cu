@@ -1,0 +1,619 @@
+// kernels_cache.cu -- attention of several query tokens over a KV cache, split over the cache's rows.
+//
+//   s_rj = scale * q_r . K_j,  out_r = sum_j exp(s_rj - M_r) V_j / sum_j exp(s_rj - M_r),  M_r = max_j s_rj
+//
+// For the R query rows of a KV head (tokens x query heads of the head) the cache's K and V are read once
+// and every product is a matrix instruction (m16n8k16): S^T[16 rows j x 8 query rows] = K q^T, and
+// O^T[dims x 8 query rows] += V^T P^T. Eight query rows are the N of the instruction, so one token of a
+// model with eight heads per KV head wastes nothing. The sums over j are split over CTAs, and inside a
+// CTA over warps: a warp takes 16-row chunks of the cache through a ring of its own (cp.async, no barrier
+// between warps), with its own running maximum and total, and the partial results are joined once at the
+// end of the CTA and once after all CTAs (k_cache_combine).
+//
+// Precision. K and V enter the products as they are stored. q (f32) and the weights p (f32) are written as
+// sums of f16 or bf16 terms, whatever the cache's type is: two f16 terms hold 22 bits, three bf16 terms 24, so
+// a product is f32-accurate; sums, maxima and totals are f32. For f16 the rows of q are scaled by a power of
+// two to [2^13, 2^14) and p by 2^14, which keeps the terms out of f16's subnormal range; the factors are taken out
+// of the scores (exactly) and cancel in p / total.
+#include "common.cuh"
+#include "kernels_cache.h"
+#include "async_copy.cuh"
+
+namespace hoard {
+
+namespace {
+
+template <typename KT> struct Terms;
+template <> struct Terms<__half> {
+    static constexpr int N = 2, Q_EXP = 13;
+    static constexpr float P_EXP = 14.f;
+    static constexpr uint32_t INF2 = 0x7C007C00u;        // exponent bits of two values
+};
+template <> struct Terms<__nv_bfloat16> {
+    static constexpr int N = 3, Q_EXP = 0;
+    static constexpr float P_EXP = 0.f;
+    static constexpr uint32_t INF2 = 0x7F807F80u;
+};
+
+// two f32 -> packed terms: a's rounding in the low half, b's in the high half; a and b become the remainders
+template <typename KT> __device__ __forceinline__ uint32_t take_term(float& a, float& b);
+template <> __device__ __forceinline__ uint32_t take_term<__half>(float& a, float& b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    a -= f.x;
+    b -= f.y;
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t take_term<__nv_bfloat16>(float& a, float& b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    a -= f.x;
+    b -= f.y;
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename KT> __device__ __forceinline__ float kv_lo(uint32_t w);
+template <> __device__ __forceinline__ float kv_lo<__half>(uint32_t w) { return h2f(w); }
+template <> __device__ __forceinline__ float kv_lo<__nv_bfloat16>(uint32_t w) { return __uint_as_float(w << 16); }
+
+template <typename KT>
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(KT) == 2 && Terms<KT>::N == 2)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldm4(uint32_t* r, unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t* r, unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// 16 bytes global -> shared, or 16 zero bytes where !there (the source is not read)
+__device__ __forceinline__ void cp16z(unsigned dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+template <int N> __device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Warps and ring stages of one CTA (one CTA per SM): with head_dim 128 a stage is 16 rows of K and V, 8 KiB,
+// and eight warps keep two stages each in flight, 128 KiB per SM, while they work on a third.
+template <int HD> struct Plan {
+    static constexpr int W = HD == 256 ? 4 : 8;
+    static constexpr int ST = HD == 64 ? 4 : 3;
+    static constexpr int STAGE = 2 * KV_CHUNK * HD * 2;            // bytes
+    static constexpr int RING = W * ST * STAGE;
+};
+template <typename KT, int HD, int NT> constexpr int q_bytes() { return HD / 16 * NT * Terms<KT>::N * 32 * 8; }
+template <typename KT, int HD, int NT> constexpr int attn_smem() {
+    return Plan<HD>::RING + q_bytes<KT, HD, NT>();
+}
+
+__device__ __forceinline__ int past_rows(const CacheAttn& a) {
+    return a.n_past_dev ? max(0, min(*a.n_past_dev, a.max_rows - a.m)) : a.n_past;
+}
+
+template <typename KT, int HD, int NT, bool BLOCKS>
+__global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const CacheAttn a) {
+    constexpr int W = Plan<HD>::W, ST = Plan<HD>::ST, TN = Terms<KT>::N;
+    constexpr int KS = HD / 16;                        // K steps of q . K = M tiles of V^T
+    constexpr int RT = 8 * NT;                         // query rows of the tile
+    constexpr int PITCH = HD * 2;                      // bytes of a staged row
+    constexpr int C16 = HD / 8;                        // 16-byte pieces of a row
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ float s_scale[RT];                      // per query row: scale, log2(e) and the row's power of two
+    __shared__ uint64_t s_vis[RT];
+    __shared__ float s_m[W][RT], s_l[W][RT];
+    pdl_enter();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = blockIdx.x, tile = blockIdx.y, prob = blockIdx.z;
+    const int n_past = past_rows(a);
+    const int kv = BLOCKS ? prob / a.m : prob;
+    const int t0 = BLOCKS ? prob - kv * a.m : 0;       // first token of the problem's rows
+    uint32_t* qf = reinterpret_cast<uint32_t*>(smem + Plan<HD>::RING);
+
+    // chunks of this CTA: past rows (or the listed blocks' rows), then the tokens' own rows
+    const int sub = BLOCKS ? a.block / KV_CHUNK : 1;
+    const int n_pc = BLOCKS ? a.list_n[prob] * sub : (n_past + KV_CHUNK - 1) / KV_CHUNK;
+    const int n_chunks = n_pc + (a.m + KV_CHUNK - 1) / KV_CHUNK;
+    const int c_end = (int)((int64_t)n_chunks * (split + 1) / a.splits);
+    const int c_first = (int)((int64_t)n_chunks * split / a.splits) + warp;
+    const int32_t* list = BLOCKS ? a.list + (int64_t)prob * a.list_cap : nullptr;
+    auto chunk_row = [&](int c) {                      // first cache row of chunk c
+        if (c >= n_pc) return n_past + (c - n_pc) * KV_CHUNK;
+        if (BLOCKS) return list[c / sub] * a.block + (c % sub) * KV_CHUNK;
+        return c * KV_CHUNK;
+    };
+    auto chunk_end = [&](int c) { return c >= n_pc ? n_past + a.m : n_past; };
+
+    // the warp's ring; lane -> (row of the piece, 16-byte piece) with consecutive lanes on consecutive pieces
+    const unsigned ring = smem_u32(smem) + warp * ST * Plan<HD>::STAGE;
+    const char* kbase = reinterpret_cast<const char*>(a.kc) + (int64_t)kv * a.hs * 2;
+    const char* vbase = reinterpret_cast<const char*>(a.vc) + (int64_t)kv * a.hs * 2;
+    auto issue = [&](int c, int stage) {
+        const int row0 = chunk_row(c), end = chunk_end(c);
+        const unsigned dst0 = ring + stage * Plan<HD>::STAGE;
+#pragma unroll
+        for (int i = 0; i < KV_CHUNK * C16 / 32; ++i) {
+            const int p = i * 32 + lane, r = p / C16, c16 = p % C16;
+            const bool there = row0 + r < end && c16 * 8 < a.hd;
+            const int64_t off = there ? (int64_t)(row0 + r) * a.rs * 2 + c16 * 16 : 0;
+            const unsigned dst = dst0 + r * PITCH + ((c16 ^ (r & 7)) << 4);
+            cp16z(dst, kbase + off, there);
+            cp16z(dst + KV_CHUNK * PITCH, vbase + off, there);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) {
+        if (c_first + s * W < c_end) issue(c_first + s * W, s);
+        cp_async_commit();
+    }
+
+    // the tile's q rows as fragments of the B operand: [K step][8-row tile][term][lane] of 8 bytes
+    for (int r = warp; r < RT; r += W) {
+        const int row = tile * RT + r;                 // row = (token - t0) * g + head of the KV head
+        const bool live = row < a.R;
+        const int t = t0 + (live ? row / a.g : 0), h = kv * a.g + (live ? row % a.g : 0);
+        const float* q = a.q + t * a.q_ts + h * a.q_hs;
+        float x[HD / 32];
+        float am = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+            const int d = i * 32 + lane;
+            x[i] = live && d < a.hd ? q[d] : 0.f;
+            bad |= !(fabsf(x[i]) <= 3.4e38f);
+            am = fmaxf(am, fabsf(x[i]));
+        }
+        am = warp_max(am);
+        bad = __any_sync(0xffffffffu, bad);
+        // 2^e <= am < 2^(e+1); q is scaled by 2^(Q_EXP - e), exactly
+        int e = (int)(__float_as_uint(am) >> 23) - 127;
+        e = bad || am == 0.f ? Terms<KT>::Q_EXP : max(e, -100);
+        const float up = __uint_as_float((uint32_t)(127 + Terms<KT>::Q_EXP - e) << 23);
+        if (lane == 0) {
+            s_scale[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - Terms<KT>::Q_EXP + e) << 23);
+            uint64_t own = 0;
+            if (live) own = a.vis ? a.vis[t] : (t >= 63 ? ~0ull : (1ull << (t + 1)) - 1);
+            s_vis[r] = own;
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+            // lanes 2c, 2c + 1 hold the pair of dims that one fragment register packs
+            float lo = x[i] * up;
+            float hi = __shfl_down_sync(0xffffffffu, lo, 1);
+            const int d = i * 32 + lane, kk = d >> 4, reg = (d >> 3) & 1, c = (d & 7) >> 1;
+#pragma unroll
+            for (int u = 0; u < TN; ++u) {
+                const uint32_t w = take_term<KT>(lo, hi);
+                if (!(lane & 1))
+                    qf[((((kk * NT + (r >> 3)) * TN + u) * 32) + ((r & 7) << 2) + c) * 2 + reg] = w;
+            }
+        }
+    }
+    __syncthreads();
+
+    // fragment addresses inside a stage
+    const int k_r = (lane & 7) + ((lane >> 3) & 1) * 8, k_c = lane >> 4;         // K: rows j, dims
+    const int v_r = (lane & 7) + (lane >> 4) * 8, v_c = (lane >> 3) & 1;         // V transposed: keys, dims
+    const int cq = lane & 3;                            // query rows 2 cq, 2 cq + 1 of each 8-row tile
+
+    float o[KS][NT][4];
+    float mx[NT][2], tot[NT][2], sc[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mx[n][i] = -INFINITY;
+            tot[n][i] = 0.f;
+            sc[n][i] = s_scale[8 * n + 2 * cq + i];
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
+    }
+
+    int stage = 0;
+    for (int c = c_first; c < c_end; c += W) {
+        cp_wait<ST - 2>();
+        __syncwarp();
+        {
+            const int nx = c + (ST - 1) * W;
+            const int ns = stage == 0 ? ST - 1 : stage - 1;
+            if (nx < c_end) issue(nx, ns);
+            cp_async_commit();
+        }
+        const unsigned ks = ring + stage * Plan<HD>::STAGE, vs = ks + KV_CHUNK * PITCH;
+        // ---- S^T = K q^T ----
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            uint32_t af[4];
+            ldm4(af, ks + k_r * PITCH + (((2 * k + k_c) ^ (k_r & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int u = 0; u < TN; ++u) {
+                    const uint2 b = *reinterpret_cast<const uint2*>(qf + ((((k * NT + n) * TN + u) * 32) + lane) * 2);
+                    mma16816<KT>(s[n], af, b.x, b.y);
+                }
+        }
+        // ---- scores in log2 units; masked ones -inf ----
+        const int row0 = chunk_row(c), left = chunk_end(c) - row0;               // rows of the chunk that exist
+        const bool own = c >= n_pc;
+        const int j0 = lane >> 2, j1 = j0 + 8;                                   // this thread's rows of the chunk
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] *= sc[n][i & 1];
+        if (left < KV_CHUNK || own) {
+            const int sh = own ? row0 - n_past : 0;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = i < 2 ? j0 : j1;
+                    const bool see = j < left && (!own || (s_vis[8 * n + 2 * cq + (i & 1)] >> (sh + j) & 1));
+                    if (!see) s[n][i] = -INFINITY;
+                }
+        }
+        if (!BLOCKS && a.logits) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = tile * RT + 8 * n + 2 * cq + (i & 1), j = i < 2 ? j0 : j1;
+                    if (row < a.R && j < left) a.logits[((int64_t)kv * a.R + row) * a.logits_ld + row0 + j] = s[n][i];
+                }
+        }
+        // ---- running maximum; earlier sums are rescaled only when one rises ----
+        bool rises = false;
+        float top[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float v = fmaxf(s[n][i], s[n][i + 2]);
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                top[n][i] = fmaxf(mx[n][i], v);
+                rises |= top[n][i] > mx[n][i];
+            }
+        if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float f[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    f[i] = top[n][i] > mx[n][i] ? ex2(mx[n][i] - top[n][i]) : 1.f;
+                    mx[n][i] = top[n][i];
+                    tot[n][i] *= f[i];
+                }
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    o[k][n][0] *= f[0];
+                    o[k][n][1] *= f[1];
+                    o[k][n][2] *= f[0];
+                    o[k][n][3] *= f[1];
+                }
+            }
+        }
+        // ---- weights, their terms as B fragments ----
+        uint32_t pf[NT][TN][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) b[i] = mx[n][i] == -INFINITY ? 0.f : mx[n][i] - Terms<KT>::P_EXP;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = ex2(s[n][i] - b[i & 1]);
+            tot[n][0] += s[n][0] + s[n][2];
+            tot[n][1] += s[n][1] + s[n][3];
+        }
+        // masked own rows may hold infinities or NaN (0 * inf): such a chunk takes its products one by one
+        bool odd = false;
+        if (own) {
+            for (int i = lane; i < KV_CHUNK * C16; i += 32) {
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(vs + i * 16) : "memory");
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t e = w[k] & Terms<KT>::INF2;
+                    odd |= (e & 0xFFFFu) == (Terms<KT>::INF2 & 0xFFFFu) || (e >> 16) == (Terms<KT>::INF2 >> 16);
+                }
+            }
+            odd = __any_sync(0xffffffffu, odd);
+        }
+        if (!odd) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float r[4] = {s[n][0], s[n][1], s[n][2], s[n][3]};
+#pragma unroll
+                for (int u = 0; u < TN; ++u) {
+                    pf[n][u][0] = transpose8(take_term<KT>(r[0], r[1]));
+                    pf[n][u][1] = transpose8(take_term<KT>(r[2], r[3]));
+                }
+            }
+            // ---- O^T += V^T P^T ----
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t af[4];
+                ldm4t(af, vs + v_r * PITCH + (((2 * k + v_c) ^ (v_r & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int u = 0; u < TN; ++u) mma16816<KT>(o[k][n], af, pf[n][u][0], pf[n][u][1]);
+            }
+        } else {
+            for (int j = 0; j < KV_CHUNK; ++j) {
+                const int src = ((j & 7) << 2) + cq;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float p0 = __shfl_sync(0xffffffffu, j < 8 ? s[n][0] : s[n][2], src);
+                    const float p1 = __shfl_sync(0xffffffffu, j < 8 ? s[n][1] : s[n][3], src);
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int d = 16 * k + 8 * i + (lane >> 2);
+                            unsigned short hv;
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(hv)
+                                         : "r"(vs + j * PITCH + (((d >> 3) ^ (j & 7)) << 4) + (d & 7) * 2) : "memory");
+                            const float v = kv_lo<KT>(hv);
+                            if (p0 != 0.f) o[k][n][2 * i] += p0 * v;
+                            if (p1 != 0.f) o[k][n][2 * i + 1] += p1 * v;
+                        }
+                }
+            }
+        }
+        stage = stage == ST - 1 ? 0 : stage + 1;
+    }
+    cp_async_wait_all();
+
+    // ---- join the warps: totals over the four lanes' rows, then sums relative to the CTA's maximum ----
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float v = tot[n][i];
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 8);
+            v += __shfl_xor_sync(0xffffffffu, v, 16);
+            // a total of NaN without a maximum (every score NaN) has to reach the output: any finite maximum does
+            if (v != v && mx[n][i] == -INFINITY) mx[n][i] = 0.f;
+            if (lane < 4) {
+                s_m[warp][8 * n + 2 * cq + i] = mx[n][i];
+                s_l[warp][8 * n + 2 * cq + i] = v;
+            }
+        }
+    __syncthreads();                                   // every warp has left its ring
+    constexpr int OP = HD + 4;                         // floats of a row in the join buffer (over the ring)
+    static_assert(W * RT * OP * 4 <= attn_smem<KT, HD, NT>(), "join buffer");
+    float* joined = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = 8 * n + 2 * cq + i;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][r]);
+            const float f = mx[n][i] == -INFINITY ? 0.f : ex2(mx[n][i] - top);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                joined[(warp * RT + r) * OP + 16 * k + (lane >> 2)] = mx[n][i] == -INFINITY ? 0.f : o[k][n][i] * f;
+                joined[(warp * RT + r) * OP + 16 * k + 8 + (lane >> 2)] = mx[n][i] == -INFINITY ? 0.f : o[k][n][i + 2] * f;
+            }
+        }
+    __syncthreads();
+    const bool whole = a.splits == 1 && !a.logits;     // nothing to join with: the output itself
+    const int64_t part = ((int64_t)prob * a.row_tiles + tile) * a.splits + split;
+    for (int x = tid; x < RT * (HD / 4); x += W * 32) {
+        const int r = x / (HD / 4), d = (x - r * (HD / 4)) * 4;
+        const int row = tile * RT + r;
+        if (row >= a.R) continue;
+        float top = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][r]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) l += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * ex2(s_m[w][r] - top);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float4 u = *reinterpret_cast<const float4*>(joined + (w * RT + r) * OP + d);
+            v.x += u.x;
+            v.y += u.y;
+            v.z += u.z;
+            v.w += u.w;
+        }
+        if (whole) {
+            if (d >= a.hd) continue;
+            const int t = t0 + row / a.g, h = kv * a.g + row % a.g;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+            if (a.gate) {
+                const float* gp = a.gate + t * a.gate_ts + h * a.gate_hs + d;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] *= sigmoid_f(gp[i]);
+            }
+            float* op = a.out + ((int64_t)t * a.n_head + h) * a.hd + d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) op[i] = y[i];
+        } else {
+            *reinterpret_cast<float4*>(a.part_o + (part * RT + r) * HD + d) = v;
+            if (d == 0) a.part_ml[part * RT + r] = make_float2(top, l);
+        }
+    }
+}
+
+// ---- joins the splits of every query row, and with acc adds the rows' weights to the accumulated ones -------
+// A CTA of 128 threads per query row (token, head): factors 2^(m_s - M) of the splits, then float4 columns x
+// split groups. The CTAs after them take 512 cache rows of a KV head each: w = sum over the head's query rows
+// of 2^(s - M) / L in row order, one thread per cache row.
+constexpr int CB = 128, ACC_ROWS = 512, ACC_MAX_R = 512;
+__global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int rt, int hdt, int per) {
+    pdl_enter();
+    __shared__ float s_f[KV_SMS];
+    __shared__ float4 s_o[CB];
+    __shared__ float s_mr[ACC_MAX_R], s_ir[ACC_MAX_R];
+    const int tid = threadIdx.x;
+    const int n_rows = a.problems * a.R;
+    if ((int)blockIdx.x < n_rows) {
+        const int prob = blockIdx.x / a.R, row = blockIdx.x - prob * a.R;
+        const int tile = row / rt, r = row - tile * rt;
+        const int64_t part = ((int64_t)prob * a.row_tiles + tile) * a.splits;
+        float top = -INFINITY;
+        for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[(part + s) * rt + r].x);
+        for (int s = tid; s < a.splits; s += CB) {
+            const float ms = a.part_ml[(part + s) * rt + r].x;
+            s_f[s] = ms == -INFINITY ? 0.f : ex2(ms - top);
+        }
+        __syncthreads();
+        float l = 0.f;
+        for (int s = 0; s < a.splits; ++s) l += s_f[s] == 0.f ? 0.f : s_f[s] * a.part_ml[(part + s) * rt + r].y;
+        const int v4 = a.hd / 4, groups = CB / v4, gi = tid / v4, c = tid - gi * v4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (gi < groups) {
+            for (int s = gi; s < a.splits; s += groups) {
+                const float f = s_f[s];
+                if (f != 0.f) {
+                    const float4 u = *reinterpret_cast<const float4*>(a.part_o + ((part + s) * rt + r) * hdt + 4 * c);
+                    v.x += f * u.x;
+                    v.y += f * u.y;
+                    v.z += f * u.z;
+                    v.w += f * u.w;
+                }
+            }
+            s_o[tid] = v;
+        }
+        __syncthreads();
+        if (gi == 0) {
+            for (int k = 1; k < groups; ++k) {
+                const float4 u = s_o[k * v4 + c];
+                v.x += u.x;
+                v.y += u.y;
+                v.z += u.z;
+                v.w += u.w;
+            }
+            const bool blocks = a.list != nullptr;
+            const int kv = blocks ? prob / a.m : prob;
+            const int t = (blocks ? prob - kv * a.m : 0) + row / a.g, h = kv * a.g + row % a.g;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+            if (a.gate) {
+                const float* gp = a.gate + t * a.gate_ts + h * a.gate_hs + 4 * c;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] *= sigmoid_f(gp[i]);
+            }
+            float* op = a.out + ((int64_t)t * a.n_head + h) * a.hd + 4 * c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) op[i] = y[i];
+        }
+        return;
+    }
+    // accumulation
+    const int n = past_rows(a) + a.m;
+    const int x = blockIdx.x - n_rows, kv = x / per, j0 = (x - kv * per) * ACC_ROWS;
+    if (j0 >= n) return;
+    for (int row = tid; row < a.R; row += CB) {
+        const int tile = row / rt, r = row - tile * rt;
+        const int64_t part = ((int64_t)kv * a.row_tiles + tile) * a.splits;
+        float top = -INFINITY, l = 0.f;
+        for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[(part + s) * rt + r].x);
+        for (int s = 0; s < a.splits; ++s) {
+            const float2 ml = a.part_ml[(part + s) * rt + r];
+            l += ml.x == -INFINITY ? 0.f : ex2(ml.x - top) * ml.y;
+        }
+        s_mr[row] = top;
+        s_ir[row] = l == 0.f ? 0.f : 1.f / l;
+    }
+    __syncthreads();
+    const float pe = a.bf16 ? Terms<__nv_bfloat16>::P_EXP : Terms<__half>::P_EXP;      // l holds 2^P_EXP sum p
+    for (int j = j0 + tid; j < min(n, j0 + ACC_ROWS); j += CB) {
+        const float* lg = a.logits + (int64_t)kv * a.R * a.logits_ld + j;
+        float w = 0.f;
+        for (int row = 0; row < a.R; ++row)
+            if (s_ir[row] != 0.f) w += ex2(lg[row * a.logits_ld] - (s_mr[row] - pe)) * s_ir[row];
+        a.acc[(int64_t)kv * a.max_rows + j] += w;
+    }
+}
+
+template <typename KT, int HD, int NT, bool BLOCKS>
+cudaError_t attention_go(const CacheAttn& a, cudaStream_t s) {
+    constexpr int smem = attn_smem<KT, HD, NT>();
+    cudaError_t e = cudaFuncSetAttribute(k_cache_attention<KT, HD, NT, BLOCKS>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k_cache_attention<KT, HD, NT, BLOCKS>, dim3(a.splits, a.row_tiles, a.problems), Plan<HD>::W * 32,
+                      smem, s, a);
+}
+template <typename KT, int HD, int NT> cudaError_t attention_form(const CacheAttn& a, cudaStream_t s) {
+    return a.list ? attention_go<KT, HD, NT, true>(a, s) : attention_go<KT, HD, NT, false>(a, s);
+}
+template <typename KT> cudaError_t attention_type(const CacheAttn& a, cudaStream_t s) {
+    const int nt = cache_tile_rows(a.hd, a.R) / 8;
+    switch (cache_tile_dims(a.hd)) {
+        case 64:
+            return nt == 1 ? attention_form<KT, 64, 1>(a, s) : nt == 2 ? attention_form<KT, 64, 2>(a, s)
+                                                                      : attention_form<KT, 64, 4>(a, s);
+        case 128:
+            return nt == 1 ? attention_form<KT, 128, 1>(a, s) : nt == 2 ? attention_form<KT, 128, 2>(a, s)
+                                                                       : attention_form<KT, 128, 4>(a, s);
+        default:
+            return nt == 1 ? attention_form<KT, 256, 1>(a, s) : attention_form<KT, 256, 2>(a, s);
+    }
+}
+
+}  // namespace
+
+int cache_tile_dims(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+
+// Query rows of a tile: the fewest multiples of 8 that hold the problem's rows, up to what the accumulators of a
+// warp (head_dim x rows f32) leave of the registers.
+int cache_tile_rows(int hd, int R) {
+    const int most = cache_tile_dims(hd) == 256 ? 16 : 32;
+    return R <= 8 ? 8 : R <= 16 ? 16 : most;
+}
+
+// Splits of the cache's chunks: one CTA per SM over all problems and row tiles, but not more than leave every
+// warp of a CTA a chunk.
+int cache_splits(int hd, int problems, int row_tiles, int n_chunks) {
+    const int w = cache_tile_dims(hd) == 256 ? 4 : 8;
+    const int most = KV_SMS / (problems * row_tiles);
+    const int useful = (n_chunks + w - 1) / w;
+    return most < 1 ? 1 : most < useful ? most : useful < 1 ? 1 : useful;
+}
+
+cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s) {
+    cudaError_t e = a.bf16 ? attention_type<__nv_bfloat16>(a, s) : attention_type<__half>(a, s);
+    if (e != cudaSuccess || (a.splits == 1 && !a.logits)) return e;
+    const int rows = a.n_past_dev ? a.max_rows : a.n_past + a.m;
+    const int per = (rows + ACC_ROWS - 1) / ACC_ROWS;                  // accumulating CTAs of a KV head
+    return launch_pdl(k_cache_combine, dim3((unsigned)(a.problems * a.R + (a.logits ? a.n_kv * per : 0))), CB, 0, s, a,
+                      cache_tile_rows(a.hd, a.R), cache_tile_dims(a.hd), per);
+}
+
+}  // namespace hoard

@@ -1,0 +1,82 @@
+// kernels_cache.h -- launch interface of the cache operators (kernels_cache.cu, kernels_cache_select.cu),
+// called by cache_api.cpp after its argument checks.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace hoard {
+
+constexpr int KV_SMS = 148;              // B200: one split CTA per SM
+constexpr int KV_CHUNK = 16;             // rows of one step of a warp (the M of m16n8k16)
+
+// The cache and the query side of one attention call. Strides in elements (caches) and floats (q, gate).
+struct CacheAttn {
+    const float* q;
+    int64_t q_ts, q_hs;
+    const void *kc, *vc;
+    int64_t rs, hs;
+    const uint64_t* vis;
+    const float* gate;
+    int64_t gate_ts, gate_hs;
+    float* out;
+    int n_head, n_kv, g, hd, m, n_past, max_rows;
+    const int32_t* n_past_dev;
+    bool bf16;
+    float scale_log2;                    // scale * log2(e): scores are kept in units of log2
+    // A problem is the set of query rows that read the same cache rows: a KV head with the R = m * g rows of
+    // its query heads, or with a block list a (token, KV head) with R = g.
+    int problems, R, row_tiles, splits;
+    // partial results of each (problem, row tile, split): unnormalised sums, running maxima and totals
+    float* part_o;                       // [problems * row_tiles][splits][tile rows][tile dims]
+    float2* part_ml;                     // [problems * row_tiles][splits][tile rows]
+    float* logits;                       // optional [n_kv][R][logits_ld], in log2 units
+    int64_t logits_ld;
+    float* acc;                          // optional [n_kv][max_rows]
+    // block lists (sparse form): ascending block ids of each problem, and their number
+    const int32_t* list;
+    const int32_t* list_n;
+    int list_cap, block;
+};
+
+// Rows of a query tile, dims of the instantiation that runs a call, and split counts.
+int cache_tile_rows(int hd, int R);
+int cache_tile_dims(int hd);
+int cache_splits(int hd, int problems, int row_tiles, int n_chunks);
+cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s);
+
+struct CacheEvict {
+    void *kc, *vc;
+    int64_t rs, hs;
+    const float* acc;
+    const int32_t* pos;
+    float* acc_out;
+    int32_t* pos_out;
+    int n_kv, hd, max_rows, n_rows, n_keep, n_sink, recent_from;
+    int32_t *to, *from, *n_moves;        // [n_kv][max_rows] twice, [n_kv]
+};
+cudaError_t launch_cache_evict(const CacheEvict& e, cudaStream_t s);
+
+cudaError_t launch_cache_bounds(const void* kc, int64_t rs, int64_t hs, bool bf16, int n_kv, int hd, int max_rows,
+                                int block, int row0, int row1, const int32_t* row1_dev, void* bounds, cudaStream_t s);
+
+// Scores of the candidate blocks, their selection, and the ascending lists that launch_cache_attention reads.
+struct CacheSelect {
+    const float* q;
+    int64_t q_ts, q_hs;
+    const void* bounds;
+    bool bf16;
+    int n_head, n_kv, g, hd, m, n_past, max_rows, block, n_sink, n_local, n_sel;
+    const int32_t* n_past_dev;
+    double* u;                           // [n_kv][m * g][nb_cap]
+    int32_t *list, *list_n, *sel_out;
+    int list_cap;
+};
+cudaError_t launch_cache_select(const CacheSelect& c, cudaStream_t s);
+
+struct TakePath {
+    int32_t row[64];
+};
+cudaError_t launch_cache_take(void* kc, void* vc, int64_t rs, int64_t hs, int n_kv, int hd, int row0,
+                              const TakePath& path, int n, cudaStream_t s);
+
+}  // namespace hoard

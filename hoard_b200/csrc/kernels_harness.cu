@@ -383,26 +383,15 @@ __global__ void __launch_bounds__(256) k_qgemv_set(GemvSet g, int K, const int8_
 // ---- fused QK RMSNorm (mode 1: over the whole projection, weights [n*hd]; mode 2: per head, weights
 //      [hd]; 0: none) + NEOX RoPE + KV store: one CTA per q or k head, one thread per rotated pair.
 //      Rotated q goes to q_out (mode 1 reads the whole input vector in every CTA); rotated k and v
-//      go to the caches ----
+//      go to the caches. `vec`: the token's q or k vector, xh: this head's values in it; q_out, kc, vc:
+//      the head's destinations (kc, vc null: not stored) ----
 template <typename KT>
-__global__ void __launch_bounds__(128) k_qknorm_rope_store(const float* __restrict__ q, const float* __restrict__ k,
-                                                           const float* __restrict__ v, const float* __restrict__ qn,
-                                                           const float* __restrict__ kn, int mode, float eps,
-                                                           int n_head, int n_kv, int hd, int q_stride, int rope_dim,
-                                                           int pos, const int32_t* __restrict__ pos_dev, int max_ctx,
-                                                           float theta_scale, float* __restrict__ q_out,
-                                                           KT* __restrict__ kc, KT* __restrict__ vc) {
-    pdl_enter();
+__device__ __forceinline__ void qknorm_rope_head(const float* __restrict__ vec, int nvec, const float* __restrict__ xh,
+                                                 const float* __restrict__ vh, const float* __restrict__ wn, int hh,
+                                                 bool isq, int mode, float eps, int hd, int rope_dim, int pos,
+                                                 float theta_scale, float* __restrict__ q_out, KT* __restrict__ kc,
+                                                 KT* __restrict__ vc) {
     __shared__ double redd[32];
-    if (pos_dev) pos = *pos_dev;
-    if (pos < 0 || pos >= max_ctx) return;
-    const int head = blockIdx.x;
-    const bool isq = head < n_head;
-    const int hh = isq ? head : head - n_head;
-    const float* vec = isq ? q : k;
-    const int nvec = (isq ? n_head : n_kv) * hd;
-    const float* wn = isq ? qn : kn;
-    const float* xh = vec + (int64_t)hh * (isq ? q_stride : hd);
     const int rh = rope_dim / 2;
     float scale = 1.f;
     if (mode != 0) {
@@ -417,12 +406,8 @@ __global__ void __launch_bounds__(128) k_qknorm_rope_store(const float* __restri
         return x;
     };
     auto put = [&](int j, float r) {
-        if (isq) {
-            q_out[(int64_t)hh * hd + j] = r;
-        } else {
-            const int64_t o = ((int64_t)pos * n_kv + hh) * hd;
-            kv_put(kc + o + j, r);
-        }
+        if (isq) q_out[j] = r;
+        else if (kc) kv_put(kc + j, r);
     };
     // NEOX rotation of the first rope_dim values (pairs j, j + rope_dim/2, theta_j = pos * base^(-2j/rope_dim));
     // values past rope_dim pass through
@@ -437,10 +422,60 @@ __global__ void __launch_bounds__(128) k_qknorm_rope_store(const float* __restri
         } else if (j >= rope_dim) {
             put(j, normed(j));
         }
-        if (!isq) {
-            const int64_t o = ((int64_t)pos * n_kv + hh) * hd;
-            kv_put(vc + o + j, v[(int64_t)hh * hd + j]);
-        }
+        if (!isq && vc) kv_put(vc + j, vh[j]);
+    }
+}
+
+template <typename KT>
+__global__ void __launch_bounds__(128) k_qknorm_rope_store(const float* __restrict__ q, const float* __restrict__ k,
+                                                           const float* __restrict__ v, const float* __restrict__ qn,
+                                                           const float* __restrict__ kn, int mode, float eps,
+                                                           int n_head, int n_kv, int hd, int q_stride, int rope_dim,
+                                                           int pos, const int32_t* __restrict__ pos_dev, int max_ctx,
+                                                           float theta_scale, float* __restrict__ q_out,
+                                                           KT* __restrict__ kc, KT* __restrict__ vc) {
+    pdl_enter();
+    if (pos_dev) pos = *pos_dev;
+    if (pos < 0 || pos >= max_ctx) return;
+    const bool isq = (int)blockIdx.x < n_head;
+    const int hh = isq ? blockIdx.x : blockIdx.x - n_head;
+    const float* vec = isq ? q : k;
+    const int64_t o = ((int64_t)pos * n_kv + hh) * hd;
+    qknorm_rope_head<KT>(vec, (isq ? n_head : n_kv) * hd, vec + (int64_t)hh * (isq ? q_stride : hd),
+                         v + (int64_t)hh * hd, isq ? qn : kn, hh, isq, mode, eps, hd, rope_dim, pos, theta_scale,
+                         q_out + (int64_t)hh * hd, kc + o, vc + o);
+}
+
+// ---- the same for several tokens whose cache rows need not be their positions: CTA (head, token). A stored
+//      row starts with accumulated weight 0 and its position (both optional, [n_kv][max_rows]) ----
+template <typename KT>
+__global__ void __launch_bounds__(128) k_qknorm_rope_store_rows(const float* __restrict__ q, int64_t q_ts, int64_t q_hs,
+                                                                const float* __restrict__ k,
+                                                                const float* __restrict__ v,
+                                                                const float* __restrict__ qn,
+                                                                const float* __restrict__ kn, int mode, float eps,
+                                                                int n_head, int n_kv, int hd, int rope_dim,
+                                                                const int32_t* __restrict__ pos, int row0,
+                                                                const int32_t* __restrict__ row0_dev, int max_rows,
+                                                                float theta_scale, float* __restrict__ q_out,
+                                                                KT* __restrict__ kc, KT* __restrict__ vc, int64_t rs,
+                                                                int64_t hs, float* __restrict__ acc,
+                                                                int32_t* __restrict__ row_pos) {
+    pdl_enter();
+    const int t = blockIdx.y;
+    const int64_t row = (int64_t)(row0_dev ? *row0_dev : row0) + t;
+    const bool isq = (int)blockIdx.x < n_head, stored = row >= 0 && row < max_rows;
+    const int hh = isq ? blockIdx.x : blockIdx.x - n_head, p = pos[t];
+    if (!isq && !stored) return;
+    const float* vec = isq ? q + t * q_ts : k + (int64_t)t * n_kv * hd;
+    KT* kr = isq ? nullptr : kc + row * rs + hh * hs;
+    KT* vr = isq ? nullptr : vc + row * rs + hh * hs;
+    qknorm_rope_head<KT>(vec, (isq ? n_head : n_kv) * hd, vec + hh * (isq ? q_hs : (int64_t)hd),
+                         v + ((int64_t)t * n_kv + hh) * hd, isq ? qn : kn, hh, isq, mode, eps, hd, rope_dim, p,
+                         theta_scale, q_out + ((int64_t)t * n_head + hh) * hd, kr, vr);
+    if (!isq && threadIdx.x == 0) {
+        if (acc) acc[(int64_t)hh * max_rows + row] = 0.f;
+        if (row_pos) row_pos[(int64_t)hh * max_rows + row] = p;
     }
 }
 
@@ -548,6 +583,23 @@ cudaError_t launch_qknorm_rope_store(const float* q, const float* k, const float
                           (__nv_bfloat16*)kc, (__nv_bfloat16*)vc);
     return launch_pdl(k_qknorm_rope_store<__half>, n_head + n_kv, 128, 0, s, q, k, v, qn, kn, mode, eps, n_head, n_kv,
                       hd, q_stride, rope_dim, pos, pos_dev, max_ctx, theta_scale, q_out, (__half*)kc, (__half*)vc);
+}
+
+cudaError_t launch_qknorm_rope_store_rows(const float* q, int64_t q_ts, int64_t q_hs, const float* k, const float* v,
+                                          const float* qn, const float* kn, int mode, float eps, int n_head, int n_kv,
+                                          int hd, int rope_dim, const int32_t* pos, int m, int row0,
+                                          const int32_t* row0_dev, int max_rows, float freq_base, float* q_out, void* kc,
+                                          void* vc, int64_t rs, int64_t hs, bool kv_bf16, float* acc, int32_t* row_pos,
+                                          cudaStream_t s) {
+    const float theta_scale = powf(freq_base, -2.0f / (float)rope_dim);
+    const dim3 grid(n_head + n_kv, m);
+    if (kv_bf16)
+        return launch_pdl(k_qknorm_rope_store_rows<__nv_bfloat16>, grid, 128, 0, s, q, q_ts, q_hs, k, v, qn, kn, mode,
+                          eps, n_head, n_kv, hd, rope_dim, pos, row0, row0_dev, max_rows, theta_scale, q_out,
+                          (__nv_bfloat16*)kc, (__nv_bfloat16*)vc, rs, hs, acc, row_pos);
+    return launch_pdl(k_qknorm_rope_store_rows<__half>, grid, 128, 0, s, q, q_ts, q_hs, k, v, qn, kn, mode, eps, n_head,
+                      n_kv, hd, rope_dim, pos, row0, row0_dev, max_rows, theta_scale, q_out, (__half*)kc, (__half*)vc,
+                      rs, hs, acc, row_pos);
 }
 
 cudaError_t launch_embed(int type, const uint8_t* table, int H, int64_t n_vocab, const int32_t* token,
