@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -29,14 +30,10 @@ class Desc(ctypes.Structure):
                 ("head_stride", ctypes.c_int64), ("scale", ctypes.c_float)]
 
 
-class Query(ctypes.Structure):
-    """hoard_kv_query"""
-    _fields_ = [("q", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
-                ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p), ("visible", ctypes.c_void_p),
-                ("gate", ctypes.c_void_p), ("gate_token_stride", ctypes.c_int64), ("gate_head_stride", ctypes.c_int64),
-                ("out", ctypes.c_void_p), ("m", ctypes.c_int), ("n_past", ctypes.c_int), ("n_past_dev", ctypes.c_void_p)]
-
-
+# hoard_kv_query: q and its token and head strides, k_cache, v_cache, visible, gate and its strides, out, m, n_past,
+# n_past_dev
+_QUERY = struct.Struct("@PqqPPPPqqPiiP")
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _bound = False
 
 
@@ -91,24 +88,25 @@ class CacheOps:
         self.max_rows, self.max_tokens, self.block = max_rows, max_tokens, block
         self._d = Desc(n_head, n_head_kv, head_dim, KV_TYPES[kv_dtype], max_rows, max_tokens, max_acc_tokens, block, 0, 0,
                        1.0 / math.sqrt(head_dim) if scale is None else scale)
-        self._q = Query()
+        self._q = ctypes.create_string_buffer(_QUERY.size)
         self._dp, self._qp = ctypes.addressof(self._d), ctypes.addressof(self._q)
+        self._cache_shape, self._cache_stride = (max_rows, n_head_kv, head_dim), None
         n = _kv().hoard_kv_ws_bytes(self._dp)
         if n < 0:
             raise HoardError(-1, "hoard_kv_ws_bytes: descriptor refused")
         self.device = torch.cuda.current_device() if device is None else device
-        self._dev = torch.device("cuda", self.device)
-        self._ws = torch.empty(n, dtype=torch.uint8, device=self._dev)
+        self._ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", self.device))
         self._wsp = self._ws.data_ptr()
 
     # ---- plumbing ----
+    # The checks read each attribute of a tensor once: at the sizes of a decode step they are a good part of a call.
     def _run(self, fn, stream, *args):
         """fn(*args, stream) on this object's device."""
         if torch.cuda.current_device() != self.device:
             with torch.cuda.device(self.device):
                 return self._run(fn, stream, *args)
         if stream is None:
-            stream = torch.cuda.current_stream().cuda_stream
+            stream = _raw_stream(self.device)
         elif hasattr(stream, "cuda_stream"):
             stream = stream.cuda_stream
         rc = fn(*args, stream)
@@ -117,52 +115,46 @@ class CacheOps:
 
     def _caches(self, k_cache, v_cache=None):
         """Checks the caches and sets the descriptor's strides to theirs."""
-        shape = (self.max_rows, self.n_head_kv, self.head_dim)
-        if k_cache.shape != shape or k_cache.dtype != self.kv_dtype or k_cache.device != self._dev:
-            raise ValueError(f"caches are {list(shape)} {self.kv_dtype} tensors on {self._dev}")
-        s = k_cache.stride()
-        if s[2] != 1 and self.head_dim != 1:
-            raise ValueError("the values of a head are contiguous")
-        if v_cache is not None and (v_cache.shape != shape or v_cache.dtype != self.kv_dtype or v_cache.device != self._dev
-                                    or v_cache.stride() != s):
+        s, dev = k_cache.stride(), self.device
+        if (k_cache.shape != self._cache_shape or k_cache.dtype is not self.kv_dtype or k_cache.get_device() != dev
+                or s[2] != 1):
+            raise ValueError(f"caches are {list(self._cache_shape)} {self.kv_dtype} tensors on device {dev} with "
+                             "contiguous heads")
+        if v_cache is not None and (v_cache.shape != self._cache_shape or v_cache.dtype is not self.kv_dtype
+                                    or v_cache.get_device() != dev or v_cache.stride() != s):
             raise ValueError("the V cache has the K cache's shape, type, device and strides")
-        self._d.row_stride, self._d.head_stride = s[0], s[1]
+        if s != self._cache_stride:
+            self._d.row_stride, self._d.head_stride = s[0], s[1]
+            self._cache_stride = s
 
-    def _f32(self, x, shape, what):
-        if x.shape != shape or x.dtype != torch.float32 or x.device != self._dev:
-            raise ValueError(f"{what} is a {list(shape)} float32 tensor on {self._dev}")
-        return x
+    def _heads(self, x, shape, what):
+        """Strides of a float32 [m][n_head][head_dim] tensor with contiguous heads."""
+        s = x.stride()
+        if x.shape != shape or x.dtype is not torch.float32 or x.get_device() != self.device or s[2] != 1:
+            raise ValueError(f"{what} is a {list(shape)} float32 tensor on device {self.device} with contiguous heads")
+        return s
 
     def _contiguous(self, x, shape, dtype, what):
-        if x.shape != shape or x.dtype != dtype or x.device != self._dev or not x.is_contiguous():
-            raise ValueError(f"{what} is a contiguous {list(shape)} {dtype} tensor on {self._dev}")
+        if x.shape != shape or x.dtype is not dtype or x.get_device() != self.device or not x.is_contiguous():
+            raise ValueError(f"{what} is a contiguous {list(shape)} {dtype} tensor on device {self.device}")
         return x.data_ptr()
 
     def _query(self, q, k_cache, v_cache, n_past, vis, gate, out, n_past_dev):
-        m = q.shape[0]
+        m = len(q)
         shape = (m, self.n_head, self.head_dim)
-        self._f32(q, shape, "q")
-        if q.stride(2) != 1:
-            raise ValueError("the values of a q head are contiguous")
+        qs = self._heads(q, shape, "q")
         self._caches(k_cache, v_cache)
-        a = self._q
-        a.q, a.q_token_stride, a.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
-        a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-        a.visible = None if vis is None else self._contiguous(vis, (m,), torch.int64, "vis")
         if gate is None:
-            a.gate = None
+            gp, gs = 0, (0, 0)
         else:
-            self._f32(gate, shape, "gate")
-            if gate.stride(2) != 1:
-                raise ValueError("the values of a gate head are contiguous")
-            a.gate, a.gate_token_stride, a.gate_head_stride = gate.data_ptr(), gate.stride(0), gate.stride(1)
+            gs = self._heads(gate, shape, "gate")
+            gp = gate.data_ptr()
         if out is None:
-            out = torch.empty(shape, dtype=torch.float32, device=self._dev)
-            a.out = out.data_ptr()
-        else:
-            a.out = self._contiguous(out, shape, torch.float32, "out")
-        a.m, a.n_past = m, n_past
-        a.n_past_dev = None if n_past_dev is None else self._contiguous(n_past_dev, (1,), torch.int32, "n_past_dev")
+            out = torch.empty(shape, dtype=torch.float32, device=q.device)
+        _QUERY.pack_into(self._q, 0, q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(),
+                         0 if vis is None else self._contiguous(vis, (m,), torch.int64, "vis"), gp, gs[0], gs[1],
+                         self._contiguous(out, shape, torch.float32, "out"), m, n_past,
+                         0 if n_past_dev is None else self._contiguous(n_past_dev, (1,), torch.int32, "n_past_dev"))
         return out
 
     # ---- attention ----
@@ -233,13 +225,11 @@ class CacheOps:
         their k, v [m][n_head_kv][head_dim] into cache rows row0.. (row0_dev: in device memory). Returns the rotated q."""
         m = q.shape[0]
         shape, kshape = (m, self.n_head, self.head_dim), (m, self.n_head_kv, self.head_dim)
-        self._f32(q, shape, "q")
-        if q.stride(2) != 1:
-            raise ValueError("the values of a q head are contiguous")
+        qs = self._heads(q, shape, "q")
         self._caches(k_cache, v_cache)
         kp, vp = (self._contiguous(x, kshape, torch.float32, w) for x, w in ((k, "k"), (v, "v")))
         if q_out is None:
-            q_out = torch.empty(shape, dtype=torch.float32, device=self._dev)
+            q_out = torch.empty(shape, dtype=torch.float32, device=q.device)
         qo = self._contiguous(q_out, shape, torch.float32, "q_out")
         if mode in (1, 2):
             full = mode == 1
@@ -252,7 +242,7 @@ class CacheOps:
         side = (self.n_head_kv, self.max_rows)
         ap = None if acc is None else self._contiguous(acc, side, torch.float32, "acc")
         rp = None if row_pos is None else self._contiguous(row_pos, side, torch.int32, "row_pos")
-        self._run(_kv().hoard_kv_store, stream, self._dp, q.data_ptr(), q.stride(0), q.stride(1), kp, vp, _ptr(q_norm),
+        self._run(_kv().hoard_kv_store, stream, self._dp, q.data_ptr(), qs[0], qs[1], kp, vp, _ptr(q_norm),
                   _ptr(k_norm), mode, eps, self.head_dim if rope_dim is None else rope_dim, freq_base, pp, m, row0, rd, qo,
                   k_cache.data_ptr(), v_cache.data_ptr(), ap, rp)
         return q_out

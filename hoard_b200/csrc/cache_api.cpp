@@ -50,7 +50,7 @@ bool desc_ok(const hoard_kv_desc* d) {
 // The workspace: the splits' partial results, the logits that accumulation needs, and the block operators'
 // scores and lists; an eviction's lists take the same bytes, no call needs both.
 struct Ws {
-    int64_t part_o, part_ml, logits, u, list, list_n, attn_end;
+    int64_t part_o, part_ml, logits, u, u_top, list, list_n, attn_end;
     int64_t to, from, n_moves, evict_end;
     int64_t logits_ld;
     int list_cap;
@@ -78,6 +78,7 @@ Ws ws_plan(const hoard_kv_desc* d) {
     if (d->block) {
         w.list_cap = (int)ceil_div(d->max_rows, d->block);
         w.u = take((int64_t)d->max_tokens * d->n_head * (d->max_rows / d->block) * 8);
+        w.u_top = take((int64_t)d->max_tokens * d->n_head * ceil_div(d->max_rows / d->block, 32) * 8);
         w.list = take((int64_t)d->max_tokens * d->n_head_kv * w.list_cap * 4);
         w.list_n = take((int64_t)d->max_tokens * d->n_head_kv * 4);
     }
@@ -230,6 +231,7 @@ int hoard_kv_block_attention(const hoard_kv_desc* d, const hoard_kv_query* a, co
     s.n_sel = n_sel;
     s.n_past_dev = c.n_past_dev;
     s.u = reinterpret_cast<double*>(b + w.u);
+    s.u_top = reinterpret_cast<double*>(b + w.u_top);
     s.list = reinterpret_cast<int32_t*>(b + w.list);
     s.list_n = reinterpret_cast<int32_t*>(b + w.list_n);
     s.list_cap = w.list_cap;

@@ -165,21 +165,32 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
         cp_async_commit();
     }
 
-    // the tile's q rows as fragments of the B operand: [K step][8-row tile][term][lane] of 8 bytes
-    for (int r = warp; r < RT; r += W) {
-        const int row = tile * RT + r;                 // row = (token - t0) * g + head of the KV head
+    // the tile's q rows as fragments of the B operand: [K step][8-row tile][term][lane] of 8 bytes. A warp takes
+    // every W-th row and loads all of them before it uses the first
+    constexpr int QR = RT / W;
+    float x[QR][HD / 32];
+#pragma unroll
+    for (int i = 0; i < QR; ++i) {
+        const int row = tile * RT + warp + i * W;      // row = (token - t0) * g + head of the KV head
         const bool live = row < a.R;
         const int t = t0 + (live ? row / a.g : 0), h = kv * a.g + (live ? row % a.g : 0);
         const float* q = a.q + t * a.q_ts + h * a.q_hs;
-        float x[HD / 32];
+#pragma unroll
+        for (int k = 0; k < HD / 32; ++k) x[i][k] = live && k * 32 + lane < a.hd ? q[k * 32 + lane] : 0.f;
+    }
+    if (tid < RT) {
+        const int row = tile * RT + tid, t = t0 + row / a.g;
+        s_vis[tid] = row >= a.R ? 0 : a.vis ? a.vis[t] : t >= 63 ? ~0ull : (1ull << (t + 1)) - 1;
+    }
+#pragma unroll
+    for (int i = 0; i < QR; ++i) {
+        const int r = warp + i * W;
         float am = 0.f;
         bool bad = false;
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-            const int d = i * 32 + lane;
-            x[i] = live && d < a.hd ? q[d] : 0.f;
-            bad |= !(fabsf(x[i]) <= 3.4e38f);
-            am = fmaxf(am, fabsf(x[i]));
+        for (int k = 0; k < HD / 32; ++k) {
+            bad |= !(fabsf(x[i][k]) <= 3.4e38f);
+            am = fmaxf(am, fabsf(x[i][k]));
         }
         am = warp_max(am);
         bad = __any_sync(0xffffffffu, bad);
@@ -187,18 +198,13 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
         int e = (int)(__float_as_uint(am) >> 23) - 127;
         e = bad || am == 0.f ? Terms<KT>::Q_EXP : max(e, -100);
         const float up = __uint_as_float((uint32_t)(127 + Terms<KT>::Q_EXP - e) << 23);
-        if (lane == 0) {
-            s_scale[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - Terms<KT>::Q_EXP + e) << 23);
-            uint64_t own = 0;
-            if (live) own = a.vis ? a.vis[t] : (t >= 63 ? ~0ull : (1ull << (t + 1)) - 1);
-            s_vis[r] = own;
-        }
+        if (lane == 0) s_scale[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - Terms<KT>::Q_EXP + e) << 23);
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
+        for (int k = 0; k < HD / 32; ++k) {
             // lanes 2c, 2c + 1 hold the pair of dims that one fragment register packs
-            float lo = x[i] * up;
+            float lo = x[i][k] * up;
             float hi = __shfl_down_sync(0xffffffffu, lo, 1);
-            const int d = i * 32 + lane, kk = d >> 4, reg = (d >> 3) & 1, c = (d & 7) >> 1;
+            const int d = k * 32 + lane, kk = d >> 4, reg = (d >> 3) & 1, c = (d & 7) >> 1;
 #pragma unroll
             for (int u = 0; u < TN; ++u) {
                 const uint32_t w = take_term<KT>(lo, hi);
@@ -241,7 +247,8 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
             cp_async_commit();
         }
         const unsigned ks = ring + stage * Plan<HD>::STAGE, vs = ks + KV_CHUNK * PITCH;
-        // ---- S^T = K q^T ----
+        // ---- S^T = K q^T: each K step's products by matrix instructions, added with rounding (the instructions
+        // truncate as they accumulate), which also leaves no chain of instructions longer than the terms ----
         float s[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -253,11 +260,16 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
             ldm4(af, ks + k_r * PITCH + (((2 * k + k_c) ^ (k_r & 7)) << 4));
 #pragma unroll
             for (int n = 0; n < NT; ++n)
+            {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int u = 0; u < TN; ++u) {
+                for (int u = TN - 1; u >= 0; --u) {
                     const uint2 b = *reinterpret_cast<const uint2*>(qf + ((((k * NT + n) * TN + u) * 32) + lane) * 2);
-                    mma16816<KT>(s[n], af, b.x, b.y);
+                    mma16816<KT>(x, af, b.x, b.y);
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] += x[i];
+            }
         }
         // ---- scores in log2 units; masked ones -inf ----
         const int row0 = chunk_row(c), left = chunk_end(c) - row0;               // rows of the chunk that exist
@@ -357,15 +369,20 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
                     pf[n][u][1] = transpose8(take_term<KT>(r[2], r[3]));
                 }
             }
-            // ---- O^T += V^T P^T ----
+            // ---- O^T += V^T P^T, added likewise: left in the instructions' accumulators over 8192 rows the sums
+            // were 2e-5 off ----
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t af[4];
                 ldm4t(af, vs + v_r * PITCH + (((2 * k + v_c) ^ (v_r & 7)) << 4));
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
+                    float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int u = 0; u < TN; ++u) mma16816<KT>(o[k][n], af, pf[n][u][0], pf[n][u][1]);
+                    for (int u = TN - 1; u >= 0; --u) mma16816<KT>(x, af, pf[n][u][0], pf[n][u][1]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[k][n][i] += x[i];
+                }
             }
         } else {
             for (int j = 0; j < KV_CHUNK; ++j) {
@@ -470,41 +487,59 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
 }
 
 // ---- joins the splits of every query row, and with acc adds the rows' weights to the accumulated ones -------
-// A CTA of 128 threads per query row (token, head): factors 2^(m_s - M) of the splits, then float4 columns x
-// split groups. The CTAs after them take 512 cache rows of a KV head each: w = sum over the head's query rows
-// of 2^(s - M) / L in row order, one thread per cache row.
-constexpr int CB = 128, ACC_ROWS = 512, ACC_MAX_R = 512;
+// A CTA per query row (token, head): the factors 2^(m_s - M) of the splits, one split per thread, then float4
+// columns x split groups, eight partial rows in flight per thread. The CTAs after them take 256 cache rows of a KV
+// head each: w = sum over the head's query rows of 2^(s - M) / L in row order, one thread per cache row.
+constexpr int CB = 256, ACC_ROWS = CB, ACC_MAX_R = 512;
+static_assert(KV_SMS <= CB, "one split per thread");
 __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int rt, int hdt, int per) {
     pdl_enter();
-    __shared__ float s_f[KV_SMS];
+    __shared__ float s_f[CB];
+    __shared__ float s_red[2][CB / 32];
     __shared__ float4 s_o[CB];
     __shared__ float s_mr[ACC_MAX_R], s_ir[ACC_MAX_R];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n_rows = a.problems * a.R;
     if ((int)blockIdx.x < n_rows) {
         const int prob = blockIdx.x / a.R, row = blockIdx.x - prob * a.R;
         const int tile = row / rt, r = row - tile * rt;
         const int64_t part = ((int64_t)prob * a.row_tiles + tile) * a.splits;
-        float top = -INFINITY;
-        for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[(part + s) * rt + r].x);
-        for (int s = tid; s < a.splits; s += CB) {
-            const float ms = a.part_ml[(part + s) * rt + r].x;
-            s_f[s] = ms == -INFINITY ? 0.f : ex2(ms - top);
-        }
+        const float2 ml = tid < a.splits ? a.part_ml[(part + tid) * rt + r] : make_float2(-INFINITY, 0.f);
+        const float wm = warp_max(ml.x);
+        if (lane == 0) s_red[0][warp] = wm;
         __syncthreads();
-        float l = 0.f;
-        for (int s = 0; s < a.splits; ++s) l += s_f[s] == 0.f ? 0.f : s_f[s] * a.part_ml[(part + s) * rt + r].y;
+        float top = s_red[0][0];
+#pragma unroll
+        for (int w = 1; w < CB / 32; ++w) top = fmaxf(top, s_red[0][w]);
+        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+        s_f[tid] = f;
+        const float wl = warp_sum(ml.x == -INFINITY ? 0.f : f * ml.y);
+        if (lane == 0) s_red[1][warp] = wl;
+        __syncthreads();
+        float l = s_red[1][0];
+#pragma unroll
+        for (int w = 1; w < CB / 32; ++w) l += s_red[1][w];
         const int v4 = a.hd / 4, groups = CB / v4, gi = tid / v4, c = tid - gi * v4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (gi < groups) {
-            for (int s = gi; s < a.splits; s += groups) {
-                const float f = s_f[s];
-                if (f != 0.f) {
-                    const float4 u = *reinterpret_cast<const float4*>(a.part_o + ((part + s) * rt + r) * hdt + 4 * c);
-                    v.x += f * u.x;
-                    v.y += f * u.y;
-                    v.z += f * u.z;
-                    v.w += f * u.w;
+            const float* po = a.part_o + (part * rt + r) * hdt + 4 * c;
+            for (int s0 = gi; s0 < a.splits; s0 += 8 * groups) {
+                float4 u[8];
+                float w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int s = s0 + k * groups;
+                    w[k] = s < a.splits ? s_f[s] : 0.f;
+                    // a split that saw nothing has left zeros
+                    if (s < a.splits) u[k] = *reinterpret_cast<const float4*>(po + (int64_t)s * rt * hdt);
+                    else u[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    v.x += w[k] * u[k].x;
+                    v.y += w[k] * u[k].y;
+                    v.z += w[k] * u[k].z;
+                    v.w += w[k] * u[k].w;
                 }
             }
             s_o[tid] = v;
@@ -536,36 +571,51 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int rt,
     }
     // accumulation
     const int n = past_rows(a) + a.m;
-    const int x = blockIdx.x - n_rows, kv = x / per, j0 = (x - kv * per) * ACC_ROWS;
-    if (j0 >= n) return;
-    for (int row = tid; row < a.R; row += CB) {
+    const int x = blockIdx.x - n_rows, kv = x / per, j = (x - kv * per) * ACC_ROWS + tid;
+    if (j - tid >= n) return;
+    const float* lg = a.logits + (int64_t)kv * a.R * a.logits_ld + min(j, n - 1);
+    float* acc = a.acc + (int64_t)kv * a.max_rows + min(j, n - 1);
+    const float before = *acc;
+    // a warp per query row: its maximum and total over the splits
+    for (int row = warp; row < a.R; row += CB / 32) {
         const int tile = row / rt, r = row - tile * rt;
-        const int64_t part = ((int64_t)kv * a.row_tiles + tile) * a.splits;
+        const float2* ml = a.part_ml + ((int64_t)kv * a.row_tiles + tile) * a.splits * rt + r;
+        float2 v[(KV_SMS + 31) / 32];
         float top = -INFINITY, l = 0.f;
-        for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[(part + s) * rt + r].x);
-        for (int s = 0; s < a.splits; ++s) {
-            const float2 ml = a.part_ml[(part + s) * rt + r];
-            l += ml.x == -INFINITY ? 0.f : ex2(ml.x - top) * ml.y;
+#pragma unroll
+        for (int k = 0; k < (KV_SMS + 31) / 32; ++k) {
+            const int s = lane + 32 * k;
+            v[k] = s < a.splits ? ml[(int64_t)s * rt] : make_float2(-INFINITY, 0.f);
+            top = fmaxf(top, v[k].x);
         }
-        s_mr[row] = top;
-        s_ir[row] = l == 0.f ? 0.f : 1.f / l;
+        top = warp_max(top);
+#pragma unroll
+        for (int k = 0; k < (KV_SMS + 31) / 32; ++k) l += v[k].x == -INFINITY ? 0.f : ex2(v[k].x - top) * v[k].y;
+        l = warp_sum(l);
+        if (lane == 0) {
+            s_mr[row] = top;
+            s_ir[row] = l == 0.f ? 0.f : 1.f / l;
+        }
     }
     __syncthreads();
     const float pe = a.bf16 ? Terms<__nv_bfloat16>::P_EXP : Terms<__half>::P_EXP;      // l holds 2^P_EXP sum p
-    for (int j = j0 + tid; j < min(n, j0 + ACC_ROWS); j += CB) {
-        const float* lg = a.logits + (int64_t)kv * a.R * a.logits_ld + j;
-        float w = 0.f;
-        for (int row = 0; row < a.R; ++row)
-            if (s_ir[row] != 0.f) w += ex2(lg[row * a.logits_ld] - (s_mr[row] - pe)) * s_ir[row];
-        a.acc[(int64_t)kv * a.max_rows + j] += w;
+    float w = 0.f;
+    for (int r0 = 0; r0 < a.R; r0 += 8) {
+        float s[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] = r0 + k < a.R ? lg[(r0 + k) * a.logits_ld] : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (r0 + k < a.R && s_ir[r0 + k] != 0.f) w += ex2(s[k] - (s_mr[r0 + k] - pe)) * s_ir[r0 + k];
     }
+    if (j < n) *acc = before + w;
 }
 
 template <typename KT, int HD, int NT, bool BLOCKS>
 cudaError_t attention_go(const CacheAttn& a, cudaStream_t s) {
     constexpr int smem = attn_smem<KT, HD, NT>();
-    cudaError_t e = cudaFuncSetAttribute(k_cache_attention<KT, HD, NT, BLOCKS>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static SmemLimit limit;
+    cudaError_t e = limit.raise((const void*)k_cache_attention<KT, HD, NT, BLOCKS>, smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(k_cache_attention<KT, HD, NT, BLOCKS>, dim3(a.splits, a.row_tiles, a.problems), Plan<HD>::W * 32,
                       smem, s, a);

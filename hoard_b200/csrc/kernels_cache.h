@@ -1,6 +1,7 @@
 // kernels_cache.h -- launch interface of the cache operators (kernels_cache.cu, kernels_cache_select.cu),
 // called by cache_api.cpp after its argument checks.
 #pragma once
+#include <atomic>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -8,6 +9,22 @@ namespace hoard {
 
 constexpr int KV_SMS = 148;              // B200: one split CTA per SM
 constexpr int KV_CHUNK = 16;             // rows of one step of a warp (the M of m16n8k16)
+
+// Dynamic shared memory above 48 KiB has to be allowed once for each kernel and device; asking again costs a
+// launch's time in every call.
+struct SmemLimit {
+    std::atomic<uint64_t> done{0};       // devices 0..63
+    cudaError_t raise(const void* fn, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+};
 
 // The cache and the query side of one attention call. Strides in elements (caches) and floats (q, gate).
 struct CacheAttn {
@@ -67,7 +84,8 @@ struct CacheSelect {
     bool bf16;
     int n_head, n_kv, g, hd, m, n_past, max_rows, block, n_sink, n_local, n_sel;
     const int32_t* n_past_dev;
-    double* u;                           // [n_kv][m * g][nb_cap]
+    double* u;                           // [n_kv][m * g][max_rows / block]
+    double* u_top;                       // [n_kv][m * g][ceil of that / 32]
     int32_t *list, *list_n, *sel_out;
     int list_cap;
 };

@@ -1,14 +1,15 @@
 // kernels_cache_select.cu -- choosing rows and blocks of a KV cache: eviction by accumulated weight, the
 // blocks' bounds and scores, the selection of blocks, and the moves of rows.
 //
-// Both selections are "the k largest of n keys, the lower index where equal", n from a few to 10^5. A cluster
-// of eight CTAs holds the keys of one problem in shared memory, each CTA a contiguous range so that order is
-// kept, and narrows the threshold by radix: histograms of eight bits from the top, added up over the cluster
-// through distributed shared memory, until the bin that holds the k-th key holds no more than are wanted.
-// Counting ranks by pairs is n^2, a sort moves what is not asked for, and one CTA alone is bound by the
-// bandwidth of one SM.
+// Both selections are "the k largest of n keys, the lower index where equal", n from a few to 10^5. The keys of a
+// problem sit in the shared memory of one CTA, or where there are many in that of a cluster of eight, each CTA a
+// contiguous range so that order is kept. The threshold is narrowed by radix, eleven bits at a time from the
+// top (the exponent of a weight and two bits of its mantissa, the exponent of a score), histograms added up over the
+// cluster through distributed shared memory, until the bin that holds the k-th key holds no more than are
+// wanted: two or three passes. Counting ranks by pairs is n^2, and a sort moves what is not asked for.
 #include "common.cuh"
 #include "kernels_cache.h"
+#include "async_copy.cuh"
 
 #include <cooperative_groups.h>
 
@@ -19,126 +20,205 @@ namespace hoard {
 namespace {
 
 constexpr int CL = 8;                    // CTAs of a cluster (the portable maximum)
+constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32;
+constexpr int DIGIT = 11, BINS = 1 << DIGIT;
+static_assert(BINS == 2 * SEL_THREADS, "two bins per thread");
 
-// exclusive prefix sum over the CTA; total receives the sum. One 64-bit value per thread.
-template <int THREADS>
+// exclusive prefix sum over the CTA; total receives the sum
 __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* s_warp,
                                                          unsigned long long& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned long long x = v;
+    auto scan32 = [&](unsigned long long x) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        return x;
+    };
+    const unsigned long long x = scan32(v);
     __syncthreads();                     // s_warp may still be read from an earlier scan
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    unsigned long long before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-        const unsigned long long y = s_warp[w];
-        if (w < warp) before += y;
-        all += y;
-    }
-    total = all;
-    return before + x - v;
+    const unsigned long long w = scan32(s_warp[lane]);
+    total = __shfl_sync(0xffffffffu, w, SEL_WARPS - 1);
+    const unsigned long long before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+    return (warp ? before : 0) + x - v;
 }
 
-struct Exchange {                        // one CTA's contribution to cluster-wide prefixes
-    unsigned long long v[2];
+// Shared state of a selection
+struct Select {
+    unsigned hist[2][BINS];
+    unsigned long long warp[SEL_WARPS];
+    unsigned long long ex[2];            // this CTA's totals, for prefixes over the cluster
+    unsigned bin, in_bin, above;
 };
 
-// exclusive prefix over the cluster's CTAs of `total` (slot: which of the two buffers; a buffer is not
-// written again before every CTA has passed another cluster barrier)
-__device__ __forceinline__ unsigned long long cluster_before(cg::cluster_group& cl, Exchange* ex, int slot,
-                                                             unsigned long long total) {
-    if (threadIdx.x == 0) ex->v[slot] = total;
+// exclusive prefix over the cluster's CTAs of `total` (a slot is used once, so nothing overwrites it)
+template <int CLN>
+__device__ __forceinline__ unsigned long long cluster_before(Select& s, int slot, unsigned long long total) {
+    if constexpr (CLN == 1) return 0;
+    cg::cluster_group cl = cg::this_cluster();
+    if (threadIdx.x == 0) s.ex[slot] = total;
     cl.sync();
-    unsigned long long before = 0;
-    for (unsigned r = 0; r < cl.block_rank(); ++r) before += cl.map_shared_rank(ex, r)->v[slot];
+    unsigned long long v[CLN], before = 0;
+#pragma unroll
+    for (int r = 0; r < CLN; ++r) v[r] = *cl.map_shared_rank(&s.ex[slot], r);
+#pragma unroll
+    for (int r = 0; r < CLN; ++r)
+        if (r < (int)cl.block_rank()) before += v[r];
     return before;
 }
 
-// The `need` largest of the cluster's keys: afterwards a key is in if (key >> shift) > prefix, and of those
-// with (key >> shift) == prefix the first `eq_need` in index order are. key(i): this CTA's i-th key.
-// hist: two buffers of 256 counts.
+// The `need` largest of the keys: afterwards a key is in if (key >> shift) > prefix, and of those with
+// (key >> shift) == prefix the first `eq_need` in index order are. key(i): this CTA's i-th key.
 struct Threshold {
     unsigned long long prefix;
     int shift, eq_need;
 };
-template <int THREADS, int BITS, typename Key>
-__device__ __forceinline__ Threshold cluster_threshold(cg::cluster_group& cl, Key key, int n_local, int need,
-                                                       unsigned (*hist)[256], unsigned long long* s_warp) {
-    __shared__ unsigned s_bin, s_in_bin, s_above;
+template <int CLN, int BITS, typename Key>
+__device__ __forceinline__ Threshold select_threshold(Select& s, Key key, int n_local, int need) {
     unsigned long long prefix = 0;
     int shift = BITS, buf = 0;
-    for (;;) {
-        shift -= 8;
-        for (int i = threadIdx.x; i < 256; i += THREADS) hist[buf][i] = 0;
+    for (bool first = true;; first = false) {
+        const int width = min(DIGIT, shift);
+        shift -= width;
+        unsigned* hist = s.hist[buf];
+        hist[threadIdx.x] = 0;
+        hist[threadIdx.x + SEL_THREADS] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < n_local; i += THREADS) {
+        for (int i = threadIdx.x; i < n_local; i += SEL_THREADS) {
             const unsigned long long k = key(i);
-            if (shift == BITS - 8 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[buf][(k >> shift) & 255], 1u);
+            const unsigned d = (unsigned)(k >> shift) & ((1u << width) - 1);
+            if (first) {                 // exponents: few bins, so a warp's equal ones are added at once
+                const unsigned act = __activemask(), same = __match_any_sync(act, d);
+                if ((int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&hist[d], (unsigned)__popc(same));
+            } else if ((k >> (shift + width)) == prefix) {
+                atomicAdd(&hist[d], 1u);
+            }
         }
-        cl.sync();
-        unsigned mine = 0;               // thread i: bin 255 - i, so that the scan runs from the top
-        if (threadIdx.x < 256)
-            for (int r = 0; r < CL; ++r) mine += cl.map_shared_rank(&hist[buf][0], r)[255 - threadIdx.x];
+        // thread i: bins BINS - 1 - 2i and BINS - 2 - 2i, so that the scan runs from the top
+        unsigned hi = 0, lo = 0;
+        if constexpr (CLN == 1) {
+            __syncthreads();
+            const uint2 h = *reinterpret_cast<const uint2*>(hist + BINS - 2 - 2 * threadIdx.x);
+            lo = h.x;
+            hi = h.y;
+        } else {
+            cg::cluster_group cl = cg::this_cluster();
+            cl.sync();
+            uint2 h[CLN];
+#pragma unroll
+            for (int r = 0; r < CLN; ++r)
+                h[r] = *reinterpret_cast<const uint2*>(cl.map_shared_rank(hist, r) + BINS - 2 - 2 * threadIdx.x);
+#pragma unroll
+            for (int r = 0; r < CLN; ++r) {
+                lo += h[r].x;
+                hi += h[r].y;
+            }
+        }
         unsigned long long total;
-        const unsigned above = (unsigned)block_scan<THREADS>(mine, s_warp, total);
-        if (threadIdx.x < 256 && above < (unsigned)need && above + mine >= (unsigned)need) {
-            s_bin = 255 - threadIdx.x;
-            s_in_bin = mine;
-            s_above = above;
+        const unsigned above = (unsigned)block_scan(hi + lo, s.warp, total), n = (unsigned)need;
+        if (above < n && above + hi >= n) {
+            s.bin = BINS - 1 - 2 * threadIdx.x;
+            s.in_bin = hi;
+            s.above = above;
+        } else if (above + hi < n && above + hi + lo >= n) {
+            s.bin = BINS - 2 - 2 * threadIdx.x;
+            s.in_bin = lo;
+            s.above = above + hi;
         }
         __syncthreads();
-        prefix = prefix << 8 | s_bin;
-        need -= (int)s_above;
-        const bool done = shift == 0 || s_in_bin == (unsigned)need;
-        __syncthreads();                 // s_bin is read before the next pass writes it
+        prefix = prefix << width | s.bin;
+        need -= (int)s.above;
+        const bool done = shift == 0 || s.in_bin == (unsigned)need;
+        __syncthreads();                 // read before the next pass writes
         if (done) return {prefix, shift, need};
-        buf ^= 1;
+        buf ^= 1;                        // the cluster's other CTAs may still read this pass's counts
     }
 }
 
-// ---- eviction: the moves ------------------------------------------------------------------------------------
+// ---- eviction -------------------------------------------------------------------------------------------------
 // Key of a row: protected rows above everything; weights in order; NaN below everything. -0 equals +0.
-constexpr int EV_THREADS = 1024, EV_KEYS = 40960;      // keys a CTA holds in shared memory (160 KiB)
+constexpr int EV_KEYS = 40960;           // keys that a CTA holds in shared memory (160 KiB)
+constexpr int EV_SINGLE = 8192;          // rows up to which one CTA chooses alone
+constexpr int EV_FUSED = 1024;           // moves up to which that CTA makes them itself
 __device__ __forceinline__ unsigned evict_key(float acc, int pos, int n_sink, int recent_from) {
     if (pos < n_sink || pos >= recent_from) return 0xFFFFFFFFu;
     if (acc != acc) return 0u;
     const unsigned b = __float_as_uint(acc + 0.f);
     return b >> 31 ? ~b : b | 0x80000000u;
 }
-// Grid (CL, n_kv). Writes to[], from[] (rows, ascending both) and the number of moves of each head, and
-// acc_out / pos_out of the kept rows that stay where they are.
-__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(EV_THREADS) k_evict_choose(const CacheEvict e) {
+// Moves i0, i0 + 1, .. of N: K and V rows by 16-byte pieces, all N loads before the first store. Rows read are at or
+// above n_keep, rows written below it.
+template <int N>
+__device__ __forceinline__ void move_rows(const CacheEvict& e, int kv, const int32_t* to, const int32_t* from, int i0,
+                                          int n) {
+    const int lane = threadIdx.x & 31, c16 = e.hd / 8;
+    const int64_t hb = (int64_t)kv * e.max_rows;
+    int t[N], f[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        t[k] = i0 + k < n ? to[i0 + k] : -1;
+        f[k] = i0 + k < n ? from[i0 + k] : 0;
+    }
+    for (int p = lane; p < 2 * c16; p += 32) {
+        char* c = static_cast<char*>(p < c16 ? e.kc : e.vc) + (int64_t)kv * e.hs * 2 + (p < c16 ? p : p - c16) * 16;
+        uint4 v[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (t[k] >= 0) v[k] = *reinterpret_cast<const uint4*>(c + (int64_t)f[k] * e.rs * 2);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (t[k] >= 0) *reinterpret_cast<uint4*>(c + (int64_t)t[k] * e.rs * 2) = v[k];
+    }
+    if (lane < N && i0 + lane < n) {
+        const int tt = to[i0 + lane], ff = from[i0 + lane];
+        e.acc_out[hb + tt] = e.acc[hb + ff];
+        e.pos_out[hb + tt] = e.pos[hb + ff];
+    }
+}
+// Grid (CLN, n_kv). Lists the rows to fill and the rows to move (ascending both), writes acc_out / pos_out of the
+// kept rows that stay where they are, and makes the moves itself where there are few (to, from then sit in
+// shared memory).
+template <int CLN>
+__global__ void __launch_bounds__(SEL_THREADS) k_evict_choose(const CacheEvict e, const bool fused) {
     pdl_enter();
     extern __shared__ unsigned s_key[];
-    __shared__ unsigned hist[2][256];
-    __shared__ unsigned long long s_warp[EV_THREADS / 32];
-    __shared__ Exchange s_ex;
-    cg::cluster_group cl = cg::this_cluster();
-    const int kv = blockIdx.y, rank = (int)cl.block_rank(), tid = threadIdx.x;
+    __shared__ Select sel;
+    __shared__ int32_t s_to[CLN == 1 ? EV_FUSED : 1], s_from[CLN == 1 ? EV_FUSED : 1];
+    const int kv = blockIdx.y, rank = CLN == 1 ? 0 : blockIdx.x, tid = threadIdx.x;
     const float* acc = e.acc + (int64_t)kv * e.max_rows;
     const int32_t* pos = e.pos + (int64_t)kv * e.max_rows;
-    const int first = (int)((int64_t)e.n_rows * rank / CL), last = (int)((int64_t)e.n_rows * (rank + 1) / CL);
+    const int first = (int)((int64_t)e.n_rows * rank / CLN), last = (int)((int64_t)e.n_rows * (rank + 1) / CLN);
     const int n = last - first;
-    const bool held = n <= EV_KEYS;
+    const bool held = CLN == 1 || n <= EV_KEYS;
     auto fresh = [&](int i) { return evict_key(acc[first + i], pos[first + i], e.n_sink, e.recent_from); };
-    if (held)
-        for (int i = tid; i < n; i += EV_THREADS) s_key[i] = fresh(i);
+    if (held) {
+        for (int i0 = tid; i0 < n; i0 += 8 * SEL_THREADS) {
+            float a[8];
+            int p[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i0 + k * SEL_THREADS < n) {
+                    a[k] = acc[first + i0 + k * SEL_THREADS];
+                    p[k] = pos[first + i0 + k * SEL_THREADS];
+                }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i0 + k * SEL_THREADS < n) s_key[i0 + k * SEL_THREADS] = evict_key(a[k], p[k], e.n_sink, e.recent_from);
+        }
+    }
     __syncthreads();
     auto key = [&](int i) { return held ? s_key[i] : fresh(i); };
-    const Threshold th = cluster_threshold<EV_THREADS, 32>(cl, key, n, e.n_keep, hist, s_warp);
+    const Threshold th = select_threshold<CLN, 32>(sel, key, n, e.n_keep);
 
     // a thread owns a run of rows (odd length: the runs' first words fall in different banks)
-    const int len = (n + EV_THREADS - 1) / EV_THREADS | 1, i0 = min(n, tid * len), i1 = min(n, i0 + len);
+    const int len = (n + SEL_THREADS - 1) / SEL_THREADS | 1, i0 = min(n, tid * len), i1 = min(n, i0 + len);
     unsigned long long eq = 0, total;
     for (int i = i0; i < i1; ++i) eq += (unsigned long long)(key(i) >> th.shift) == th.prefix;
-    unsigned long long eq_rank = block_scan<EV_THREADS>(eq, s_warp, total);
-    eq_rank += cluster_before(cl, &s_ex, 0, total);
+    unsigned long long eq_rank = block_scan(eq, sel.warp, total);
+    eq_rank += cluster_before<CLN>(sel, 0, total);
     const unsigned long long eq_rank0 = eq_rank;
     auto kept = [&](int i) {
         const unsigned long long k = key(i) >> th.shift;
@@ -150,21 +230,22 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(EV_THREADS) k_evict
         if (first + i < e.n_keep) counts += !k;
         else if (k) counts += 1ull << 32;
     }
-    unsigned long long at = block_scan<EV_THREADS>(counts, s_warp, total);
-    const unsigned long long before = cluster_before(cl, &s_ex, 1, total);
+    unsigned long long at = block_scan(counts, sel.warp, total);
+    const unsigned long long before = cluster_before<CLN>(sel, 1, total);
     at += before;
-    if (rank == CL - 1 && tid == 0) e.n_moves[kv] = (int)((before + total) & 0xFFFFFFFFu);
+    if (rank == CLN - 1 && tid == 0) e.n_moves[kv] = (int)((before + total) & 0xFFFFFFFFu);
     eq_rank = eq_rank0;
-    int32_t* to = e.to + (int64_t)kv * e.max_rows;
-    int32_t* from = e.from + (int64_t)kv * e.max_rows;
+    int32_t* to = CLN == 1 && fused ? s_to : e.to + (int64_t)kv * e.max_rows;
+    int32_t* from = CLN == 1 && fused ? s_from : e.from + (int64_t)kv * e.max_rows;
     int n_to = (int)(at & 0xFFFFFFFFu), n_from = (int)(at >> 32);
+    const bool stay = e.acc_out != e.acc || e.pos_out != e.pos;
     for (int i = i0; i < i1; ++i) {
         const bool k = kept(i);
         const int row = first + i;
         if (row < e.n_keep) {
             if (!k) {
                 to[n_to++] = row;
-            } else {
+            } else if (stay) {
                 e.acc_out[(int64_t)kv * e.max_rows + row] = acc[row];
                 e.pos_out[(int64_t)kv * e.max_rows + row] = pos[row];
             }
@@ -172,26 +253,21 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(EV_THREADS) k_evict
             from[n_from++] = row;
         }
     }
-    cl.sync();                                         // no CTA leaves while its counts may be read
+    if constexpr (CLN == 1) {
+        if (fused) {
+            const int moves = (int)(total & 0xFFFFFFFFu);
+            __syncthreads();
+            for (int i = (tid >> 5) * 4; i < moves; i += SEL_WARPS * 4) move_rows<4>(e, kv, s_to, s_from, i, moves);
+        }
+    } else {
+        cg::this_cluster().sync();                     // no CTA leaves while its counts may be read
+    }
 }
-// One warp per move: lanes take the K row's 16-byte pieces, then the V row's. Rows read are at or above n_keep,
-// rows written below it.
 __global__ void __launch_bounds__(256) k_evict_move(const CacheEvict e) {
     pdl_enter();
-    const int kv = blockIdx.y, i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (i >= e.n_moves[kv]) return;
-    const int64_t hb = (int64_t)kv * e.max_rows;
-    const int to = e.to[hb + i], from = e.from[hb + i];
-    const int c16 = e.hd / 8;
-    const int64_t src = ((int64_t)from * e.rs + (int64_t)kv * e.hs) * 2, dst = ((int64_t)to * e.rs + (int64_t)kv * e.hs) * 2;
-    for (int p = lane; p < 2 * c16; p += 32) {
-        char* c = static_cast<char*>(p < c16 ? e.kc : e.vc) + (p < c16 ? p : p - c16) * 16;
-        *reinterpret_cast<uint4*>(c + dst) = *reinterpret_cast<const uint4*>(c + src);
-    }
-    if (lane == 0) {
-        e.acc_out[hb + to] = e.acc[hb + from];
-        e.pos_out[hb + to] = e.pos[hb + from];
-    }
+    const int kv = blockIdx.y, i = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 4, n = e.n_moves[kv];
+    if (i >= n) return;
+    move_rows<4>(e, kv, e.to + (int64_t)kv * e.max_rows, e.from + (int64_t)kv * e.max_rows, i, n);
 }
 
 // ---- bounds of complete blocks: one CTA per (block, KV head) --------------------------------------------------
@@ -224,15 +300,18 @@ __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __r
         const uint16_t* base = kc + (int64_t)b * block * rs + (int64_t)kv * hs + 8 * c;
         const int r0 = min(gi, block - 1);
         lo.u = hi.u = *reinterpret_cast<const uint4*>(base + r0 * rs);
-#pragma unroll 4
-        for (int r = gi + groups; r < block; r += groups) {
-            V x;
-            x.u = *reinterpret_cast<const uint4*>(base + r * rs);
+        for (int r = gi + groups; r < block; r += 8 * groups) {      // eight rows' loads in flight
+            V x[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                lo.h[i] = min2(lo.h[i], x.h[i]);
-                hi.h[i] = max2(hi.h[i], x.h[i]);
-            }
+            for (int k = 0; k < 8; ++k)
+                x[k].u = r + k * groups < block ? *reinterpret_cast<const uint4*>(base + (r + k * groups) * rs) : lo.u;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    lo.h[i] = min2(lo.h[i], x[k].h[i]);
+                    hi.h[i] = max2(hi.h[i], x[k].h[i]);
+                }
         }
         s_lo[threadIdx.x] = lo.u;
         s_hi[threadIdx.x] = hi.u;
@@ -258,8 +337,9 @@ __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __r
 // ---- scores: u[kv][row][b - first] = sum_d max(q_d kmin_d, q_d kmax_d) = sum_d q_d (q_d > 0 ? kmax_d : kmin_d) ----
 // In 64 bits, because the scores decide which rows are read: products of 24 and 11 (or 8) bits are exact, and
 // sums differ from the true ones in the 16th digit. A CTA takes 32 blocks (one per lane) and eight query rows;
-// its warps share out the dims and their sums are added in warp order. A value is converted once for the
-// eight rows, since conversions to f64 run at a quarter of the rate of its multiply-adds.
+// its warps share out the dims, eight at a time, and their sums are added in warp order. A value is converted once
+// for the eight rows, since conversions to f64 run at a quarter of the rate of its multiply-adds. u_top receives
+// the rows' maxima over the CTA's blocks.
 struct Candidates {
     int n_past, nb, first, last;
 };
@@ -277,6 +357,7 @@ template <> __device__ __forceinline__ double2 to_double2<__nv_bfloat16>(uint32_
 }
 
 constexpr int SC_THREADS = 256, SC_ROWS = 8, SC_BLOCKS = 32;
+constexpr int score_smem(int hd) { return SC_ROWS * hd * 8 + 8 * SC_ROWS * 32 * 8 + SC_BLOCKS * (hd + 4) * 4; }
 template <typename KT>
 __global__ void __launch_bounds__(SC_THREADS) k_block_score(const CacheSelect c, int nb_cap) {
     pdl_enter();
@@ -287,30 +368,43 @@ __global__ void __launch_bounds__(SC_THREADS) k_block_score(const CacheSelect c,
     const int R = c.m * c.g, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     double* sq = reinterpret_cast<double*>(s_raw);                              // [SC_ROWS][hd]
     double* red = sq + SC_ROWS * c.hd;                                          // [8 warps][SC_ROWS][32]
-    uint32_t* sb = reinterpret_cast<uint32_t*>(red + 8 * SC_ROWS * 32);         // [32][hd + 1] words
-    for (int i = tid; i < SC_ROWS * c.hd; i += SC_THREADS) {
-        const int r = i / c.hd, d = i - r * c.hd, row = row0 + r;
-        sq[i] = row < R ? (double)c.q[(row / c.g) * c.q_ts + (kv * c.g + row % c.g) * c.q_hs + d] : 0.0;
-    }
-    const int n = min(SC_BLOCKS, n_cand - b0);
+    // [32][hd + 4] words: 16-byte reads of eight lanes fall in eight bank groups
+    uint32_t* sb = reinterpret_cast<uint32_t*>(red + 8 * SC_ROWS * 32);
+    const int n = min(SC_BLOCKS, n_cand - b0), c4 = c.hd / 4, c8 = c.hd / 8;
     const uint32_t* src = reinterpret_cast<const uint32_t*>(c.bounds) +
                           ((int64_t)kv * (c.max_rows / c.block) + cd.first + b0) * c.hd;      // hd words a block
-    for (int i = tid; i < n * c.hd; i += SC_THREADS) {
-        const int b = i / c.hd, w = i - b * c.hd;
-        sb[b * (c.hd + 1) + w] = src[i];
+    for (int b = warp; b < n; b += 8)
+        for (int p = lane; p < c4; p += 32) cp_async16(sb + b * (c.hd + 4) + 4 * p, src + b * c.hd + 4 * p);
+    cp_async_commit();
+    {
+        const int row = row0 + warp;                   // a warp converts a query row
+        const float* q = c.q + (row / c.g) * c.q_ts + (kv * c.g + row % c.g) * c.q_hs;
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = row < R && k * 32 + lane < c.hd ? q[k * 32 + lane] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k * 32 + lane < c.hd) sq[warp * c.hd + k * 32 + lane] = (double)x[k];
     }
+    cp_async_wait_all();
     __syncthreads();
     double acc[SC_ROWS];
 #pragma unroll
     for (int r = 0; r < SC_ROWS; ++r) acc[r] = 0.0;
-    const uint32_t* mine = sb + min(lane, n - 1) * (c.hd + 1);
-    for (int p = warp; p < c.hd / 2; p += 8) {
-        const double2 lo = to_double2<KT>(mine[p]), hi = to_double2<KT>(mine[c.hd / 2 + p]);
+    const uint32_t* mine = sb + min(lane, n - 1) * (c.hd + 4);
+    for (int p = warp; p < c8; p += 8) {
+        const uint4 l4 = *reinterpret_cast<const uint4*>(mine + 4 * p);
+        const uint4 h4 = *reinterpret_cast<const uint4*>(mine + c.hd / 2 + 4 * p);
+        const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
 #pragma unroll
-        for (int r = 0; r < SC_ROWS; ++r) {
-            const double2 q = *reinterpret_cast<const double2*>(sq + r * c.hd + 2 * p);
-            acc[r] = fma(q.x, q.x > 0.0 ? hi.x : lo.x, acc[r]);
-            acc[r] = fma(q.y, q.y > 0.0 ? hi.y : lo.y, acc[r]);
+        for (int k = 0; k < 4; ++k) {
+            const double2 lo = to_double2<KT>(lw[k]), hi = to_double2<KT>(hw[k]);
+#pragma unroll
+            for (int r = 0; r < SC_ROWS; ++r) {
+                const double2 q = *reinterpret_cast<const double2*>(sq + r * c.hd + 8 * p + 2 * k);
+                acc[r] = fma(q.x, q.x > 0.0 ? hi.x : lo.x, acc[r]);
+                acc[r] = fma(q.y, q.y > 0.0 ? hi.y : lo.y, acc[r]);
+            }
         }
     }
 #pragma unroll
@@ -319,25 +413,29 @@ __global__ void __launch_bounds__(SC_THREADS) k_block_score(const CacheSelect c,
     double s = 0.0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) s += red[(w * SC_ROWS + warp) * 32 + lane];     // thread = (row, block)
-    if (lane < n && row0 + warp < R) c.u[((int64_t)kv * R + row0 + warp) * nb_cap + b0 + lane] = s;
+    const int row = row0 + warp;
+    if (row >= R) return;
+    if (lane < n) c.u[((int64_t)kv * R + row) * nb_cap + b0 + lane] = s;
+    double top = lane < n ? s : -INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) c.u_top[((int64_t)kv * R + row) * ((nb_cap + SC_BLOCKS - 1) / SC_BLOCKS) + blockIdx.x] = top;
 }
 
-// ---- selection: one cluster per (KV head, token) -----------------------------------------------------------------
-constexpr int BS_THREADS = 256, BS_MAX_G = 64;
-__device__ __forceinline__ unsigned long long order_key(double v) {
-    if (v != v) return 0ull;
-    const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
-    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+// ---- selection: one CTA or cluster per (KV head, token) -------------------------------------------------------
+// Key of a score max_h (u_h - top_h) <= 0: the bits of its magnitude, turned over; NaN lowest.
+constexpr int BS_MAX_G = 64;
+constexpr int BS_SINGLE = 2048;          // candidates up to which one CTA chooses alone
+__device__ __forceinline__ unsigned long long score_key(double v) {
+    return v != v ? 0ull : 0x7FFFFFFFFFFFFFFFull - (unsigned long long)__double_as_longlong(fabs(v));
 }
-__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(BS_THREADS) k_block_choose(const CacheSelect c, int nb_cap) {
+template <int CLN>
+__global__ void __launch_bounds__(SEL_THREADS) k_block_choose(const CacheSelect c, int nb_cap) {
     pdl_enter();
     extern __shared__ unsigned long long s_keys[];
-    __shared__ unsigned hist[2][256];
-    __shared__ unsigned long long s_warp[BS_THREADS / 32];
-    __shared__ double s_max[BS_MAX_G], s_top[BS_MAX_G];
-    __shared__ Exchange s_ex;
-    cg::cluster_group cl = cg::this_cluster();
-    const int kv = blockIdx.y, t = blockIdx.z, rank = (int)cl.block_rank(), tid = threadIdx.x;
+    __shared__ Select ss;
+    __shared__ double s_top[BS_MAX_G];
+    const int kv = blockIdx.y, t = blockIdx.z, rank = CLN == 1 ? 0 : blockIdx.x, tid = threadIdx.x;
     const int lane = tid & 31, warp = tid >> 5;
     const Candidates cd = candidates(c);
     const int n_cand = cd.last - cd.first, n_take = min(n_cand, c.n_sel);
@@ -345,7 +443,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(BS_THREADS) k_block
     int32_t* list = c.list + (int64_t)prob * c.list_cap;
     int32_t* sel = c.sel_out ? c.sel_out + ((int64_t)t * c.n_kv + kv) * c.n_sel : nullptr;
     // the blocks that are always attended, and the tail of sel
-    const int gtid = rank * BS_THREADS + tid, gn = CL * BS_THREADS;
+    const int gtid = rank * SEL_THREADS + tid, gn = CLN * SEL_THREADS;
     for (int i = gtid; i < cd.first; i += gn) list[i] = i;
     for (int i = gtid; i < cd.nb - cd.last; i += gn) list[cd.first + n_take + i] = cd.last + i;
     if (sel)
@@ -359,43 +457,58 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(BS_THREADS) k_block
         return;
     }
     if (n_take == 0) return;
-    const int i0 = (int)((int64_t)n_cand * rank / CL), i1 = (int)((int64_t)n_cand * (rank + 1) / CL), n = i1 - i0;
-    const double* u = c.u + ((int64_t)kv * c.m + t) * c.g * nb_cap + i0;
-    for (int h = warp; h < c.g; h += BS_THREADS / 32) {
+    const int i0 = (int)((int64_t)n_cand * rank / CLN), i1 = (int)((int64_t)n_cand * (rank + 1) / CLN), n = i1 - i0;
+    const int64_t row0 = ((int64_t)kv * c.m + t) * c.g;
+    const int tops = (n_cand + SC_BLOCKS - 1) / SC_BLOCKS, top_cap = (nb_cap + SC_BLOCKS - 1) / SC_BLOCKS;
+    for (int h = warp; h < c.g; h += SEL_WARPS) {
+        const double* p = c.u_top + (row0 + h) * top_cap;
         double mx = -INFINITY;
-        for (int i = lane; i < n; i += 32) mx = fmax(mx, u[(int64_t)h * nb_cap + i]);
+        for (int i = lane; i < tops; i += 8 * 32) {
+            double v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = i + 32 * k < tops ? p[i + 32 * k] : -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mx = fmax(mx, v[k]);
+        }
+#pragma unroll
         for (int o = 16; o > 0; o >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (lane == 0) s_max[h] = mx;
+        if (lane == 0) s_top[h] = mx;
     }
-    cl.sync();
-    if (tid < c.g) {
-        double mx = -INFINITY;
-        for (int r = 0; r < CL; ++r) mx = fmax(mx, cl.map_shared_rank(s_max, r)[tid]);
-        s_top[tid] = mx;
-    }
+    // this thread's blocks' u are on their way while the maxima are waited for
+    const double* u = c.u + row0 * nb_cap + i0;
+    double v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = tid < n && k < c.g ? u[k * (int64_t)nb_cap + tid] : 0.0;
     __syncthreads();
-    for (int i = tid; i < n; i += BS_THREADS) {
+    for (int i = tid; i < n; i += SEL_THREADS) {
         double best = -INFINITY;
-        for (int h = 0; h < c.g; ++h) best = fmax(best, u[(int64_t)h * nb_cap + i] - s_top[h]);
-        s_keys[i] = order_key(best);
+        for (int h0 = 0; h0 < c.g; h0 += 8) {
+            if (i != tid || h0) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = h0 + k < c.g ? u[(h0 + k) * (int64_t)nb_cap + i] : 0.0;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (h0 + k < c.g) best = fmax(best, v[k] - s_top[h0 + k]);
+        }
+        s_keys[i] = score_key(best);
     }
     __syncthreads();
     auto key = [&](int i) { return s_keys[i]; };
-    const Threshold th = cluster_threshold<BS_THREADS, 64>(cl, key, n, n_take, hist, s_warp);
-    const int len = (n + BS_THREADS - 1) / BS_THREADS | 1, a0 = min(n, tid * len), a1 = min(n, a0 + len);
-    unsigned long long eq = 0, total;
+    const Threshold th = select_threshold<CLN, 63>(ss, key, n, n_take);
+    const int len = (n + SEL_THREADS - 1) / SEL_THREADS | 1, a0 = min(n, tid * len), a1 = min(n, a0 + len);
+    unsigned long long eq = 0, count = 0, total;
     for (int i = a0; i < a1; ++i) eq += (s_keys[i] >> th.shift) == th.prefix;
-    unsigned long long eq_rank = block_scan<BS_THREADS>(eq, s_warp, total);
-    eq_rank += cluster_before(cl, &s_ex, 0, total);
-    unsigned long long count = 0;
+    unsigned long long eq_rank = block_scan(eq, ss.warp, total);
+    eq_rank += cluster_before<CLN>(ss, 0, total);
     const unsigned long long eq_rank0 = eq_rank;
     auto kept = [&](int i) {
         const unsigned long long k = s_keys[i] >> th.shift;
         return k > th.prefix || (k == th.prefix && eq_rank++ < (unsigned long long)th.eq_need);
     };
     for (int i = a0; i < a1; ++i) count += kept(i);
-    unsigned long long at = block_scan<BS_THREADS>(count, s_warp, total);
-    at += cluster_before(cl, &s_ex, 1, total);
+    unsigned long long at = block_scan(count, ss.warp, total);
+    at += cluster_before<CLN>(ss, 1, total);
     eq_rank = eq_rank0;
     for (int i = a0; i < a1; ++i)
         if (kept(i)) {
@@ -404,7 +517,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(BS_THREADS) k_block
             if (sel) sel[at] = b;
             ++at;
         }
-    cl.sync();
+    if constexpr (CLN > 1) cg::this_cluster().sync();  // no CTA leaves while its counts may be read
 }
 
 // ---- the accepted path of a tree: thread = a 16-byte column of the K or V rows of a KV head. Rows ascend and
@@ -428,16 +541,44 @@ __global__ void __launch_bounds__(32) k_cache_take(char* kc, char* vc, int64_t r
 
 }  // namespace
 
+// a programmatic dependent launch in clusters of `cl` CTAs along x
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_cluster(void (*kernel)(KArgs...), int cl, dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                                  Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cl;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 cudaError_t launch_cache_evict(const CacheEvict& e, cudaStream_t s) {
-    const int n = (int)(((int64_t)e.n_rows + CL - 1) / CL);
-    const size_t smem = n <= EV_KEYS ? (size_t)n * 4 : 0;
-    cudaError_t rc = cudaFuncSetAttribute(k_evict_choose, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_KEYS * 4);
-    if (rc != cudaSuccess) return rc;
-    rc = launch_pdl(k_evict_choose, dim3(CL, e.n_kv), EV_THREADS, smem, s, e);
-    if (rc != cudaSuccess) return rc;
-    const int most = e.n_keep < e.n_rows - e.n_keep ? e.n_keep : e.n_rows - e.n_keep;
+    const int most = e.n_keep < e.n_rows - e.n_keep ? e.n_keep : e.n_rows - e.n_keep;      // moves
+    if (e.n_rows <= EV_SINGLE) {
+        const bool fused = most <= EV_FUSED;
+        const cudaError_t rc = launch_pdl(k_evict_choose<1>, dim3(1, e.n_kv), SEL_THREADS, (size_t)e.n_rows * 4, s, e, fused);
+        if (rc != cudaSuccess || fused) return rc;
+    } else {
+        static SmemLimit limit;
+        cudaError_t rc = limit.raise((const void*)k_evict_choose<CL>, EV_KEYS * 4);
+        if (rc != cudaSuccess) return rc;
+        const int n = (e.n_rows + CL - 1) / CL;
+        rc = launch_cluster(k_evict_choose<CL>, CL, dim3(CL, e.n_kv), SEL_THREADS, n <= EV_KEYS ? (size_t)n * 4 : 0, s, e,
+                            false);
+        if (rc != cudaSuccess) return rc;
+    }
     if (most == 0) return cudaSuccess;
-    return launch_pdl(k_evict_move, dim3((most + 7) / 8, e.n_kv), 256, 0, s, e);
+    return launch_pdl(k_evict_move, dim3((most + 31) / 32, e.n_kv), 256, 0, s, e);
 }
 
 cudaError_t launch_cache_bounds(const void* kc, int64_t rs, int64_t hs, bool bf16, int n_kv, int hd, int max_rows,
@@ -460,17 +601,20 @@ cudaError_t launch_cache_select(const CacheSelect& c, cudaStream_t s) {
     cudaError_t e;
     if (n_cand > c.n_sel && c.n_sel > 0) {
         const dim3 grid((n_cand + SC_BLOCKS - 1) / SC_BLOCKS, c.n_kv, (c.m * c.g + SC_ROWS - 1) / SC_ROWS);
-        const size_t smem = (size_t)SC_ROWS * c.hd * 8 + 8 * SC_ROWS * 32 * 8 + (size_t)SC_BLOCKS * (c.hd + 1) * 4;
         auto fn = c.bf16 ? k_block_score<__nv_bfloat16> : k_block_score<__half>;
-        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
+        static SmemLimit limit[2];
+        e = limit[c.bf16].raise((const void*)fn, score_smem(256));
         if (e != cudaSuccess) return e;
-        e = launch_pdl(fn, grid, SC_THREADS, smem, s, c, nb_cap);
+        e = launch_pdl(fn, grid, SC_THREADS, score_smem(c.hd), s, c, nb_cap);
         if (e != cudaSuccess) return e;
     }
-    const size_t smem = (size_t)((n_cand + CL - 1) / CL) * 8;
-    e = cudaFuncSetAttribute(k_block_choose, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+    if (n_cand <= BS_SINGLE)
+        return launch_pdl(k_block_choose<1>, dim3(1, c.n_kv, c.m), SEL_THREADS, (size_t)n_cand * 8, s, c, nb_cap);
+    static SmemLimit limit;
+    e = limit.raise((const void*)k_block_choose<CL>, 128 * 1024);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_block_choose, dim3(CL, c.n_kv, c.m), BS_THREADS, smem, s, c, nb_cap);
+    return launch_cluster(k_block_choose<CL>, CL, dim3(CL, c.n_kv, c.m), SEL_THREADS, (size_t)((n_cand + CL - 1) / CL) * 8, s,
+                          c, nb_cap);
 }
 
 cudaError_t launch_cache_take(void* kc, void* vc, int64_t rs, int64_t hs, int n_kv, int hd, int row0,
