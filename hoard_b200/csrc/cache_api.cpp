@@ -58,12 +58,19 @@ struct Ws {
 Ws ws_plan(const hoard_kv_desc* d) {
     Ws w{};
     const int g = d->n_head / d->n_head_kv, hdt = cache_tile_dims(d->head_dim);
-    // problems x row tiles x splits is at most one CTA per SM, or one split each where there are more tiles
-    const int rt = cache_tile_rows(d->head_dim, d->max_tokens * g), rt1 = cache_tile_rows(d->head_dim, g);
-    int64_t dense = (int64_t)d->n_head_kv * ceil_div((int64_t)d->max_tokens * g, rt);
+    // problems x row tiles x splits is at most one CTA per SM, or one split each where there are more tiles; the
+    // tensor-core form has tiles of 128 rows and the own rows' split beside them
+    const int64_t R = (int64_t)d->max_tokens * g;
+    const int rt = cache_tile_rows(d->head_dim, (int)R), rt1 = cache_tile_rows(d->head_dim, g);
+    int64_t dense = d->n_head_kv * ceil_div(R, rt);
     int64_t lists = d->block ? (int64_t)d->n_head_kv * d->max_tokens * ceil_div(g, rt1) : 0;
     dense = (dense > KV_SMS ? dense : KV_SMS) * rt;
     lists = d->block ? (lists > KV_SMS ? lists : KV_SMS) * rt1 : 0;
+    if (R > TC_MIN_R && hdt <= 128) {
+        int64_t tc = d->n_head_kv * ceil_div(R, 128);
+        tc = (tc > KV_SMS ? tc : KV_SMS) * 128 + d->n_head_kv * R;
+        if (tc > dense) dense = tc;
+    }
     const int64_t rows = dense > lists ? dense : lists;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -160,7 +167,10 @@ int hoard_kv_attention(const hoard_kv_desc* d, const hoard_kv_query* a, float* a
         c.logits = reinterpret_cast<float*>(b + w.logits);
         c.logits_ld = w.logits_ld;
     }
-    plan_splits(c, chunks_of(c, c.n_past_dev ? c.max_rows - c.m : c.n_past));
+    const int64_t past = c.n_past_dev ? c.max_rows - c.m : c.n_past;
+    if (!acc) c.tc_splits = cache_tc_splits(c.hd, c.n_kv, c.R, past);
+    plan_splits(c, chunks_of(c, past));
+    if (c.tc_splits) c.splits = c.tc_splits + 1;
     return st(launch_cache_attention(c, (cudaStream_t)stream));
 }
 

@@ -11,46 +11,17 @@
 // end of the CTA and once after all CTAs (k_cache_combine).
 //
 // Precision. K and V enter the products as they are stored. q (f32) and the weights p (f32) are written as
-// sums of f16 or bf16 terms, whatever the cache's type is: two f16 terms hold 22 bits, three bf16 terms 24, so
-// a product is f32-accurate; sums, maxima and totals are f32. For f16 the rows of q are scaled by a power of
-// two to [2^13, 2^14) and p by 2^14, which keeps the terms out of f16's subnormal range; the factors are taken out
-// of the scores (exactly) and cancel in p / total.
+// sums of f16 or bf16 terms (kv_terms.cuh), whatever the cache's type is, so a product is f32-accurate; sums, maxima
+// and totals are f32.
 #include "common.cuh"
 #include "kernels_cache.h"
 #include "async_copy.cuh"
+#include "kv_terms.cuh"
 
 namespace hoard {
 
 namespace {
 
-template <typename KT> struct Terms;
-template <> struct Terms<__half> {
-    static constexpr int N = 2, Q_EXP = 13;
-    static constexpr float P_EXP = 14.f;
-    static constexpr uint32_t INF2 = 0x7C007C00u;        // exponent bits of two values
-};
-template <> struct Terms<__nv_bfloat16> {
-    static constexpr int N = 3, Q_EXP = 0;
-    static constexpr float P_EXP = 0.f;
-    static constexpr uint32_t INF2 = 0x7F807F80u;
-};
-
-// two f32 -> packed terms: a's rounding in the low half, b's in the high half; a and b become the remainders
-template <typename KT> __device__ __forceinline__ uint32_t take_term(float& a, float& b);
-template <> __device__ __forceinline__ uint32_t take_term<__half>(float& a, float& b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    a -= f.x;
-    b -= f.y;
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <> __device__ __forceinline__ uint32_t take_term<__nv_bfloat16>(float& a, float& b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    const float2 f = __bfloat1622float2(h);
-    a -= f.x;
-    b -= f.y;
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 template <typename KT> __device__ __forceinline__ float kv_lo(uint32_t w);
 template <> __device__ __forceinline__ float kv_lo<__half>(uint32_t w) { return h2f(w); }
 template <> __device__ __forceinline__ float kv_lo<__nv_bfloat16>(uint32_t w) { return __uint_as_float(w << 16); }
@@ -86,12 +57,6 @@ __device__ __forceinline__ void cp16z(unsigned dst, const void* src, bool there)
 template <int N> __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Warps and ring stages of one CTA (one CTA per SM): with head_dim 128 a stage is 16 rows of K and V, 8 KiB,
 // and eight warps keep two stages each in flight, 128 KiB per SM, while they work on a third.
 template <int HD> struct Plan {
@@ -128,12 +93,13 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
     const int t0 = BLOCKS ? prob - kv * a.m : 0;       // first token of the problem's rows
     uint32_t* qf = reinterpret_cast<uint32_t*>(smem + Plan<HD>::RING);
 
-    // chunks of this CTA: past rows (or the listed blocks' rows), then the tokens' own rows
+    // chunks of this CTA: past rows (or the listed blocks' rows; none where k_cache_attention_tc has them), then the
+    // tokens' own rows
     const int sub = BLOCKS ? a.block / KV_CHUNK : 1;
-    const int n_pc = BLOCKS ? a.list_n[prob] * sub : (n_past + KV_CHUNK - 1) / KV_CHUNK;
+    const int n_pc = BLOCKS ? a.list_n[prob] * sub : a.tc_splits ? 0 : (n_past + KV_CHUNK - 1) / KV_CHUNK;
     const int n_chunks = n_pc + (a.m + KV_CHUNK - 1) / KV_CHUNK;
-    const int c_end = (int)((int64_t)n_chunks * (split + 1) / a.splits);
-    const int c_first = (int)((int64_t)n_chunks * split / a.splits) + warp;
+    const int c_end = (int)((int64_t)n_chunks * (split + 1) / gridDim.x);
+    const int c_first = (int)((int64_t)n_chunks * split / gridDim.x) + warp;
     const int32_t* list = BLOCKS ? a.list + (int64_t)prob * a.list_cap : nullptr;
     auto chunk_row = [&](int c) {                      // first cache row of chunk c
         if (c >= n_pc) return n_past + (c - n_pc) * KV_CHUNK;
@@ -194,15 +160,12 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
         }
         am = warp_max(am);
         bad = __any_sync(0xffffffffu, bad);
-        // 2^e <= am < 2^(e+1); q is scaled by 2^(Q_EXP - e), exactly
-        int e = (int)(__float_as_uint(am) >> 23) - 127;
-        e = bad || am == 0.f ? Terms<KT>::Q_EXP : max(e, -100);
-        const float up = __uint_as_float((uint32_t)(127 + Terms<KT>::Q_EXP - e) << 23);
-        if (lane == 0) s_scale[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - Terms<KT>::Q_EXP + e) << 23);
+        const RowScale rs = row_scale<KT>(am, bad);
+        if (lane == 0) s_scale[r] = a.scale_log2 * rs.down;
 #pragma unroll
         for (int k = 0; k < HD / 32; ++k) {
             // lanes 2c, 2c + 1 hold the pair of dims that one fragment register packs
-            float lo = x[i][k] * up;
+            float lo = x[i][k] * rs.up;
             float hi = __shfl_down_sync(0xffffffffu, lo, 1);
             const int d = k * 32 + lane, kk = d >> 4, reg = (d >> 3) & 1, c = (d & 7) >> 1;
 #pragma unroll
@@ -319,7 +282,7 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
                 float f[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    f[i] = top[n][i] > mx[n][i] ? ex2(mx[n][i] - top[n][i]) : 1.f;
+                    f[i] = top[n][i] > mx[n][i] ? ex2f(mx[n][i] - top[n][i]) : 1.f;
                     mx[n][i] = top[n][i];
                     tot[n][i] *= f[i];
                 }
@@ -340,7 +303,7 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
 #pragma unroll
             for (int i = 0; i < 2; ++i) b[i] = mx[n][i] == -INFINITY ? 0.f : mx[n][i] - Terms<KT>::P_EXP;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = ex2(s[n][i] - b[i & 1]);
+            for (int i = 0; i < 4; ++i) s[n][i] = ex2f(s[n][i] - b[i & 1]);
             tot[n][0] += s[n][0] + s[n][2];
             tot[n][1] += s[n][1] + s[n][3];
         }
@@ -438,7 +401,7 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
             float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][r]);
-            const float f = mx[n][i] == -INFINITY ? 0.f : ex2(mx[n][i] - top);
+            const float f = mx[n][i] == -INFINITY ? 0.f : ex2f(mx[n][i] - top);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 joined[(warp * RT + r) * OP + 16 * k + (lane >> 2)] = mx[n][i] == -INFINITY ? 0.f : o[k][n][i] * f;
@@ -447,7 +410,7 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
         }
     __syncthreads();
     const bool whole = a.splits == 1 && !a.logits;     // nothing to join with: the output itself
-    const int64_t part = ((int64_t)prob * a.row_tiles + tile) * a.splits + split;
+    const int64_t part = ((int64_t)prob * a.splits + a.tc_splits + split) * a.R;
     for (int x = tid; x < RT * (HD / 4); x += W * 32) {
         const int r = x / (HD / 4), d = (x - r * (HD / 4)) * 4;
         const int row = tile * RT + r;
@@ -456,7 +419,7 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
 #pragma unroll
         for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][r]);
 #pragma unroll
-        for (int w = 0; w < W; ++w) l += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * ex2(s_m[w][r] - top);
+        for (int w = 0; w < W; ++w) l += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * ex2f(s_m[w][r] - top);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -480,8 +443,8 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
 #pragma unroll
             for (int i = 0; i < 4; ++i) op[i] = y[i];
         } else {
-            *reinterpret_cast<float4*>(a.part_o + (part * RT + r) * HD + d) = v;
-            if (d == 0) a.part_ml[part * RT + r] = make_float2(top, l);
+            *reinterpret_cast<float4*>(a.part_o + (part + row) * HD + d) = v;
+            if (d == 0) a.part_ml[part + row] = make_float2(top, l);
         }
     }
 }
@@ -491,8 +454,8 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
 // columns x split groups, eight partial rows in flight per thread. The CTAs after them take 256 cache rows of a KV
 // head each: w = sum over the head's query rows of 2^(s - M) / L in row order, one thread per cache row.
 constexpr int CB = 256, ACC_ROWS = CB, ACC_MAX_R = 512;
-static_assert(KV_SMS <= CB, "one split per thread");
-__global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int rt, int hdt, int per) {
+static_assert(KV_SMS + 1 <= CB, "one split per thread");
+__global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt, int per) {
     pdl_enter();
     __shared__ float s_f[CB];
     __shared__ float s_red[2][CB / 32];
@@ -502,16 +465,15 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int rt,
     const int n_rows = a.problems * a.R;
     if ((int)blockIdx.x < n_rows) {
         const int prob = blockIdx.x / a.R, row = blockIdx.x - prob * a.R;
-        const int tile = row / rt, r = row - tile * rt;
-        const int64_t part = ((int64_t)prob * a.row_tiles + tile) * a.splits;
-        const float2 ml = tid < a.splits ? a.part_ml[(part + tid) * rt + r] : make_float2(-INFINITY, 0.f);
+        const int64_t part = (int64_t)prob * a.splits * a.R + row;       // + split * R
+        const float2 ml = tid < a.splits ? a.part_ml[part + (int64_t)tid * a.R] : make_float2(-INFINITY, 0.f);
         const float wm = warp_max(ml.x);
         if (lane == 0) s_red[0][warp] = wm;
         __syncthreads();
         float top = s_red[0][0];
 #pragma unroll
         for (int w = 1; w < CB / 32; ++w) top = fmaxf(top, s_red[0][w]);
-        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+        const float f = ml.x == -INFINITY ? 0.f : ex2f(ml.x - top);
         s_f[tid] = f;
         const float wl = warp_sum(ml.x == -INFINITY ? 0.f : f * ml.y);
         if (lane == 0) s_red[1][warp] = wl;
@@ -522,7 +484,7 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int rt,
         const int v4 = a.hd / 4, groups = CB / v4, gi = tid / v4, c = tid - gi * v4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (gi < groups) {
-            const float* po = a.part_o + (part * rt + r) * hdt + 4 * c;
+            const float* po = a.part_o + part * hdt + 4 * c;
             for (int s0 = gi; s0 < a.splits; s0 += 8 * groups) {
                 float4 u[8];
                 float w[8];
@@ -530,9 +492,8 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int rt,
                 for (int k = 0; k < 8; ++k) {
                     const int s = s0 + k * groups;
                     w[k] = s < a.splits ? s_f[s] : 0.f;
-                    // a split that saw nothing has left zeros
-                    if (s < a.splits) u[k] = *reinterpret_cast<const float4*>(po + (int64_t)s * rt * hdt);
-                    else u[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    u[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (w[k] != 0.f) u[k] = *reinterpret_cast<const float4*>(po + (int64_t)s * a.R * hdt);
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
@@ -578,19 +539,18 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int rt,
     const float before = *acc;
     // a warp per query row: its maximum and total over the splits
     for (int row = warp; row < a.R; row += CB / 32) {
-        const int tile = row / rt, r = row - tile * rt;
-        const float2* ml = a.part_ml + ((int64_t)kv * a.row_tiles + tile) * a.splits * rt + r;
-        float2 v[(KV_SMS + 31) / 32];
+        const float2* ml = a.part_ml + (int64_t)kv * a.splits * a.R + row;
+        float2 v[(KV_SMS + 32) / 32];
         float top = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int k = 0; k < (KV_SMS + 31) / 32; ++k) {
+        for (int k = 0; k < (KV_SMS + 32) / 32; ++k) {
             const int s = lane + 32 * k;
-            v[k] = s < a.splits ? ml[(int64_t)s * rt] : make_float2(-INFINITY, 0.f);
+            v[k] = s < a.splits ? ml[(int64_t)s * a.R] : make_float2(-INFINITY, 0.f);
             top = fmaxf(top, v[k].x);
         }
         top = warp_max(top);
 #pragma unroll
-        for (int k = 0; k < (KV_SMS + 31) / 32; ++k) l += v[k].x == -INFINITY ? 0.f : ex2(v[k].x - top) * v[k].y;
+        for (int k = 0; k < (KV_SMS + 32) / 32; ++k) l += v[k].x == -INFINITY ? 0.f : ex2f(v[k].x - top) * v[k].y;
         l = warp_sum(l);
         if (lane == 0) {
             s_mr[row] = top;
@@ -606,7 +566,7 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int rt,
         for (int k = 0; k < 8; ++k) s[k] = r0 + k < a.R ? lg[(r0 + k) * a.logits_ld] : -INFINITY;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            if (r0 + k < a.R && s_ir[r0 + k] != 0.f) w += ex2(s[k] - (s_mr[r0 + k] - pe)) * s_ir[r0 + k];
+            if (r0 + k < a.R && s_ir[r0 + k] != 0.f) w += ex2f(s[k] - (s_mr[r0 + k] - pe)) * s_ir[r0 + k];
     }
     if (j < n) *acc = before + w;
 }
@@ -617,8 +577,8 @@ cudaError_t attention_go(const CacheAttn& a, cudaStream_t s) {
     static SmemLimit limit;
     cudaError_t e = limit.raise((const void*)k_cache_attention<KT, HD, NT, BLOCKS>, smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_cache_attention<KT, HD, NT, BLOCKS>, dim3(a.splits, a.row_tiles, a.problems), Plan<HD>::W * 32,
-                      smem, s, a);
+    return launch_pdl(k_cache_attention<KT, HD, NT, BLOCKS>, dim3(a.splits - a.tc_splits, a.row_tiles, a.problems),
+                      Plan<HD>::W * 32, smem, s, a);
 }
 template <typename KT, int HD, int NT> cudaError_t attention_form(const CacheAttn& a, cudaStream_t s) {
     return a.list ? attention_go<KT, HD, NT, true>(a, s) : attention_go<KT, HD, NT, false>(a, s);
@@ -657,13 +617,22 @@ int cache_splits(int hd, int problems, int row_tiles, int n_chunks) {
     return most < 1 ? 1 : most < useful ? most : useful < 1 ? 1 : useful;
 }
 
+// Splits of the past rows for the tensor-core form: one CTA per SM over KV heads and tiles of 128 query rows, each
+// with two tiles of 64 rows (one for each of its softmax groups) at least; 0: the other form takes all rows.
+int cache_tc_splits(int hd, int n_kv, int R, int64_t past_rows) {
+    if (cache_tile_dims(hd) > 128 || R <= TC_MIN_R || past_rows < TC_MIN_PAST) return 0;
+    const int64_t tiles = (past_rows + 127) / 128, most = KV_SMS / ((int64_t)n_kv * ((R + 127) / 128));
+    return (int)(most < 1 ? 1 : most < tiles ? most : tiles);
+}
+
 cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s) {
     cudaError_t e = a.bf16 ? attention_type<__nv_bfloat16>(a, s) : attention_type<__half>(a, s);
     if (e != cudaSuccess || (a.splits == 1 && !a.logits)) return e;
+    if (a.tc_splits && (e = launch_cache_attention_tc(a, s)) != cudaSuccess) return e;
     const int rows = a.n_past_dev ? a.max_rows : a.n_past + a.m;
     const int per = (rows + ACC_ROWS - 1) / ACC_ROWS;                  // accumulating CTAs of a KV head
     return launch_pdl(k_cache_combine, dim3((unsigned)(a.problems * a.R + (a.logits ? a.n_kv * per : 0))), CB, 0, s, a,
-                      cache_tile_rows(a.hd, a.R), cache_tile_dims(a.hd), per);
+                      cache_tile_dims(a.hd), per);
 }
 
 }  // namespace hoard

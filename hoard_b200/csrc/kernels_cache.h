@@ -9,6 +9,8 @@ namespace hoard {
 
 constexpr int KV_SMS = 148;              // B200: one split CTA per SM
 constexpr int KV_CHUNK = 16;             // rows of one step of a warp (the M of m16n8k16)
+// The tensor-core form takes the past rows where a KV head has more query rows and the past more rows than these.
+constexpr int TC_MIN_R = 32, TC_MIN_PAST = 512;
 
 // Dynamic shared memory above 48 KiB has to be allowed once for each kernel and device; asking again costs a
 // launch's time in every call.
@@ -42,10 +44,12 @@ struct CacheAttn {
     float scale_log2;                    // scale * log2(e): scores are kept in units of log2
     // A problem is the set of query rows that read the same cache rows: a KV head with the R = m * g rows of
     // its query heads, or with a block list a (token, KV head) with R = g.
-    int problems, R, row_tiles, splits;
-    // partial results of each (problem, row tile, split): unnormalised sums, running maxima and totals
-    float* part_o;                       // [problems * row_tiles][splits][tile rows][tile dims]
-    float2* part_ml;                     // [problems * row_tiles][splits][tile rows]
+    // The first tc_splits of the splits are k_cache_attention_tc's, over the past rows; the rest, over all rows or with
+    // tc_splits over the tokens' own, k_cache_attention's.
+    int problems, R, row_tiles, splits, tc_splits;
+    // partial results of each (problem, split, query row): unnormalised sums, running maxima and totals
+    float* part_o;                       // [problems][splits][R][tile dims]
+    float2* part_ml;                     // [problems][splits][R]
     float* logits;                       // optional [n_kv][R][logits_ld], in log2 units
     int64_t logits_ld;
     float* acc;                          // optional [n_kv][max_rows]
@@ -59,7 +63,9 @@ struct CacheAttn {
 int cache_tile_rows(int hd, int R);
 int cache_tile_dims(int hd);
 int cache_splits(int hd, int problems, int row_tiles, int n_chunks);
+int cache_tc_splits(int hd, int n_kv, int R, int64_t past_rows);
 cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s);
+cudaError_t launch_cache_attention_tc(const CacheAttn& a, cudaStream_t s);
 
 struct CacheEvict {
     void *kc, *vc;

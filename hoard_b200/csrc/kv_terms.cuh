@@ -1,0 +1,57 @@
+// kv_terms.cuh -- f32 values as sums of f16 or bf16 terms, for matrix instructions on a cache of that type.
+//
+// Two f16 terms hold 22 bits of a value, three bf16 terms 24. For f16 the rows of q are scaled by a power of two to
+// [2^13, 2^14) and softmax weights by 2^14, which keeps the terms out of f16's subnormal range; the factors are taken
+// out of the scores (exactly) and cancel between the weighted sum and the total.
+#pragma once
+#include "common.cuh"
+
+namespace hoard {
+
+template <typename KT> struct Terms;
+template <> struct Terms<__half> {
+    static constexpr int N = 2, Q_EXP = 13;
+    static constexpr float P_EXP = 14.f;
+    static constexpr uint32_t INF2 = 0x7C007C00u;        // exponent bits of two values
+};
+template <> struct Terms<__nv_bfloat16> {
+    static constexpr int N = 3, Q_EXP = 0;
+    static constexpr float P_EXP = 0.f;
+    static constexpr uint32_t INF2 = 0x7F807F80u;
+};
+
+// two f32 -> packed terms: a's rounding in the low half, b's in the high half; a and b become the remainders
+template <typename KT> __device__ __forceinline__ uint32_t take_term(float& a, float& b);
+template <> __device__ __forceinline__ uint32_t take_term<__half>(float& a, float& b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    a -= f.x;
+    b -= f.y;
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t take_term<__nv_bfloat16>(float& a, float& b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    a -= f.x;
+    b -= f.y;
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The power of two that brings a row with largest magnitude am (2^e <= am < 2^(e + 1)) to exponent Q_EXP, and its
+// inverse. Rows of zeros, and rows with infinities or NaN (bad), are left as they are.
+struct RowScale {
+    float up, down;
+};
+template <typename KT> __device__ __forceinline__ RowScale row_scale(float am, bool bad) {
+    int e = (int)(__float_as_uint(am) >> 23) - 127;
+    e = bad || am == 0.f ? Terms<KT>::Q_EXP : max(e, -100);
+    return {__uint_as_float((uint32_t)(127 + Terms<KT>::Q_EXP - e) << 23),
+            __uint_as_float((uint32_t)(127 - Terms<KT>::Q_EXP + e) << 23)};
+}
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace hoard
