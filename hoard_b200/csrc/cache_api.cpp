@@ -59,7 +59,7 @@ Ws ws_plan(const hoard_kv_desc* d) {
     Ws w{};
     const int g = d->n_head / d->n_head_kv, hdt = cache_tile_dims(d->head_dim);
     // problems x row tiles x splits is at most one CTA per SM, or one split each where there are more tiles; the
-    // tensor-core form has tiles of 128 rows and the own rows' split beside them
+    // tensor-core form has tiles of 128 rows
     const int64_t R = (int64_t)d->max_tokens * g;
     const int rt = cache_tile_rows(d->head_dim, (int)R), rt1 = cache_tile_rows(d->head_dim, g);
     int64_t dense = d->n_head_kv * ceil_div(R, rt);
@@ -68,7 +68,7 @@ Ws ws_plan(const hoard_kv_desc* d) {
     lists = d->block ? (lists > KV_SMS ? lists : KV_SMS) * rt1 : 0;
     if (R > TC_MIN_R && hdt <= 128) {
         int64_t tc = d->n_head_kv * ceil_div(R, 128);
-        tc = (tc > KV_SMS ? tc : KV_SMS) * 128 + d->n_head_kv * R;
+        tc = (tc > KV_SMS ? tc : KV_SMS) * 128;
         if (tc > dense) dense = tc;
     }
     const int64_t rows = dense > lists ? dense : lists;
@@ -170,7 +170,7 @@ int hoard_kv_attention(const hoard_kv_desc* d, const hoard_kv_query* a, float* a
     const int64_t past = c.n_past_dev ? c.max_rows - c.m : c.n_past;
     if (!acc) c.tc_splits = cache_tc_splits(c.hd, c.n_kv, c.R, past);
     plan_splits(c, chunks_of(c, past));
-    if (c.tc_splits) c.splits = c.tc_splits + 1;
+    if (c.tc_splits) c.splits = c.tc_splits;
     return st(launch_cache_attention(c, (cudaStream_t)stream));
 }
 

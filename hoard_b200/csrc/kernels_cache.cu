@@ -22,10 +22,6 @@ namespace hoard {
 
 namespace {
 
-template <typename KT> __device__ __forceinline__ float kv_lo(uint32_t w);
-template <> __device__ __forceinline__ float kv_lo<__half>(uint32_t w) { return h2f(w); }
-template <> __device__ __forceinline__ float kv_lo<__nv_bfloat16>(uint32_t w) { return __uint_as_float(w << 16); }
-
 template <typename KT>
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
     if constexpr (sizeof(KT) == 2 && Terms<KT>::N == 2)
@@ -93,10 +89,9 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
     const int t0 = BLOCKS ? prob - kv * a.m : 0;       // first token of the problem's rows
     uint32_t* qf = reinterpret_cast<uint32_t*>(smem + Plan<HD>::RING);
 
-    // chunks of this CTA: past rows (or the listed blocks' rows; none where k_cache_attention_tc has them), then the
-    // tokens' own rows
+    // chunks of this CTA: past rows (or the listed blocks' rows), then the tokens' own rows
     const int sub = BLOCKS ? a.block / KV_CHUNK : 1;
-    const int n_pc = BLOCKS ? a.list_n[prob] * sub : a.tc_splits ? 0 : (n_past + KV_CHUNK - 1) / KV_CHUNK;
+    const int n_pc = BLOCKS ? a.list_n[prob] * sub : (n_past + KV_CHUNK - 1) / KV_CHUNK;
     const int n_chunks = n_pc + (a.m + KV_CHUNK - 1) / KV_CHUNK;
     const int c_end = (int)((int64_t)n_chunks * (split + 1) / gridDim.x);
     const int c_first = (int)((int64_t)n_chunks * split / gridDim.x) + warp;
@@ -315,10 +310,7 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
                 asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                              : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(vs + i * 16) : "memory");
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t e = w[k] & Terms<KT>::INF2;
-                    odd |= (e & 0xFFFFu) == (Terms<KT>::INF2 & 0xFFFFu) || (e >> 16) == (Terms<KT>::INF2 >> 16);
-                }
+                for (int k = 0; k < 4; ++k) odd |= odd_pair<KT>(w[k]);
             }
             odd = __any_sync(0xffffffffu, odd);
         }
@@ -410,7 +402,7 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
         }
     __syncthreads();
     const bool whole = a.splits == 1 && !a.logits;     // nothing to join with: the output itself
-    const int64_t part = ((int64_t)prob * a.splits + a.tc_splits + split) * a.R;
+    const int64_t part = ((int64_t)prob * a.splits + split) * a.R;
     for (int x = tid; x < RT * (HD / 4); x += W * 32) {
         const int r = x / (HD / 4), d = (x - r * (HD / 4)) * 4;
         const int row = tile * RT + r;
@@ -439,9 +431,7 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
 #pragma unroll
                 for (int i = 0; i < 4; ++i) y[i] *= sigmoid_f(gp[i]);
             }
-            float* op = a.out + ((int64_t)t * a.n_head + h) * a.hd + d;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) op[i] = y[i];
+            store4(a.out + ((int64_t)t * a.n_head + h) * a.hd + d, y);
         } else {
             *reinterpret_cast<float4*>(a.part_o + (part + row) * HD + d) = v;
             if (d == 0) a.part_ml[part + row] = make_float2(top, l);
@@ -524,9 +514,7 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
 #pragma unroll
                 for (int i = 0; i < 4; ++i) y[i] *= sigmoid_f(gp[i]);
             }
-            float* op = a.out + ((int64_t)t * a.n_head + h) * a.hd + 4 * c;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) op[i] = y[i];
+            store4(a.out + ((int64_t)t * a.n_head + h) * a.hd + 4 * c, y);
         }
         return;
     }
@@ -577,7 +565,7 @@ cudaError_t attention_go(const CacheAttn& a, cudaStream_t s) {
     static SmemLimit limit;
     cudaError_t e = limit.raise((const void*)k_cache_attention<KT, HD, NT, BLOCKS>, smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_cache_attention<KT, HD, NT, BLOCKS>, dim3(a.splits - a.tc_splits, a.row_tiles, a.problems),
+    return launch_pdl(k_cache_attention<KT, HD, NT, BLOCKS>, dim3(a.splits, a.row_tiles, a.problems),
                       Plan<HD>::W * 32, smem, s, a);
 }
 template <typename KT, int HD, int NT> cudaError_t attention_form(const CacheAttn& a, cudaStream_t s) {
@@ -617,18 +605,20 @@ int cache_splits(int hd, int problems, int row_tiles, int n_chunks) {
     return most < 1 ? 1 : most < useful ? most : useful < 1 ? 1 : useful;
 }
 
-// Splits of the past rows for the tensor-core form: one CTA per SM over KV heads and tiles of 128 query rows, each
-// with two tiles of 64 rows (one for each of its softmax groups) at least; 0: the other form takes all rows.
+// Splits for the tensor-core form: one CTA per SM over KV heads and tiles of 128 query rows, each with TC_MIN_TILES
+// tiles of 64 rows at least; 0: the other form runs the call.
 int cache_tc_splits(int hd, int n_kv, int R, int64_t past_rows) {
     if (cache_tile_dims(hd) > 128 || R <= TC_MIN_R || past_rows < TC_MIN_PAST) return 0;
-    const int64_t tiles = (past_rows + 127) / 128, most = KV_SMS / ((int64_t)n_kv * ((R + 127) / 128));
-    return (int)(most < 1 ? 1 : most < tiles ? most : tiles);
+    const int64_t tiles = (past_rows + 63) / 64 + 1, few = (tiles + TC_MIN_TILES - 1) / TC_MIN_TILES;
+    const int64_t most = KV_SMS / ((int64_t)n_kv * ((R + 127) / 128));
+    return (int)(most < 1 ? 1 : most < few ? most : few);
 }
 
 cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s) {
-    cudaError_t e = a.bf16 ? attention_type<__nv_bfloat16>(a, s) : attention_type<__half>(a, s);
+    const cudaError_t e = a.tc_splits ? launch_cache_attention_tc(a, s)
+                          : a.bf16    ? attention_type<__nv_bfloat16>(a, s)
+                                      : attention_type<__half>(a, s);
     if (e != cudaSuccess || (a.splits == 1 && !a.logits)) return e;
-    if (a.tc_splits && (e = launch_cache_attention_tc(a, s)) != cudaSuccess) return e;
     const int rows = a.n_past_dev ? a.max_rows : a.n_past + a.m;
     const int per = (rows + ACC_ROWS - 1) / ACC_ROWS;                  // accumulating CTAs of a KV head
     return launch_pdl(k_cache_combine, dim3((unsigned)(a.problems * a.R + (a.logits ? a.n_kv * per : 0))), CB, 0, s, a,

@@ -9,8 +9,8 @@ namespace hoard {
 
 constexpr int KV_SMS = 148;              // B200: one split CTA per SM
 constexpr int KV_CHUNK = 16;             // rows of one step of a warp (the M of m16n8k16)
-// The tensor-core form takes the past rows where a KV head has more query rows and the past more rows than these.
-constexpr int TC_MIN_R = 32, TC_MIN_PAST = 512;
+// The tensor-core form runs where a KV head has more query rows and the past more rows than these.
+constexpr int TC_MIN_R = 32, TC_MIN_PAST = 512, TC_MIN_TILES = 2;
 
 // Dynamic shared memory above 48 KiB has to be allowed once for each kernel and device; asking again costs a
 // launch's time in every call.
@@ -44,9 +44,8 @@ struct CacheAttn {
     float scale_log2;                    // scale * log2(e): scores are kept in units of log2
     // A problem is the set of query rows that read the same cache rows: a KV head with the R = m * g rows of
     // its query heads, or with a block list a (token, KV head) with R = g.
-    // The first tc_splits of the splits are k_cache_attention_tc's, over the past rows; the rest, over all rows or with
-    // tc_splits over the tokens' own, k_cache_attention's.
-    int problems, R, row_tiles, splits, tc_splits;
+    int problems, R, row_tiles, splits;
+    int tc_splits;                       // splits of the tensor-core form, 0 where it does not run
     // partial results of each (problem, split, query row): unnormalised sums, running maxima and totals
     float* part_o;                       // [problems][splits][R][tile dims]
     float2* part_ml;                     // [problems][splits][R]

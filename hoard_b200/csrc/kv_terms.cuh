@@ -37,6 +37,16 @@ template <> __device__ __forceinline__ uint32_t take_term<__nv_bfloat16>(float& 
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+template <typename KT> __device__ __forceinline__ float kv_lo(uint32_t w);
+template <> __device__ __forceinline__ float kv_lo<__half>(uint32_t w) { return h2f(w); }
+template <> __device__ __forceinline__ float kv_lo<__nv_bfloat16>(uint32_t w) { return __uint_as_float(w << 16); }
+
+// whether either of two packed values is an infinity or NaN
+template <typename KT> __device__ __forceinline__ bool odd_pair(uint32_t w) {
+    const uint32_t e = w & Terms<KT>::INF2;
+    return (e & 0xFFFFu) == (Terms<KT>::INF2 & 0xFFFFu) || (e >> 16) == (Terms<KT>::INF2 >> 16);
+}
+
 // The power of two that brings a row with largest magnitude am (2^e <= am < 2^(e + 1)) to exponent Q_EXP, and its
 // inverse. Rows of zeros, and rows with infinities or NaN (bad), are left as they are.
 struct RowScale {
@@ -47,6 +57,15 @@ template <typename KT> __device__ __forceinline__ RowScale row_scale(float am, b
     e = bad || am == 0.f ? Terms<KT>::Q_EXP : max(e, -100);
     return {__uint_as_float((uint32_t)(127 + Terms<KT>::Q_EXP - e) << 23),
             __uint_as_float((uint32_t)(127 - Terms<KT>::Q_EXP + e) << 23)};
+}
+// four floats to an address of any alignment that floats have
+__device__ __forceinline__ void store4(float* p, const float* v) {
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = v[i];
+    }
 }
 __device__ __forceinline__ float ex2f(float x) {
     float y;
