@@ -58,20 +58,12 @@ struct Ws {
 Ws ws_plan(const hoard_kv_desc* d) {
     Ws w{};
     const int g = d->n_head / d->n_head_kv, hdt = cache_tile_dims(d->head_dim);
-    // problems x row tiles x splits is at most one CTA per SM, or one split each where there are more tiles; the
-    // tensor-core form has tiles of 128 rows
+    // partial results exist where there are splits: then problems x row tiles x splits is at most one CTA per SM, with
+    // tiles of 16 query rows or in the tensor-core form 128; a call that accumulates has them without splits too
     const int64_t R = (int64_t)d->max_tokens * g;
-    const int rt = cache_tile_rows(d->head_dim, (int)R), rt1 = cache_tile_rows(d->head_dim, g);
-    int64_t dense = d->n_head_kv * ceil_div(R, rt);
-    int64_t lists = d->block ? (int64_t)d->n_head_kv * d->max_tokens * ceil_div(g, rt1) : 0;
-    dense = (dense > KV_SMS ? dense : KV_SMS) * rt;
-    lists = d->block ? (lists > KV_SMS ? lists : KV_SMS) * rt1 : 0;
-    if (R > TC_MIN_R && hdt <= 128) {
-        int64_t tc = d->n_head_kv * ceil_div(R, 128);
-        tc = (tc > KV_SMS ? tc : KV_SMS) * 128;
-        if (tc > dense) dense = tc;
-    }
-    const int64_t rows = dense > lists ? dense : lists;
+    int64_t rows = KV_SMS * 16;
+    if (R > TC_MIN_R && hdt <= 128) rows = KV_SMS * 128;
+    if (rows < (int64_t)d->max_acc_tokens * d->n_head) rows = (int64_t)d->max_acc_tokens * d->n_head;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t o = at;
@@ -138,11 +130,6 @@ CacheAttn attn_of(const hoard_kv_desc* d, const hoard_kv_query* a) {
 int chunks_of(const CacheAttn& c, int64_t past_rows) {
     return (int)(ceil_div(past_rows, KV_CHUNK) + ceil_div(c.m, KV_CHUNK));
 }
-void plan_splits(CacheAttn& c, int n_chunks) {
-    c.row_tiles = (int)ceil_div(c.R, cache_tile_rows(c.hd, c.R));
-    c.splits = cache_splits(c.hd, c.problems, c.row_tiles, n_chunks);
-}
-
 }  // namespace
 
 extern "C" {
@@ -169,8 +156,8 @@ int hoard_kv_attention(const hoard_kv_desc* d, const hoard_kv_query* a, float* a
     }
     const int64_t past = c.n_past_dev ? c.max_rows - c.m : c.n_past;
     if (!acc) c.tc_splits = cache_tc_splits(c.hd, c.n_kv, c.R, past);
-    plan_splits(c, chunks_of(c, past));
     if (c.tc_splits) c.splits = c.tc_splits;
+    else cache_plan(c, chunks_of(c, past), acc != nullptr);
     return st(launch_cache_attention(c, (cudaStream_t)stream));
 }
 
@@ -258,7 +245,7 @@ int hoard_kv_block_attention(const hoard_kv_desc* d, const hoard_kv_query* a, co
     c.block = d->block;
     int64_t blocks = (int64_t)s.n_sink + s.n_local + n_sel;
     if (blocks > nb_most) blocks = nb_most;
-    plan_splits(c, chunks_of(c, blocks * d->block));
+    cache_plan(c, chunks_of(c, blocks * d->block), false);
     return st(launch_cache_attention(c, (cudaStream_t)stream));
 }
 

@@ -53,13 +53,13 @@ __device__ __forceinline__ void cp16z(unsigned dst, const void* src, bool there)
 template <int N> __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// Warps and ring stages of one CTA (one CTA per SM): with head_dim 128 a stage is 16 rows of K and V, 8 KiB,
-// and eight warps keep two stages each in flight, 128 KiB per SM, while they work on a third.
+// Warps and ring slots of one CTA (one CTA per SM). A slot is the K or the V of 16 rows; eight warps with all but one
+// of their slots in flight keep 128 to 160 KiB per SM on the way.
+constexpr int W = 8;
 template <int HD> struct Plan {
-    static constexpr int W = HD == 256 ? 4 : 8;
-    static constexpr int ST = HD == 64 ? 4 : 3;
-    static constexpr int STAGE = 2 * KV_CHUNK * HD * 2;            // bytes
-    static constexpr int RING = W * ST * STAGE;
+    static constexpr int NS = HD == 256 ? 3 : 6;
+    static constexpr int SLOT = KV_CHUNK * HD * 2;                 // bytes
+    static constexpr int RING = W * NS * SLOT;
 };
 template <typename KT, int HD, int NT> constexpr int q_bytes() { return HD / 16 * NT * Terms<KT>::N * 32 * 8; }
 template <typename KT, int HD, int NT> constexpr int attn_smem() {
@@ -71,8 +71,8 @@ __device__ __forceinline__ int past_rows(const CacheAttn& a) {
 }
 
 template <typename KT, int HD, int NT, bool BLOCKS>
-__global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const CacheAttn a) {
-    constexpr int W = Plan<HD>::W, ST = Plan<HD>::ST, TN = Terms<KT>::N;
+__global__ void __launch_bounds__(W * 32, 1) k_cache_attention(const CacheAttn a) {
+    constexpr int NS = Plan<HD>::NS, SLOT = Plan<HD>::SLOT, TN = Terms<KT>::N;
     constexpr int KS = HD / 16;                        // K steps of q . K = M tiles of V^T
     constexpr int RT = 8 * NT;                         // query rows of the tile
     constexpr int PITCH = HD * 2;                      // bytes of a staged row
@@ -104,27 +104,29 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
     auto chunk_end = [&](int c) { return c >= n_pc ? n_past + a.m : n_past; };
 
     // the warp's ring; lane -> (row of the piece, 16-byte piece) with consecutive lanes on consecutive pieces
-    const unsigned ring = smem_u32(smem) + warp * ST * Plan<HD>::STAGE;
-    const char* kbase = reinterpret_cast<const char*>(a.kc) + (int64_t)kv * a.hs * 2;
-    const char* vbase = reinterpret_cast<const char*>(a.vc) + (int64_t)kv * a.hs * 2;
-    auto issue = [&](int c, int stage) {
-        const int row0 = chunk_row(c), end = chunk_end(c);
-        const unsigned dst0 = ring + stage * Plan<HD>::STAGE;
+    const unsigned ring = smem_u32(smem) + warp * NS * SLOT;
+    const int n_mine = c_first < c_end ? (c_end - c_first + W - 1) / W : 0;      // chunks of this warp
+    // slot load i: K (i even) or V of the warp's chunk i / 2, into ring slot i % NS
+    int load = 0, load_slot = 0;
+    auto issue = [&]() {
+        if (load < 2 * n_mine) {
+            const int c = c_first + (load >> 1) * W, row0 = chunk_row(c), end = chunk_end(c);
+            const char* base = static_cast<const char*>(load & 1 ? a.vc : a.kc) + (int64_t)kv * a.hs * 2;
+            const unsigned dst = ring + load_slot * SLOT;
 #pragma unroll
-        for (int i = 0; i < KV_CHUNK * C16 / 32; ++i) {
-            const int p = i * 32 + lane, r = p / C16, c16 = p % C16;
-            const bool there = row0 + r < end && c16 * 8 < a.hd;
-            const int64_t off = there ? (int64_t)(row0 + r) * a.rs * 2 + c16 * 16 : 0;
-            const unsigned dst = dst0 + r * PITCH + ((c16 ^ (r & 7)) << 4);
-            cp16z(dst, kbase + off, there);
-            cp16z(dst + KV_CHUNK * PITCH, vbase + off, there);
+            for (int i = 0; i < KV_CHUNK * C16 / 32; ++i) {
+                const int p = i * 32 + lane, r = p / C16, c16 = p % C16;
+                const bool there = row0 + r < end && c16 * 8 < a.hd;
+                cp16z(dst + r * PITCH + ((c16 ^ (r & 7)) << 4),
+                      there ? base + (int64_t)(row0 + r) * a.rs * 2 + c16 * 16 : base, there);
+            }
         }
-    };
-#pragma unroll
-    for (int s = 0; s < ST - 1; ++s) {
-        if (c_first + s * W < c_end) issue(c_first + s * W, s);
         cp_async_commit();
-    }
+        ++load;
+        load_slot = load_slot == NS - 1 ? 0 : load_slot + 1;
+    };
+#pragma unroll 1
+    for (int i = 0; i < NS - 1; ++i) issue();
 
     // the tile's q rows as fragments of the B operand: [K step][8-row tile][term][lane] of 8 bytes. A warp takes
     // every W-th row and loads all of them before it uses the first
@@ -194,17 +196,19 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
             for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
     }
 
-    int stage = 0;
-    for (int c = c_first; c < c_end; c += W) {
-        cp_wait<ST - 2>();
+    int slot = 0;                                      // ring slot of the next K or V
+    // the next slot's bytes have arrived; the slot before it is free and takes the next load
+    auto next_slot = [&]() {
+        cp_wait<NS - 2>();
         __syncwarp();
-        {
-            const int nx = c + (ST - 1) * W;
-            const int ns = stage == 0 ? ST - 1 : stage - 1;
-            if (nx < c_end) issue(nx, ns);
-            cp_async_commit();
-        }
-        const unsigned ks = ring + stage * Plan<HD>::STAGE, vs = ks + KV_CHUNK * PITCH;
+        issue();
+        const unsigned at = ring + slot * SLOT;
+        slot = slot == NS - 1 ? 0 : slot + 1;
+        return at;
+    };
+#pragma unroll 1
+    for (int c = c_first; c < c_end; c += W) {
+        const unsigned ks = next_slot();
         // ---- S^T = K q^T: each K step's products by matrix instructions, added with rounding (the instructions
         // truncate as they accumulate), which also leaves no chain of instructions longer than the terms ----
         float s[NT][4];
@@ -302,6 +306,7 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
             tot[n][0] += s[n][0] + s[n][2];
             tot[n][1] += s[n][1] + s[n][3];
         }
+        const unsigned vs = next_slot();
         // masked own rows may hold infinities or NaN (0 * inf): such a chunk takes its products one by one
         bool odd = false;
         if (own) {
@@ -361,7 +366,6 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
                 }
             }
         }
-        stage = stage == ST - 1 ? 0 : stage + 1;
     }
     cp_async_wait_all();
 
@@ -440,21 +444,21 @@ __global__ void __launch_bounds__(Plan<HD>::W * 32, 1) k_cache_attention(const C
 }
 
 // ---- joins the splits of every query row, and with acc adds the rows' weights to the accumulated ones -------
-// A CTA per query row (token, head): the factors 2^(m_s - M) of the splits, one split per thread, then float4
-// columns x split groups, eight partial rows in flight per thread. The CTAs after them take 256 cache rows of a KV
-// head each: w = sum over the head's query rows of 2^(s - M) / L in row order, one thread per cache row.
-constexpr int CB = 256, ACC_ROWS = CB, ACC_MAX_R = 512;
+// A CTA per query row (token, head) and block of columns (one block where there are rows enough): the factors 2^(m_s - M) of the splits, one split per thread, then float4
+// columns x split groups, eight partial rows in flight per thread. The CTAs after them take 1024 cache rows of a KV
+// head each: w = sum over the head's query rows of 2^(s - M) / L in row order, four cache rows per thread.
+constexpr int CB = 256, ACC_PER = 4, ACC_ROWS = CB * ACC_PER, ACC_MAX_R = 512;
 static_assert(KV_SMS + 1 <= CB, "one split per thread");
-__global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt, int per) {
+__global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt, int col_blocks, int per) {
     pdl_enter();
     __shared__ float s_f[CB];
     __shared__ float s_red[2][CB / 32];
     __shared__ float4 s_o[CB];
     __shared__ float s_mr[ACC_MAX_R], s_ir[ACC_MAX_R];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int n_rows = a.problems * a.R;
+    const int n_rows = a.problems * a.R * col_blocks;
     if ((int)blockIdx.x < n_rows) {
-        const int prob = blockIdx.x / a.R, row = blockIdx.x - prob * a.R;
+        const int at = blockIdx.x / col_blocks, prob = at / a.R, row = at - prob * a.R;
         const int64_t part = (int64_t)prob * a.splits * a.R + row;       // + split * R
         const float2 ml = tid < a.splits ? a.part_ml[part + (int64_t)tid * a.R] : make_float2(-INFINITY, 0.f);
         const float wm = warp_max(ml.x);
@@ -471,9 +475,11 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
         float l = s_red[1][0];
 #pragma unroll
         for (int w = 1; w < CB / 32; ++w) l += s_red[1][w];
-        const int v4 = a.hd / 4, groups = CB / v4, gi = tid / v4, c = tid - gi * v4;
+        // this CTA's float4 columns, shared out over split groups
+        const int v4 = (a.hd / 4 + col_blocks - 1) / col_blocks, groups = CB / v4, gi = tid / v4;
+        const int lc = tid - gi * v4, c = (blockIdx.x - at * col_blocks) * v4 + lc;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (gi < groups) {
+        if (gi < groups && 4 * c < a.hd) {
             const float* po = a.part_o + part * hdt + 4 * c;
             for (int s0 = gi; s0 < a.splits; s0 += 8 * groups) {
                 float4 u[8];
@@ -496,9 +502,9 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
             s_o[tid] = v;
         }
         __syncthreads();
-        if (gi == 0) {
+        if (gi == 0 && 4 * c < a.hd) {
             for (int k = 1; k < groups; ++k) {
-                const float4 u = s_o[k * v4 + c];
+                const float4 u = s_o[k * v4 + lc];
                 v.x += u.x;
                 v.y += u.y;
                 v.z += u.z;
@@ -520,11 +526,13 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
     }
     // accumulation
     const int n = past_rows(a) + a.m;
-    const int x = blockIdx.x - n_rows, kv = x / per, j = (x - kv * per) * ACC_ROWS + tid;
-    if (j - tid >= n) return;
-    const float* lg = a.logits + (int64_t)kv * a.R * a.logits_ld + min(j, n - 1);
-    float* acc = a.acc + (int64_t)kv * a.max_rows + min(j, n - 1);
-    const float before = *acc;
+    const int x = blockIdx.x - n_rows, kv = x / per, j0 = (x - kv * per) * ACC_ROWS;
+    if (j0 >= n) return;
+    const float* lg = a.logits + (int64_t)kv * a.R * a.logits_ld;
+    float* acc = a.acc + (int64_t)kv * a.max_rows;
+    float w[ACC_PER];
+#pragma unroll
+    for (int i = 0; i < ACC_PER; ++i) w[i] = j0 + i * CB + tid < n ? acc[j0 + i * CB + tid] : 0.f;
     // a warp per query row: its maximum and total over the splits
     for (int row = warp; row < a.R; row += CB / 32) {
         const float2* ml = a.part_ml + (int64_t)kv * a.splits * a.R + row;
@@ -547,16 +555,25 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
     }
     __syncthreads();
     const float pe = a.bf16 ? Terms<__nv_bfloat16>::P_EXP : Terms<__half>::P_EXP;      // l holds 2^P_EXP sum p
-    float w = 0.f;
-    for (int r0 = 0; r0 < a.R; r0 += 8) {
-        float s[8];
+    float sum[ACC_PER] = {};
+    for (int r0 = 0; r0 < a.R; r0 += 4) {
+        float s[4][ACC_PER];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s[k] = r0 + k < a.R ? lg[(r0 + k) * a.logits_ld] : -INFINITY;
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (r0 + k < a.R && s_ir[r0 + k] != 0.f) w += ex2f(s[k] - (s_mr[r0 + k] - pe)) * s_ir[r0 + k];
+            for (int i = 0; i < ACC_PER; ++i) {
+                const int j = j0 + i * CB + tid;
+                s[k][i] = r0 + k < a.R && j < n ? lg[(r0 + k) * a.logits_ld + j] : -INFINITY;
+            }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (r0 + k < a.R && s_ir[r0 + k] != 0.f)
+#pragma unroll
+                for (int i = 0; i < ACC_PER; ++i) sum[i] += ex2f(s[k][i] - (s_mr[r0 + k] - pe)) * s_ir[r0 + k];
     }
-    if (j < n) *acc = before + w;
+#pragma unroll
+    for (int i = 0; i < ACC_PER; ++i)
+        if (j0 + i * CB + tid < n) acc[j0 + i * CB + tid] = w[i] + sum[i];
 }
 
 template <typename KT, int HD, int NT, bool BLOCKS>
@@ -566,22 +583,17 @@ cudaError_t attention_go(const CacheAttn& a, cudaStream_t s) {
     cudaError_t e = limit.raise((const void*)k_cache_attention<KT, HD, NT, BLOCKS>, smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(k_cache_attention<KT, HD, NT, BLOCKS>, dim3(a.splits, a.row_tiles, a.problems),
-                      Plan<HD>::W * 32, smem, s, a);
+                      W * 32, smem, s, a);
 }
 template <typename KT, int HD, int NT> cudaError_t attention_form(const CacheAttn& a, cudaStream_t s) {
     return a.list ? attention_go<KT, HD, NT, true>(a, s) : attention_go<KT, HD, NT, false>(a, s);
 }
 template <typename KT> cudaError_t attention_type(const CacheAttn& a, cudaStream_t s) {
-    const int nt = cache_tile_rows(a.hd, a.R) / 8;
+    const bool one = a.tile_rows == 8;
     switch (cache_tile_dims(a.hd)) {
-        case 64:
-            return nt == 1 ? attention_form<KT, 64, 1>(a, s) : nt == 2 ? attention_form<KT, 64, 2>(a, s)
-                                                                      : attention_form<KT, 64, 4>(a, s);
-        case 128:
-            return nt == 1 ? attention_form<KT, 128, 1>(a, s) : nt == 2 ? attention_form<KT, 128, 2>(a, s)
-                                                                       : attention_form<KT, 128, 4>(a, s);
-        default:
-            return nt == 1 ? attention_form<KT, 256, 1>(a, s) : attention_form<KT, 256, 2>(a, s);
+        case 64: return one ? attention_form<KT, 64, 1>(a, s) : attention_form<KT, 64, 2>(a, s);
+        case 128: return one ? attention_form<KT, 128, 1>(a, s) : attention_form<KT, 128, 2>(a, s);
+        default: return one ? attention_form<KT, 256, 1>(a, s) : attention_form<KT, 256, 2>(a, s);
     }
 }
 
@@ -589,20 +601,20 @@ template <typename KT> cudaError_t attention_type(const CacheAttn& a, cudaStream
 
 int cache_tile_dims(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
-// Query rows of a tile: the fewest multiples of 8 that hold the problem's rows, up to what the accumulators of a
-// warp (head_dim x rows f32) leave of the registers.
-int cache_tile_rows(int hd, int R) {
-    const int most = cache_tile_dims(hd) == 256 ? 16 : 32;
-    return R <= 8 ? 8 : R <= 16 ? 16 : most;
-}
-
-// Splits of the cache's chunks: one CTA per SM over all problems and row tiles, but not more than leave every
-// warp of a CTA a chunk.
-int cache_splits(int hd, int problems, int row_tiles, int n_chunks) {
-    const int w = cache_tile_dims(hd) == 256 ? 4 : 8;
-    const int most = KV_SMS / (problems * row_tiles);
-    const int useful = (n_chunks + w - 1) / w;
-    return most < 1 ? 1 : most < useful ? most : useful < 1 ? 1 : useful;
+// Query rows of a tile and splits of the chunks, for P problems of R rows over n_chunks chunks.
+// Rows: 8 or 16. Tiles of 8 have the shorter code and epilogue (one call over 40 rows 4.1 us against 5.7), tiles of 16
+// read the cache half as often: with 16 rows of 4 heads of 128, 8 against 16 take 9.1 / 9.9 us over 4000 cache
+// rows, 14.5 / 14.2 over 16000, 35.5 / 30.1 over 60000; with 16 heads 9.2 / 9.8 over 1000, 15.5 / 14.0 over 4000.
+// The two cross where a warp of a full grid has about five chunks.
+// Splits: one CTA per SM over problems and tiles, each warp with a chunk; but a second kernel to join them costs
+// 3 us, about four chunks of a warp, so up to that many one CTA takes them all (`join`: it runs anyway).
+void cache_plan(CacheAttn& a, int n_chunks, bool join) {
+    const int64_t w = W, tiles8 = (a.R + 7) / 8;
+    a.tile_rows = a.R > 8 && a.problems * tiles8 * n_chunks > 5 * w * KV_SMS ? 16 : 8;
+    a.row_tiles = (a.R + a.tile_rows - 1) / a.tile_rows;
+    const int64_t most = KV_SMS / ((int64_t)a.problems * a.row_tiles), useful = (n_chunks + w - 1) / w;
+    a.splits = (int)(most < useful ? most : useful);
+    if (a.splits < 1 || (!join && n_chunks <= 4 * w)) a.splits = 1;
 }
 
 // Splits for the tensor-core form: one CTA per SM over KV heads and tiles of 128 query rows, each with TC_MIN_TILES
@@ -621,8 +633,10 @@ cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s) {
     if (e != cudaSuccess || (a.splits == 1 && !a.logits)) return e;
     const int rows = a.n_past_dev ? a.max_rows : a.n_past + a.m;
     const int per = (rows + ACC_ROWS - 1) / ACC_ROWS;                  // accumulating CTAs of a KV head
-    return launch_pdl(k_cache_combine, dim3((unsigned)(a.problems * a.R + (a.logits ? a.n_kv * per : 0))), CB, 0, s, a,
-                      cache_tile_dims(a.hd), per);
+    const int n_rows = a.problems * a.R;
+    const int col_blocks = a.hd % 64 || n_rows > KV_SMS ? 1 : a.hd / 64;
+    return launch_pdl(k_cache_combine, dim3((unsigned)(n_rows * col_blocks + (a.logits ? a.n_kv * per : 0))), CB, 0, s, a,
+                      cache_tile_dims(a.hd), col_blocks, per);
 }
 
 }  // namespace hoard

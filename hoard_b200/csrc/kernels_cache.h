@@ -44,7 +44,7 @@ struct CacheAttn {
     float scale_log2;                    // scale * log2(e): scores are kept in units of log2
     // A problem is the set of query rows that read the same cache rows: a KV head with the R = m * g rows of
     // its query heads, or with a block list a (token, KV head) with R = g.
-    int problems, R, row_tiles, splits;
+    int problems, R, tile_rows, row_tiles, splits;
     int tc_splits;                       // splits of the tensor-core form, 0 where it does not run
     // partial results of each (problem, split, query row): unnormalised sums, running maxima and totals
     float* part_o;                       // [problems][splits][R][tile dims]
@@ -58,10 +58,8 @@ struct CacheAttn {
     int list_cap, block;
 };
 
-// Rows of a query tile, dims of the instantiation that runs a call, and split counts.
-int cache_tile_rows(int hd, int R);
-int cache_tile_dims(int hd);
-int cache_splits(int hd, int problems, int row_tiles, int n_chunks);
+int cache_tile_dims(int hd);             // dims of the instantiation that runs a head_dim
+void cache_plan(CacheAttn& a, int n_chunks, bool join);                  // sets tile_rows, row_tiles, splits
 int cache_tc_splits(int hd, int n_kv, int R, int64_t past_rows);
 cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s);
 cudaError_t launch_cache_attention_tc(const CacheAttn& a, cudaStream_t s);
