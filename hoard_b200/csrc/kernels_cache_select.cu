@@ -20,129 +20,282 @@ namespace hoard {
 namespace {
 
 constexpr int CL = 8;                    // CTAs of a cluster (the portable maximum)
-constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32;
+// 512 threads: two CTAs of a cluster fit on an SM (with 1024 they do not, and of 16 clusters some wait for a second wave:
+// 65521 rows x 16 heads took 62 us), and barriers are cheaper
+constexpr int SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32;
 constexpr int DIGIT = 11, BINS = 1 << DIGIT;
-static_assert(BINS == 2 * SEL_THREADS, "two bins per thread");
-
-// exclusive prefix sum over the CTA; total receives the sum
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* s_warp,
-                                                         unsigned long long& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto scan32 = [&](unsigned long long x) {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        return x;
-    };
-    const unsigned long long x = scan32(v);
-    __syncthreads();                     // s_warp may still be read from an earlier scan
-    if (lane == 31) s_warp[warp] = x;
-    __syncthreads();
-    const unsigned long long w = scan32(s_warp[lane]);
-    total = __shfl_sync(0xffffffffu, w, SEL_WARPS - 1);
-    const unsigned long long before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
-    return (warp ? before : 0) + x - v;
-}
 
 // Shared state of a selection
 struct Select {
     unsigned hist[2][BINS];
-    unsigned long long warp[SEL_WARPS];
-    unsigned long long ex[2];            // this CTA's totals, for prefixes over the cluster
-    unsigned bin, in_bin, above;
+    unsigned warp[2][SEL_WARPS];         // one value per warp, alternately (a scan's values may still be read)
+    unsigned seg[CL], found[3];          // cluster: segment totals; bin, count in it, count above it
+    unsigned ex[2];                      // this CTA's totals, for prefixes over the cluster
 };
 
-// exclusive prefix over the cluster's CTAs of `total` (a slot is used once, so nothing overwrites it)
-template <int CLN>
-__device__ __forceinline__ unsigned long long cluster_before(Select& s, int slot, unsigned long long total) {
-    if constexpr (CLN == 1) return 0;
-    cg::cluster_group cl = cg::this_cluster();
-    if (threadIdx.x == 0) s.ex[slot] = total;
-    cl.sync();
-    unsigned long long v[CLN], before = 0;
+// exclusive prefix sum over the CTA of one value per thread; total receives the sum. `use`: 0, 1, 0, ..
+__device__ __forceinline__ unsigned block_scan(Select& s, int use, unsigned v, unsigned& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto scan32 = [&](unsigned x) {
 #pragma unroll
-    for (int r = 0; r < CLN; ++r) v[r] = *cl.map_shared_rank(&s.ex[slot], r);
-#pragma unroll
-    for (int r = 0; r < CLN; ++r)
-        if (r < (int)cl.block_rank()) before += v[r];
-    return before;
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        return x;
+    };
+    const unsigned x = scan32(v);
+    if (lane == 31) s.warp[use][warp] = x;
+    __syncthreads();
+    const unsigned w = scan32(lane < SEL_WARPS ? s.warp[use][lane] : 0);
+    total = __shfl_sync(0xffffffffu, w, SEL_WARPS - 1);
+    const unsigned before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+    return (warp ? before : 0) + x - v;
 }
 
-// The `need` largest of the keys: afterwards a key is in if (key >> shift) > prefix, and of those with
-// (key >> shift) == prefix the first `eq_need` in index order are. key(i): this CTA's i-th key.
+// sums over the cluster's CTAs before this one and over all of `total` (a slot is used once, so nothing overwrites it)
+template <int CLN>
+__device__ __forceinline__ void cluster_sums(Select& s, int slot, unsigned total, unsigned& before, unsigned& all) {
+    before = 0;
+    all = total;
+    if constexpr (CLN > 1) {
+        cg::cluster_group cl = cg::this_cluster();
+        if (threadIdx.x == 0) s.ex[slot] = total;
+        cl.sync();
+        unsigned v[CLN];
+#pragma unroll
+        for (int r = 0; r < CLN; ++r) v[r] = *cl.map_shared_rank(&s.ex[slot], r);
+        all = 0;
+#pragma unroll
+        for (int r = 0; r < CLN; ++r) {
+            all += v[r];
+            if (r < (int)cl.block_rank()) before += v[r];
+        }
+    }
+}
+
+// Up to 32 strips of SEL_THREADS flags, bit k of a thread's mask its flag in strip k: leaves in hist[0] for each (strip,
+// warp) the number of flags before it in index order, which is also returned for (strip, warp) = thread in `at`, with
+// its own number of flags; total receives the sum. The caller synchronises before others' entries are read.
+constexpr int SPAN = 32 * SEL_THREADS;
+static_assert(32 * SEL_WARPS == SEL_THREADS, "one (strip, warp) per thread");
+__device__ __forceinline__ unsigned strip_scan(Select& s, unsigned mask, unsigned& at, unsigned& total) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned any = __reduce_or_sync(0xffffffffu, mask);
+    // lane k keeps strip k's count of this warp
+    unsigned mine = 0;
+    for (unsigned left = any; left; left &= left - 1) {
+        const int k = __ffs(left) - 1;
+        const unsigned b = __ballot_sync(0xffffffffu, mask >> k & 1);
+        if (lane == k) mine = __popc(b);
+    }
+    s.hist[0][lane * SEL_WARPS + warp] = mine;
+    __syncthreads();
+    const unsigned v = s.hist[0][tid];
+    at = block_scan(s, 1, v, total);
+    s.hist[0][tid] = at;
+    return v;
+}
+
+// The bin, counted from the top of the histogram, that holds the need-th key: its number, its count, the count above.
+// Every CTA of a cluster adds up and searches its share of the bins.
+template <int CLN>
+__device__ __forceinline__ void find_bin(Select& s, const unsigned* hist, unsigned need, unsigned& bin, unsigned& in_bin,
+                                         unsigned& above) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int SHARE = BINS / CLN, PER = CLN == 1 ? BINS / SEL_THREADS : 1, LAST = SHARE / PER;      // threads with bins
+    unsigned mine[PER] = {}, sum = 0, before = 0;
+    int top = 0;                                       // this thread's highest bin
+    if constexpr (CLN == 1) {
+        __syncthreads();
+        top = BINS - 1 - PER * threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) mine[i] = hist[top - i];
+    } else {
+        cg::cluster_group cl = cg::this_cluster();
+        cl.sync();
+        top = BINS - 1 - SHARE * (int)cl.block_rank() - threadIdx.x;
+        if (threadIdx.x < LAST) {
+            unsigned v[CLN];
+#pragma unroll
+            for (int r = 0; r < CLN; ++r) v[r] = cl.map_shared_rank(hist, r)[top];
+#pragma unroll
+            for (int r = 0; r < CLN; ++r) mine[0] += v[r];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += mine[i];
+    const unsigned in_warp = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) s.warp[0][warp] = in_warp;
+    __syncthreads();
+    // every warp: the warps' totals, and which of them holds the key
+    const unsigned w = lane < LAST / 32 ? s.warp[0][lane] : 0;
+    unsigned incl = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if constexpr (CLN > 1) {
+        cg::cluster_group cl = cg::this_cluster();
+        const unsigned total = __shfl_sync(0xffffffffu, incl, 31);
+        if (threadIdx.x < CLN) cl.map_shared_rank(s.seg, threadIdx.x)[cl.block_rank()] = total;
+        cl.sync();
+#pragma unroll
+        for (int r = 0; r < CLN; ++r)
+            if (r < (int)cl.block_rank()) before += s.seg[r];
+    }
+    const unsigned below = before + incl - w;
+    const unsigned hit = __ballot_sync(0xffffffffu, below < need && below + w >= need);
+    if (hit && warp == __ffs(hit) - 1) {
+        unsigned x = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        unsigned up = __shfl_sync(0xffffffffu, below, warp) + x - sum;           // keys above this thread's bins
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (up < need && up + mine[i] >= need) {
+                const unsigned f[3] = {(unsigned)(top - i), mine[i], up};
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+                    if constexpr (CLN == 1) s.found[k] = f[k];
+                    else
+                        for (int r = 0; r < CLN; ++r) cg::this_cluster().map_shared_rank(s.found, r)[k] = f[k];
+                }
+            }
+            up += mine[i];
+        }
+    }
+    if constexpr (CLN == 1) __syncthreads();
+    else cg::this_cluster().sync();
+    bin = s.found[0];
+    in_bin = s.found[1];
+    above = s.found[2];
+}
+
+// The `need` largest of the keys, the lower index where equal: afterwards this CTA's i-th key is in if
+// (key >> shift) > prefix, or == prefix and i <= cut. key(i): this CTA's i-th key.
 struct Threshold {
     unsigned long long prefix;
-    int shift, eq_need;
+    int shift, cut;
+    __device__ __forceinline__ bool in(unsigned long long key, int i) const {
+        const unsigned long long k = key >> shift;
+        return k > prefix || (k == prefix && i <= cut);
+    }
 };
 template <int CLN, int BITS, typename Key>
 __device__ __forceinline__ Threshold select_threshold(Select& s, Key key, int n_local, int need) {
-    unsigned long long prefix = 0;
-    int shift = BITS, buf = 0;
-    for (bool first = true;; first = false) {
-        const int width = min(DIGIT, shift);
-        shift -= width;
-        unsigned* hist = s.hist[buf];
-        hist[threadIdx.x] = 0;
-        hist[threadIdx.x + SEL_THREADS] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n_local; i += SEL_THREADS) {
+    const int tid = threadIdx.x;
+    for (int i = tid; i < 2 * BINS; i += SEL_THREADS) s.hist[0][i] = 0;
+    __syncthreads();
+    Threshold th{0, BITS, 0x7fffffff};
+    for (int pass = 0;; ++pass) {
+        const int width = min(DIGIT, th.shift);
+        th.shift -= width;
+        unsigned* hist = s.hist[pass & 1];
+        for (int i = tid; i < n_local; i += SEL_THREADS) {
             const unsigned long long k = key(i);
-            const unsigned d = (unsigned)(k >> shift) & ((1u << width) - 1);
-            if (first) {                 // exponents: few bins, so a warp's equal ones are added at once
-                const unsigned act = __activemask(), same = __match_any_sync(act, d);
-                if ((int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&hist[d], (unsigned)__popc(same));
-            } else if ((k >> (shift + width)) == prefix) {
-                atomicAdd(&hist[d], 1u);
-            }
+            const unsigned d = (unsigned)(k >> th.shift) & ((1u << width) - 1);
+            if (pass == 0 || (k >> (th.shift + width)) == th.prefix) atomicAdd(&hist[d], 1u);
         }
-        // thread i: bins BINS - 1 - 2i and BINS - 2 - 2i, so that the scan runs from the top
-        unsigned hi = 0, lo = 0;
-        if constexpr (CLN == 1) {
-            __syncthreads();
-            const uint2 h = *reinterpret_cast<const uint2*>(hist + BINS - 2 - 2 * threadIdx.x);
-            lo = h.x;
-            hi = h.y;
-        } else {
-            cg::cluster_group cl = cg::this_cluster();
-            cl.sync();
-            uint2 h[CLN];
-#pragma unroll
-            for (int r = 0; r < CLN; ++r)
-                h[r] = *reinterpret_cast<const uint2*>(cl.map_shared_rank(hist, r) + BINS - 2 - 2 * threadIdx.x);
-#pragma unroll
-            for (int r = 0; r < CLN; ++r) {
-                lo += h[r].x;
-                hi += h[r].y;
-            }
+        unsigned bin, in_bin, above;
+        find_bin<CLN>(s, hist, (unsigned)need, bin, in_bin, above);
+        th.prefix = th.prefix << width | bin;
+        need -= (int)above;
+        if (in_bin == (unsigned)need) return th;
+        if (th.shift == 0) break;
+        // the next pass's counts are zero already; these are made so for the pass after it
+        for (int i = tid; i < BINS; i += SEL_THREADS) hist[i] = 0;
+    }
+    // more equal keys than are wanted: the index of the need-th of them
+    unsigned mine = 0, total, before, all;
+    for (int i = tid; i < n_local; i += SEL_THREADS) mine += key(i) == th.prefix;
+    block_scan(s, 0, mine, total);
+    cluster_sums<CLN>(s, 0, total, before, all);
+    if (before + total <= (unsigned)need) return th;   // uniform over the CTA
+    th.cut = -1;
+    if (before >= (unsigned)need) return th;
+    for (int i0 = 0; i0 < n_local; i0 += SPAN) {
+        unsigned mask = 0, at;
+        for (int k = 0; k < 32 && i0 + k * SEL_THREADS < n_local; ++k) {
+            const int i = i0 + k * SEL_THREADS + tid;
+            mask |= (unsigned)(i < n_local && key(i) == th.prefix) << k;
         }
-        unsigned long long total;
-        const unsigned above = (unsigned)block_scan(hi + lo, s.warp, total), n = (unsigned)need;
-        if (above < n && above + hi >= n) {
-            s.bin = BINS - 1 - 2 * threadIdx.x;
-            s.in_bin = hi;
-            s.above = above;
-        } else if (above + hi < n && above + hi + lo >= n) {
-            s.bin = BINS - 2 - 2 * threadIdx.x;
-            s.in_bin = lo;
-            s.above = above + hi;
+        const unsigned v = strip_scan(s, mask, at, total), x = (unsigned)need - 1 - before;
+        if (at <= x && x < at + v) {                   // one thread, at most: its (strip, warp) holds the key
+            s.found[0] = tid;
+            s.found[1] = x - at;
         }
         __syncthreads();
-        prefix = prefix << width | s.bin;
-        need -= (int)s.above;
-        const bool done = shift == 0 || s.in_bin == (unsigned)need;
-        __syncthreads();                 // read before the next pass writes
-        if (done) return {prefix, shift, need};
-        buf ^= 1;                        // the cluster's other CTAs may still read this pass's counts
+        if (x < total) {                               // uniform
+            const int k = s.found[0] / SEL_WARPS, w = s.found[0] % SEL_WARPS;
+            const unsigned b = __ballot_sync(0xffffffffu, mask >> k & 1), j = s.found[1];
+            if (tid >> 5 == w && (mask >> k & 1) && __popc(b & ((1u << (tid & 31)) - 1)) == (int)j)
+                s.found[2] = i0 + k * SEL_THREADS + tid;
+            __syncthreads();
+            th.cut = (int)s.found[2];
+            break;
+        }
+        before += total;
+    }
+    __syncthreads();
+    return th;
+}
+
+// Calls emit(i, rank) for every flagged index of this CTA, rank counted over the cluster in index order, after
+// begin(number of flagged ones over the cluster).
+template <int CLN, typename Flag, typename Begin, typename Emit>
+__device__ __forceinline__ void ranked(Select& s, Flag flag, int n_local, Begin begin, Emit emit) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto flags = [&](int i0) {
+        unsigned mask = 0;
+        for (int k = 0; k < 32 && i0 + k * SEL_THREADS < n_local; ++k) {
+            const int i = i0 + k * SEL_THREADS + tid;
+            mask |= (unsigned)(i < n_local && flag(i)) << k;
+        }
+        return mask;
+    };
+    auto report = [&](int i0, unsigned mask, unsigned before) {
+        for (int k = 0; k < 32 && i0 + k * SEL_THREADS < n_local; ++k) {
+            const unsigned b = __ballot_sync(0xffffffffu, mask >> k & 1);
+            if (mask >> k & 1)
+                emit(i0 + k * SEL_THREADS + tid, before + s.hist[0][k * SEL_WARPS + warp] + __popc(b & ((1u << lane) - 1)));
+        }
+    };
+    unsigned total, before, all, at;
+    if (n_local <= SPAN) {
+        const unsigned mask = flags(0);
+        strip_scan(s, mask, at, total);
+        cluster_sums<CLN>(s, 1, total, before, all);
+        begin(all);
+        __syncthreads();                               // the scan's ranks are in place
+        report(0, mask, before);
+        return;
+    }
+    unsigned mine = 0;
+    for (int i0 = 0; i0 < n_local; i0 += SPAN) mine += __popc(flags(i0));
+    __syncthreads();
+    block_scan(s, 0, mine, total);
+    cluster_sums<CLN>(s, 1, total, before, all);
+    begin(all);
+    for (int i0 = 0; i0 < n_local; i0 += SPAN) {
+        const unsigned mask = flags(i0);
+        __syncthreads();
+        strip_scan(s, mask, at, total);
+        __syncthreads();
+        report(i0, mask, before);
+        before += total;
     }
 }
 
 // ---- eviction -------------------------------------------------------------------------------------------------
 // Key of a row: protected rows above everything; weights in order; NaN below everything. -0 equals +0.
 constexpr int EV_KEYS = 40960;           // keys that a CTA holds in shared memory (160 KiB)
-constexpr int EV_SINGLE = 8192;          // rows up to which one CTA chooses alone
-constexpr int EV_FUSED = 1024;           // moves up to which that CTA makes them itself
+constexpr int EV_SINGLE = 32768;         // rows up to which one CTA chooses alone
+constexpr int EV_FUSED = 512;            // moves up to which that CTA makes them itself
 __device__ __forceinline__ unsigned evict_key(float acc, int pos, int n_sink, int recent_from) {
     if (pos < n_sink || pos >= recent_from) return 0xFFFFFFFFu;
     if (acc != acc) return 0u;
@@ -178,9 +331,8 @@ __device__ __forceinline__ void move_rows(const CacheEvict& e, int kv, const int
         e.pos_out[hb + tt] = e.pos[hb + ff];
     }
 }
-// Grid (CLN, n_kv). Lists the rows to fill and the rows to move (ascending both), writes acc_out / pos_out of the
-// kept rows that stay where they are, and makes the moves itself where there are few (to, from then sit in
-// shared memory).
+// Grid (CLN, n_kv). Lists the rows to fill and the rows to move (ascending both), copies acc and pos of the rows below
+// n_keep to their outputs, and makes the moves itself where there are few (to, from then sit in shared memory).
 template <int CLN>
 __global__ void __launch_bounds__(SEL_THREADS) k_evict_choose(const CacheEvict e, const bool fused) {
     pdl_enter();
@@ -193,6 +345,10 @@ __global__ void __launch_bounds__(SEL_THREADS) k_evict_choose(const CacheEvict e
     const int first = (int)((int64_t)e.n_rows * rank / CLN), last = (int)((int64_t)e.n_rows * (rank + 1) / CLN);
     const int n = last - first;
     const bool held = CLN == 1 || n <= EV_KEYS;
+    // rows that stay are copied where the outputs are other buffers; rows that are filled are written again, later
+    float* acc_out = e.acc_out + (int64_t)kv * e.max_rows;
+    int32_t* pos_out = e.pos_out + (int64_t)kv * e.max_rows;
+    const bool copy = e.acc_out != e.acc || e.pos_out != e.pos;
     auto fresh = [&](int i) { return evict_key(acc[first + i], pos[first + i], e.n_sink, e.recent_from); };
     if (held) {
         for (int i0 = tid; i0 < n; i0 += 8 * SEL_THREADS) {
@@ -206,58 +362,42 @@ __global__ void __launch_bounds__(SEL_THREADS) k_evict_choose(const CacheEvict e
                 }
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (i0 + k * SEL_THREADS < n) s_key[i0 + k * SEL_THREADS] = evict_key(a[k], p[k], e.n_sink, e.recent_from);
+                if (i0 + k * SEL_THREADS < n) {
+                    const int i = i0 + k * SEL_THREADS;
+                    s_key[i] = evict_key(a[k], p[k], e.n_sink, e.recent_from);
+                    if (copy && first + i < e.n_keep) {
+                        acc_out[first + i] = a[k];
+                        pos_out[first + i] = p[k];
+                    }
+                }
+        }
+    } else if (copy) {
+        for (int i = tid; i < n && first + i < e.n_keep; i += SEL_THREADS) {
+            acc_out[first + i] = acc[first + i];
+            pos_out[first + i] = pos[first + i];
         }
     }
     __syncthreads();
     auto key = [&](int i) { return held ? s_key[i] : fresh(i); };
     const Threshold th = select_threshold<CLN, 32>(sel, key, n, e.n_keep);
-
-    // a thread owns a run of rows (odd length: the runs' first words fall in different banks)
-    const int len = (n + SEL_THREADS - 1) / SEL_THREADS | 1, i0 = min(n, tid * len), i1 = min(n, i0 + len);
-    unsigned long long eq = 0, total;
-    for (int i = i0; i < i1; ++i) eq += (unsigned long long)(key(i) >> th.shift) == th.prefix;
-    unsigned long long eq_rank = block_scan(eq, sel.warp, total);
-    eq_rank += cluster_before<CLN>(sel, 0, total);
-    const unsigned long long eq_rank0 = eq_rank;
-    auto kept = [&](int i) {
-        const unsigned long long k = key(i) >> th.shift;
-        return k > th.prefix || (k == th.prefix && eq_rank++ < (unsigned long long)th.eq_need);
-    };
-    unsigned long long counts = 0;                     // low half: rows to fill, high half: rows to move
-    for (int i = i0; i < i1; ++i) {
-        const bool k = kept(i);
-        if (first + i < e.n_keep) counts += !k;
-        else if (k) counts += 1ull << 32;
-    }
-    unsigned long long at = block_scan(counts, sel.warp, total);
-    const unsigned long long before = cluster_before<CLN>(sel, 1, total);
-    at += before;
-    if (rank == CLN - 1 && tid == 0) e.n_moves[kv] = (int)((before + total) & 0xFFFFFFFFu);
-    eq_rank = eq_rank0;
+    // rows to fill (below n_keep, not kept) come before rows to move (at or above n_keep, kept), as many of each
     int32_t* to = CLN == 1 && fused ? s_to : e.to + (int64_t)kv * e.max_rows;
     int32_t* from = CLN == 1 && fused ? s_from : e.from + (int64_t)kv * e.max_rows;
-    int n_to = (int)(at & 0xFFFFFFFFu), n_from = (int)(at >> 32);
-    const bool stay = e.acc_out != e.acc || e.pos_out != e.pos;
-    for (int i = i0; i < i1; ++i) {
-        const bool k = kept(i);
-        const int row = first + i;
-        if (row < e.n_keep) {
-            if (!k) {
-                to[n_to++] = row;
-            } else if (stay) {
-                e.acc_out[(int64_t)kv * e.max_rows + row] = acc[row];
-                e.pos_out[(int64_t)kv * e.max_rows + row] = pos[row];
-            }
-        } else if (k) {
-            from[n_from++] = row;
-        }
-    }
+    int moves = 0;
+    ranked<CLN>(
+        sel, [&](int i) { return (first + i < e.n_keep) != th.in(key(i), i); }, n,
+        [&](unsigned all) {
+            moves = (int)(all / 2);
+            if (rank == 0 && tid == 0) e.n_moves[kv] = moves;
+        },
+        [&](int i, unsigned r) {
+            if (first + i < e.n_keep) to[r] = first + i;
+            else from[r - moves] = first + i;
+        });
     if constexpr (CLN == 1) {
         if (fused) {
-            const int moves = (int)(total & 0xFFFFFFFFu);
             __syncthreads();
-            for (int i = (tid >> 5) * 4; i < moves; i += SEL_WARPS * 4) move_rows<4>(e, kv, s_to, s_from, i, moves);
+            for (int i = (tid >> 5) * 8; i < moves; i += SEL_WARPS * 8) move_rows<8>(e, kv, s_to, s_from, i, moves);
         }
     } else {
         cg::this_cluster().sync();                     // no CTA leaves while its counts may be read
@@ -425,7 +565,7 @@ __global__ void __launch_bounds__(SC_THREADS) k_block_score(const CacheSelect c,
 // ---- selection: one CTA or cluster per (KV head, token) -------------------------------------------------------
 // Key of a score max_h (u_h - top_h) <= 0: the bits of its magnitude, turned over; NaN lowest.
 constexpr int BS_MAX_G = 64;
-constexpr int BS_SINGLE = 2048;          // candidates up to which one CTA chooses alone
+constexpr int BS_SINGLE = 8192;          // candidates up to which one CTA chooses alone
 __device__ __forceinline__ unsigned long long score_key(double v) {
     return v != v ? 0ull : 0x7FFFFFFFFFFFFFFFull - (unsigned long long)__double_as_longlong(fabs(v));
 }
@@ -496,27 +636,13 @@ __global__ void __launch_bounds__(SEL_THREADS) k_block_choose(const CacheSelect 
     __syncthreads();
     auto key = [&](int i) { return s_keys[i]; };
     const Threshold th = select_threshold<CLN, 63>(ss, key, n, n_take);
-    const int len = (n + SEL_THREADS - 1) / SEL_THREADS | 1, a0 = min(n, tid * len), a1 = min(n, a0 + len);
-    unsigned long long eq = 0, count = 0, total;
-    for (int i = a0; i < a1; ++i) eq += (s_keys[i] >> th.shift) == th.prefix;
-    unsigned long long eq_rank = block_scan(eq, ss.warp, total);
-    eq_rank += cluster_before<CLN>(ss, 0, total);
-    const unsigned long long eq_rank0 = eq_rank;
-    auto kept = [&](int i) {
-        const unsigned long long k = s_keys[i] >> th.shift;
-        return k > th.prefix || (k == th.prefix && eq_rank++ < (unsigned long long)th.eq_need);
-    };
-    for (int i = a0; i < a1; ++i) count += kept(i);
-    unsigned long long at = block_scan(count, ss.warp, total);
-    at += cluster_before<CLN>(ss, 1, total);
-    eq_rank = eq_rank0;
-    for (int i = a0; i < a1; ++i)
-        if (kept(i)) {
+    ranked<CLN>(
+        ss, [&](int i) { return th.in(s_keys[i], i); }, n, [](unsigned) {},
+        [&](int i, unsigned r) {
             const int b = cd.first + i0 + i;
-            list[cd.first + at] = b;
-            if (sel) sel[at] = b;
-            ++at;
-        }
+            list[cd.first + r] = b;
+            if (sel) sel[r] = b;
+        });
     if constexpr (CLN > 1) cg::this_cluster().sync();  // no CTA leaves while its counts may be read
 }
 
@@ -566,7 +692,10 @@ cudaError_t launch_cache_evict(const CacheEvict& e, cudaStream_t s) {
     const int most = e.n_keep < e.n_rows - e.n_keep ? e.n_keep : e.n_rows - e.n_keep;      // moves
     if (e.n_rows <= EV_SINGLE) {
         const bool fused = most <= EV_FUSED;
-        const cudaError_t rc = launch_pdl(k_evict_choose<1>, dim3(1, e.n_kv), SEL_THREADS, (size_t)e.n_rows * 4, s, e, fused);
+        static SmemLimit limit;
+        cudaError_t rc = limit.raise((const void*)k_evict_choose<1>, EV_SINGLE * 4);
+        if (rc != cudaSuccess) return rc;
+        rc = launch_pdl(k_evict_choose<1>, dim3(1, e.n_kv), SEL_THREADS, (size_t)e.n_rows * 4, s, e, fused);
         if (rc != cudaSuccess || fused) return rc;
     } else {
         static SmemLimit limit;
@@ -608,8 +737,12 @@ cudaError_t launch_cache_select(const CacheSelect& c, cudaStream_t s) {
         e = launch_pdl(fn, grid, SC_THREADS, score_smem(c.hd), s, c, nb_cap);
         if (e != cudaSuccess) return e;
     }
-    if (n_cand <= BS_SINGLE)
+    if (n_cand <= BS_SINGLE) {
+        static SmemLimit limit;
+        e = limit.raise((const void*)k_block_choose<1>, BS_SINGLE * 8);
+        if (e != cudaSuccess) return e;
         return launch_pdl(k_block_choose<1>, dim3(1, c.n_kv, c.m), SEL_THREADS, (size_t)n_cand * 8, s, c, nb_cap);
+    }
     static SmemLimit limit;
     e = limit.raise((const void*)k_block_choose<CL>, 128 * 1024);
     if (e != cudaSuccess) return e;
