@@ -476,10 +476,14 @@ __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __r
 
 // ---- scores: u[kv][row][b - first] = sum_d max(q_d kmin_d, q_d kmax_d) = sum_d q_d (q_d > 0 ? kmax_d : kmin_d) ----
 // In 64 bits, because the scores decide which rows are read: products of 24 and 11 (or 8) bits are exact, and
-// sums differ from the true ones in the 16th digit. A CTA takes 32 blocks (one per lane) and eight query rows;
-// its warps share out the dims, eight at a time, and their sums are added in warp order. A value is converted once
-// for the eight rows, since conversions to f64 run at a quarter of the rate of its multiply-adds. u_top receives
-// the rows' maxima over the CTA's blocks.
+// sums differ from the true ones in the 16th digit. A CTA takes NB x 32 blocks (NB per lane) and eight query rows; its
+// warps share out the dims, eight at a time, and their sums are added in warp order. u_top receives the rows' maxima
+// over the CTA's blocks.
+// Bound by instruction issue, so nothing but the multiply-add is done per product except a select: a bound's f64 is
+// made from its bits by shifting them under the exponent field (two or three integer instructions, where the
+// conversion instruction runs at a quarter of the multiply-add's rate), which is its value times 2^-1008 (f16) or
+// 2^-896 (bf16), subnormals included; q is scaled up to make up for all but 2^-128 of it, which cancels in nothing but
+// the comparison of scores. Infinite bounds thereby count as one step above the largest finite value.
 struct Candidates {
     int n_past, nb, first, last;
 };
@@ -488,29 +492,39 @@ __device__ __forceinline__ Candidates candidates(const CacheSelect& c) {
     const int nb = (past + c.block - 1) / c.block, first = min(c.n_sink, nb);
     return {past, nb, first, max(first, nb - min(nb, c.n_local))};
 }
-template <typename KT> __device__ __forceinline__ double2 to_double2(uint32_t w);
-template <> __device__ __forceinline__ double2 to_double2<__half>(uint32_t w) {
-    return make_double2((double)h2f(w), (double)h2f(w >> 16));
-}
-template <> __device__ __forceinline__ double2 to_double2<__nv_bfloat16>(uint32_t w) {
-    return make_double2((double)__uint_as_float(w << 16), (double)__uint_as_float(w & 0xFFFF0000u));
+template <typename KT> struct Shift;     // of a packed value's bits under f64's exponent field; the scale of q
+template <> struct Shift<__half> {
+    static constexpr int N = 6;
+    static constexpr int MASK = (int)0x81FFFC00u, Q_EXP = 1008 - 128;
+};
+template <> struct Shift<__nv_bfloat16> {
+    static constexpr int N = 3;
+    static constexpr int MASK = (int)0x8FFFE000u, Q_EXP = 896 - 128;
+};
+// high words of the f64s of a packed pair
+template <typename KT> __device__ __forceinline__ int2 high_words(uint32_t w) {
+    return make_int2(((int)(w << 16) >> Shift<KT>::N) & Shift<KT>::MASK, ((int)w >> Shift<KT>::N) & Shift<KT>::MASK);
 }
 
-constexpr int SC_THREADS = 256, SC_ROWS = 8, SC_BLOCKS = 32;
-constexpr int score_smem(int hd) { return SC_ROWS * hd * 8 + 8 * SC_ROWS * 32 * 8 + SC_BLOCKS * (hd + 4) * 4; }
-template <typename KT>
+constexpr int SC_THREADS = 256, SC_ROWS = 8;
+constexpr int SC_TOP = 32;               // blocks of an entry of u_top
+constexpr int score_smem(int hd, int nb) {
+    return SC_ROWS * hd * 8 + SC_ROWS * hd * 4 + 8 * SC_ROWS * 32 * 8 + nb * 32 * (hd + 4) * 4;
+}
+template <typename KT, int NB>
 __global__ void __launch_bounds__(SC_THREADS) k_block_score(const CacheSelect c, int nb_cap) {
     pdl_enter();
     extern __shared__ __align__(16) uint8_t s_raw[];
     const Candidates cd = candidates(c);
-    const int n_cand = cd.last - cd.first, b0 = blockIdx.x * SC_BLOCKS, kv = blockIdx.y, row0 = blockIdx.z * SC_ROWS;
+    const int n_cand = cd.last - cd.first, b0 = blockIdx.x * 32 * NB, kv = blockIdx.y, row0 = blockIdx.z * SC_ROWS;
     if (n_cand <= c.n_sel || b0 >= n_cand) return;     // every candidate is taken: no scores needed
     const int R = c.m * c.g, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     double* sq = reinterpret_cast<double*>(s_raw);                              // [SC_ROWS][hd]
     double* red = sq + SC_ROWS * c.hd;                                          // [8 warps][SC_ROWS][32]
-    // [32][hd + 4] words: 16-byte reads of eight lanes fall in eight bank groups
-    uint32_t* sb = reinterpret_cast<uint32_t*>(red + 8 * SC_ROWS * 32);
-    const int n = min(SC_BLOCKS, n_cand - b0), c4 = c.hd / 4, c8 = c.hd / 8;
+    int* sm = reinterpret_cast<int*>(red + 8 * SC_ROWS * 32);                   // [SC_ROWS][hd]: -1 where q > 0
+    // [32 NB][hd + 4] words: 16-byte reads of eight lanes fall in eight bank groups
+    uint32_t* sb = reinterpret_cast<uint32_t*>(sm + SC_ROWS * c.hd);
+    const int n = min(32 * NB, n_cand - b0), c4 = c.hd / 4, c8 = c.hd / 8;
     const uint32_t* src = reinterpret_cast<const uint32_t*>(c.bounds) +
                           ((int64_t)kv * (c.max_rows / c.block) + cd.first + b0) * c.hd;      // hd words a block
     for (int b = warp; b < n; b += 8)
@@ -519,47 +533,75 @@ __global__ void __launch_bounds__(SC_THREADS) k_block_score(const CacheSelect c,
     {
         const int row = row0 + warp;                   // a warp converts a query row
         const float* q = c.q + (row / c.g) * c.q_ts + (kv * c.g + row % c.g) * c.q_hs;
+        const double up = __hiloint2double((1023 + Shift<KT>::Q_EXP) << 20, 0);
         float x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = row < R && k * 32 + lane < c.hd ? q[k * 32 + lane] : 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            if (k * 32 + lane < c.hd) sq[warp * c.hd + k * 32 + lane] = (double)x[k];
+            if (k * 32 + lane < c.hd) {
+                sq[warp * c.hd + k * 32 + lane] = (double)x[k] * up;
+                sm[warp * c.hd + k * 32 + lane] = x[k] > 0.f ? -1 : 0;
+            }
     }
     cp_async_wait_all();
     __syncthreads();
-    double acc[SC_ROWS];
+    double acc[NB][SC_ROWS];
 #pragma unroll
-    for (int r = 0; r < SC_ROWS; ++r) acc[r] = 0.0;
-    const uint32_t* mine = sb + min(lane, n - 1) * (c.hd + 4);
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int r = 0; r < SC_ROWS; ++r) acc[i][r] = 0.0;
+    const uint32_t* mine[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) mine[i] = sb + min(32 * i + lane, n - 1) * (c.hd + 4);
     for (int p = warp; p < c8; p += 8) {
-        const uint4 l4 = *reinterpret_cast<const uint4*>(mine + 4 * p);
-        const uint4 h4 = *reinterpret_cast<const uint4*>(mine + c.hd / 2 + 4 * p);
-        const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
+        uint32_t lw[NB][4], hw[NB][4];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const uint4 l4 = *reinterpret_cast<const uint4*>(mine[i] + 4 * p);
+            const uint4 h4 = *reinterpret_cast<const uint4*>(mine[i] + c.hd / 2 + 4 * p);
+            lw[i][0] = l4.x, lw[i][1] = l4.y, lw[i][2] = l4.z, lw[i][3] = l4.w;
+            hw[i][0] = h4.x, hw[i][1] = h4.y, hw[i][2] = h4.z, hw[i][3] = h4.w;
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const double2 lo = to_double2<KT>(lw[k]), hi = to_double2<KT>(hw[k]);
+            int2 lo[NB], hi[NB];
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                lo[i] = high_words<KT>(lw[i][k]);
+                hi[i] = high_words<KT>(hw[i][k]);
+            }
 #pragma unroll
             for (int r = 0; r < SC_ROWS; ++r) {
                 const double2 q = *reinterpret_cast<const double2*>(sq + r * c.hd + 8 * p + 2 * k);
-                acc[r] = fma(q.x, q.x > 0.0 ? hi.x : lo.x, acc[r]);
-                acc[r] = fma(q.y, q.y > 0.0 ? hi.y : lo.y, acc[r]);
+                const int2 up = *reinterpret_cast<const int2*>(sm + r * c.hd + 8 * p + 2 * k);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    acc[i][r] = fma(q.x, __hiloint2double((hi[i].x & up.x) | (lo[i].x & ~up.x), 0), acc[i][r]);
+                    acc[i][r] = fma(q.y, __hiloint2double((hi[i].y & up.y) | (lo[i].y & ~up.y), 0), acc[i][r]);
+                }
             }
         }
     }
-#pragma unroll
-    for (int r = 0; r < SC_ROWS; ++r) red[(warp * SC_ROWS + r) * 32 + lane] = acc[r];
-    __syncthreads();
-    double s = 0.0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) s += red[(w * SC_ROWS + warp) * 32 + lane];     // thread = (row, block)
     const int row = row0 + warp;
-    if (row >= R) return;
-    if (lane < n) c.u[((int64_t)kv * R + row) * nb_cap + b0 + lane] = s;
-    double top = lane < n ? s : -INFINITY;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) c.u_top[((int64_t)kv * R + row) * ((nb_cap + SC_BLOCKS - 1) / SC_BLOCKS) + blockIdx.x] = top;
+    for (int i = 0; i < NB; ++i) {
+        if (i) __syncthreads();
+#pragma unroll
+        for (int r = 0; r < SC_ROWS; ++r) red[(warp * SC_ROWS + r) * 32 + lane] = acc[i][r];
+        __syncthreads();
+        double s = 0.0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += red[(w * SC_ROWS + warp) * 32 + lane];     // thread = (row, block)
+        const int left = n - 32 * i;
+        if (row < R && left > 0) {
+            if (lane < left) c.u[((int64_t)kv * R + row) * nb_cap + b0 + 32 * i + lane] = s;
+            double top = lane < left ? s : -INFINITY;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (lane == 0) c.u_top[((int64_t)kv * R + row) * ((nb_cap + SC_TOP - 1) / SC_TOP) + blockIdx.x * NB + i] = top;
+        }
+    }
 }
 
 // ---- selection: one CTA or cluster per (KV head, token) -------------------------------------------------------
@@ -599,7 +641,7 @@ __global__ void __launch_bounds__(SEL_THREADS) k_block_choose(const CacheSelect 
     if (n_take == 0) return;
     const int i0 = (int)((int64_t)n_cand * rank / CLN), i1 = (int)((int64_t)n_cand * (rank + 1) / CLN), n = i1 - i0;
     const int64_t row0 = ((int64_t)kv * c.m + t) * c.g;
-    const int tops = (n_cand + SC_BLOCKS - 1) / SC_BLOCKS, top_cap = (nb_cap + SC_BLOCKS - 1) / SC_BLOCKS;
+    const int tops = (n_cand + SC_TOP - 1) / SC_TOP, top_cap = (nb_cap + SC_TOP - 1) / SC_TOP;
     for (int h = warp; h < c.g; h += SEL_WARPS) {
         const double* p = c.u_top + (row0 + h) * top_cap;
         double mx = -INFINITY;
@@ -614,24 +656,29 @@ __global__ void __launch_bounds__(SEL_THREADS) k_block_choose(const CacheSelect 
         for (int o = 16; o > 0; o >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         if (lane == 0) s_top[h] = mx;
     }
-    // this thread's blocks' u are on their way while the maxima are waited for
-    const double* u = c.u + row0 * nb_cap + i0;
-    double v[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = tid < n && k < c.g ? u[k * (int64_t)nb_cap + tid] : 0.0;
     __syncthreads();
-    for (int i = tid; i < n; i += SEL_THREADS) {
-        double best = -INFINITY;
+    // four blocks by eight heads of loads in flight per thread
+    const double* u = c.u + row0 * nb_cap + i0;
+    for (int i = tid; i < n; i += 4 * SEL_THREADS) {
+        double best[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) best[k] = -INFINITY;
         for (int h0 = 0; h0 < c.g; h0 += 8) {
-            if (i != tid || h0) {
+            double v[4][8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = h0 + k < c.g ? u[(h0 + k) * (int64_t)nb_cap + i] : 0.0;
-            }
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (h0 + k < c.g) best = fmax(best, v[k] - s_top[h0 + k]);
+                for (int h = 0; h < 8; ++h)
+                    v[k][h] = i + k * SEL_THREADS < n && h0 + h < c.g ? u[(h0 + h) * (int64_t)nb_cap + i + k * SEL_THREADS] : 0.0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int h = 0; h < 8; ++h)
+                    if (h0 + h < c.g) best[k] = fmax(best[k], v[k][h] - s_top[h0 + h]);
         }
-        s_keys[i] = score_key(best);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k * SEL_THREADS < n) s_keys[i + k * SEL_THREADS] = score_key(best[k]);
     }
     __syncthreads();
     auto key = [&](int i) { return s_keys[i]; };
@@ -729,12 +776,16 @@ cudaError_t launch_cache_select(const CacheSelect& c, cudaStream_t s) {
     if (n_cand < 0) n_cand = 0;
     cudaError_t e;
     if (n_cand > c.n_sel && c.n_sel > 0) {
-        const dim3 grid((n_cand + SC_BLOCKS - 1) / SC_BLOCKS, c.n_kv, (c.m * c.g + SC_ROWS - 1) / SC_ROWS);
-        auto fn = c.bf16 ? k_block_score<__nv_bfloat16> : k_block_score<__half>;
-        static SmemLimit limit[2];
-        e = limit[c.bf16].raise((const void*)fn, score_smem(256));
+        // one block per lane where that fits the GPU at once (two CTAs per SM), else two: half the reads of q per product
+        const int row_groups = (c.m * c.g + SC_ROWS - 1) / SC_ROWS, chunks = (n_cand + 31) / 32;
+        const int nb = chunks * c.n_kv * row_groups <= 2 * KV_SMS ? 1 : 2;
+        const dim3 grid((chunks + nb - 1) / nb, c.n_kv, row_groups);
+        auto fn = c.bf16 ? (nb == 1 ? k_block_score<__nv_bfloat16, 1> : k_block_score<__nv_bfloat16, 2>)
+                         : (nb == 1 ? k_block_score<__half, 1> : k_block_score<__half, 2>);
+        static SmemLimit limit[4];
+        e = limit[2 * c.bf16 + nb - 1].raise((const void*)fn, score_smem(256, nb));
         if (e != cudaSuccess) return e;
-        e = launch_pdl(fn, grid, SC_THREADS, score_smem(c.hd), s, c, nb_cap);
+        e = launch_pdl(fn, grid, SC_THREADS, score_smem(c.hd, nb), s, c, nb_cap);
         if (e != cudaSuccess) return e;
     }
     if (n_cand <= BS_SINGLE) {

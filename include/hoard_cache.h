@@ -85,7 +85,8 @@ int hoard_kv_block_bounds(const hoard_kv_desc* d, const void* k_cache, void* bou
  * attends the blocks below n_sink, the last n_local (>= 1), and of the others the n_sel whose score is
  * largest (the lower block where equal), beside the token's visible own rows. The score of block b is
  * max over the KV head's query heads of U_h(b) - max_b' U_h(b'), U_h(b) = sum_d max(q_d kmin_d, q_d kmax_d), an
- * upper bound of q . k over the block's keys; formed and compared in 64 bits, NaN ranking lowest.
+ * upper bound of q . k over the block's keys; formed and compared in 64 bits, the NaN of a NaN in q ranking
+ * lowest and infinite keys counting as one step above the largest finite value.
  * bounds have to be those of the complete blocks of [0, n_past). sel_out (optional, [m][n_head_kv][n_sel]):
  * the chosen blocks in ascending order, then -1. */
 int hoard_kv_block_attention(const hoard_kv_desc* d, const hoard_kv_query* a, const void* bounds, int n_sink,
