@@ -90,15 +90,15 @@ __global__ void __launch_bounds__(W * 32, 1) k_cache_attention(const CacheAttn a
     uint32_t* qf = reinterpret_cast<uint32_t*>(smem + Plan<HD>::RING);
 
     // chunks of this CTA: past rows (or the listed blocks' rows), then the tokens' own rows
-    const int sub = BLOCKS ? a.block / KV_CHUNK : 1;
-    const int n_pc = BLOCKS ? a.list_n[prob] * sub : (n_past + KV_CHUNK - 1) / KV_CHUNK;
+    const int sub_shift = BLOCKS ? __ffs(a.block / KV_CHUNK) - 1 : 0;         // chunks of a block: a power of two
+    const int n_pc = BLOCKS ? a.list_n[prob] << sub_shift : (n_past + KV_CHUNK - 1) / KV_CHUNK;
     const int n_chunks = n_pc + (a.m + KV_CHUNK - 1) / KV_CHUNK;
     const int c_end = (int)((int64_t)n_chunks * (split + 1) / gridDim.x);
     const int c_first = (int)((int64_t)n_chunks * split / gridDim.x) + warp;
     const int32_t* list = BLOCKS ? a.list + (int64_t)prob * a.list_cap : nullptr;
     auto chunk_row = [&](int c) {                      // first cache row of chunk c
         if (c >= n_pc) return n_past + (c - n_pc) * KV_CHUNK;
-        if (BLOCKS) return list[c / sub] * a.block + (c % sub) * KV_CHUNK;
+        if (BLOCKS) return list[c >> sub_shift] * a.block + (c & ((1 << sub_shift) - 1)) * KV_CHUNK;
         return c * KV_CHUNK;
     };
     auto chunk_end = [&](int c) { return c >= n_pc ? n_past + a.m : n_past; };

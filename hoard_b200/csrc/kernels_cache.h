@@ -86,6 +86,7 @@ struct CacheSelect {
     const void* bounds;
     bool bf16;
     int n_head, n_kv, g, hd, m, n_past, max_rows, block, n_sink, n_local, n_sel;
+    int block_shift;                     // log2(block), set by the launcher
     const int32_t* n_past_dev;
     double* u;                           // [n_kv][m * g][max_rows / block]
     double* u_top;                       // [n_kv][m * g][ceil of that / 32]

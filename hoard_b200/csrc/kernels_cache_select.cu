@@ -489,7 +489,7 @@ struct Candidates {
 };
 __device__ __forceinline__ Candidates candidates(const CacheSelect& c) {
     const int past = c.n_past_dev ? max(0, min(*c.n_past_dev, c.max_rows - c.m)) : c.n_past;
-    const int nb = (past + c.block - 1) / c.block, first = min(c.n_sink, nb);
+    const int nb = (past + c.block - 1) >> c.block_shift, first = min(c.n_sink, nb);
     return {past, nb, first, max(first, nb - min(nb, c.n_local))};
 }
 template <typename KT> struct Shift;     // of a packed value's bits under f64's exponent field; the scale of q
@@ -526,13 +526,14 @@ __global__ void __launch_bounds__(SC_THREADS) k_block_score(const CacheSelect c,
     uint32_t* sb = reinterpret_cast<uint32_t*>(sm + SC_ROWS * c.hd);
     const int n = min(32 * NB, n_cand - b0), c4 = c.hd / 4, c8 = c.hd / 8;
     const uint32_t* src = reinterpret_cast<const uint32_t*>(c.bounds) +
-                          ((int64_t)kv * (c.max_rows / c.block) + cd.first + b0) * c.hd;      // hd words a block
+                          ((int64_t)kv * nb_cap + cd.first + b0) * c.hd;      // hd words a block
     for (int b = warp; b < n; b += 8)
         for (int p = lane; p < c4; p += 32) cp_async16(sb + b * (c.hd + 4) + 4 * p, src + b * c.hd + 4 * p);
     cp_async_commit();
     {
         const int row = row0 + warp;                   // a warp converts a query row
-        const float* q = c.q + (row / c.g) * c.q_ts + (kv * c.g + row % c.g) * c.q_hs;
+        const int t = row / c.g;
+        const float* q = c.q + t * c.q_ts + (kv * c.g + row - t * c.g) * c.q_hs;
         const double up = __hiloint2double((1023 + Shift<KT>::Q_EXP) << 20, 0);
         float x[8];
 #pragma unroll
@@ -769,7 +770,9 @@ cudaError_t launch_cache_bounds(const void* kc, int64_t rs, int64_t hs, bool bf1
                       row0, row1, row1_dev, (uint16_t*)bounds);
 }
 
-cudaError_t launch_cache_select(const CacheSelect& c, cudaStream_t s) {
+cudaError_t launch_cache_select(const CacheSelect& asked, cudaStream_t s) {
+    CacheSelect c = asked;
+    c.block_shift = __builtin_ctz(c.block);
     const int nb_cap = c.max_rows / c.block;
     const int past_most = c.n_past_dev ? c.max_rows - c.m : c.n_past;
     int n_cand = (past_most + c.block - 1) / c.block - c.n_sink - c.n_local;

@@ -16,7 +16,13 @@ Prompt tokens run through the same step one at a time, as in hoard; generation s
 logits of the last prompt token. Models come from a GGUF file (`DecodeModel.from_gguf`) or from
 seeded tensors generated on the device (`seeded_tensors`, the benchmark configurations' weights:
 N(0, 0.02), Q4_K_M types). The MoE layers use all experts HBM-resident (T = 1: the persistent
-decode kernel)."""
+decode kernel).
+
+Beside the plain step there are three forms of the attention over the cache (hoard_b200/cache.py):
+`tree_generate` verifies a tree of drafted tokens in one forward (`forward_tree`); `blocks=BlockChoice(..)` lets every
+token attend the first, the last and the best-scoring blocks of a long cache; `budget=CacheBudget(..)` keeps a bounded
+number of cache rows per KV head, evicting the positions with the least accumulated attention weight. Contexts too long
+for the one-CTA-per-head attention's shared memory run through the split attention of the same module."""
 from __future__ import annotations
 
 import ctypes
@@ -26,13 +32,38 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from hoard_b200 import moe, quant
+from hoard_b200 import cache, moe, quant
 from hoard_b200.moe import HoardError, _ptr, _stream, lib
 
 Q4_K, Q6_K, F32 = quant.Q4_K, quant.Q6_K, 0
 KV_TYPES = {torch.float16: 1, torch.bfloat16: 30}     # KV cache element -> HOARD_TYPE_F16 / HOARD_TYPE_BF16
 MAX_BATCH = 16          # tokens of one batched (verify) forward
 QK_MODE = {"": 0, "full": 1, "head": 2}
+LONG_CTX = 46000        # cached positions beyond which hoard_hx_attention's scores do not fit in shared memory
+
+
+@dataclass
+class BlockChoice:
+    """Attention over blocks of `block` cache rows: the first n_sink, the last n_local and the n_sel best-scoring others
+    for each token and KV head."""
+    block: int = 64
+    n_sink: int = 1
+    n_local: int = 4
+    n_sel: int = 32
+
+
+@dataclass
+class CacheBudget:
+    """A bounded cache: when n_keep + n_slack rows are filled, each KV head keeps n_keep of them -- the first n_sink and
+    the last n_recent positions, then those with the largest accumulated attention weight."""
+    n_keep: int
+    n_slack: int = 256
+    n_sink: int = 4
+    n_recent: int = 128
+
+    @property
+    def rows(self) -> int:
+        return self.n_keep + self.n_slack
 
 
 def _iarr(vals):
@@ -226,11 +257,21 @@ def config_from_hparams(hp) -> ModelConfig:
 
 class DecodeModel:
     def __init__(self, cfg: ModelConfig, tensors: dict, device: int = 0, max_ctx: int = 512, eos_id: int = -1,
-                 kv_dtype=torch.float16):
+                 kv_dtype=torch.float16, max_batch: int = MAX_BATCH, blocks: BlockChoice | None = None,
+                 budget: CacheBudget | None = None):
         """tensors: name -> (ggml type, ne, array or tensor of raw bytes / f32 values), host or device.
-        kv_dtype: torch.float16 or torch.bfloat16 elements of the KV cache."""
+        kv_dtype: torch.float16 or torch.bfloat16 elements of the KV cache. max_batch: most tokens of a batched
+        forward (verify pass), up to 64. blocks / budget: the block-sparse or the bounded form of the cache."""
         if kv_dtype not in (torch.float16, torch.bfloat16):
             raise ValueError("kv_dtype must be torch.float16 or torch.bfloat16")
+        if not 1 <= max_batch <= cache.MAX_TOKENS:
+            raise ValueError(f"max_batch must be 1..{cache.MAX_TOKENS}")
+        if blocks is not None and budget is not None:
+            raise ValueError("blocks of the cache need its rows in the order of positions: not with a budget")
+        if budget is not None and not (0 <= budget.n_sink and 0 <= budget.n_recent and budget.n_slack >= 1
+                                       and budget.n_sink + budget.n_recent < budget.n_keep):
+            raise ValueError("a budget keeps more rows than its first and last positions, and has slack")
+        self.max_batch, self.blocks, self.budget = max_batch, blocks, budget
         self.cfg, self.device, self.max_ctx, self.eos_id = cfg, device, max_ctx, eos_id
         self.kv_type = KV_TYPES[kv_dtype]
         dev = self.dev = torch.device("cuda", device)
@@ -290,7 +331,7 @@ class DecodeModel:
                                   n_layer=cfg.n_layer, norm_topk=cfg.norm_topk, eps=cfg.eps,
                                   gate_types=[t[0] for t in types], up_types=[t[1] for t in types],
                                   down_types=[t[2] for t in types], n_ff_shexp=cfg.n_ff_shexp, shexp_types=sh_types,
-                                  max_tokens=MAX_BATCH, device=device)
+                                  max_tokens=max_batch, device=device)
         for il in range(cfg.n_layer):
             b = f"blk.{il}."
             self.moe.set_router(il, f32(b + "ffn_gate_inp.weight").view(cfg.n_expert, H), f32(b + cfg.ffn_norm_name()))
@@ -315,8 +356,22 @@ class DecodeModel:
         for il, L in enumerate(self.layers):
             if not L["recurrent"]:
                 self.kv_index[il] = len(self.kv_index)
-        self.kc = torch.zeros(max(1, n_full), max_ctx, self.nkv, dtype=kv_dtype, device=dev)
+        self.n_cache = budget.rows if budget else max_ctx         # rows of a layer's cache
+        self.kc = torch.zeros(max(1, n_full), self.n_cache, self.nkv, dtype=kv_dtype, device=dev)
         self.vc = torch.zeros_like(self.kc)
+        # the split attention: long contexts, blocks, budgets, and (made when first used) trees
+        self._ops_args = dict(n_head=cfg.n_head, n_head_kv=cfg.n_head_kv, head_dim=hd, kv_dtype=kv_dtype,
+                              max_rows=self.n_cache, block=blocks.block if blocks else 0, device=device)
+        self.ops = cache.CacheOps(**self._ops_args) if blocks or budget or max_ctx > LONG_CTX else None
+        self._tree_ops = None
+        if blocks:
+            self.bounds = torch.zeros(max(1, n_full), cfg.n_head_kv, self.n_cache // blocks.block, 2, hd, dtype=kv_dtype,
+                                      device=dev)
+        if budget:
+            self.kv_acc = torch.zeros(max(1, n_full), cfg.n_head_kv, self.n_cache, dtype=torch.float32, device=dev)
+            self.kv_pos = torch.zeros(max(1, n_full), cfg.n_head_kv, self.n_cache, dtype=torch.int32, device=dev)
+            self.rows_dev = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.n_rows = 0         # filled rows of a bounded cache
         if hybrid:
             n_rec = cfg.n_layer - n_full
             self.gdn_qkv, self.gdn_z, self.gdn_ba = z(cfg.conv_dim), z(self.gdn_vd), z(2 * cfg.ssm_dt_rank)
@@ -329,12 +384,13 @@ class DecodeModel:
             self.rec_index = {il: i for i, il in enumerate(j for j, L in enumerate(self.layers) if L["recurrent"])}
         self.seq = torch.zeros(max_ctx + 1, dtype=torch.int32, device=dev)
         self.scratch_tok = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.all_pos = torch.arange(max_ctx, dtype=torch.int32, device=dev)
         self.pos_dev = torch.zeros(1, dtype=torch.int32, device=dev)
         self._graph = None
         torch.cuda.synchronize(dev)
 
     @classmethod
-    def from_gguf(cls, path: str, device: int = 0, max_ctx: int = 512, kv_dtype=torch.float16):
+    def from_gguf(cls, path: str, device: int = 0, max_ctx: int = 512, kv_dtype=torch.float16, **kw):
         from hoard_b200 import gguf_io as gi
         g = gi.GGUFFile(path)
         hp = gi.read_hparams(g)
@@ -344,7 +400,7 @@ class DecodeModel:
             tensors[name] = (t.type, t.ne, np.array(data))
         g.close()
         return cls(config_from_hparams(hp), tensors, device=device, max_ctx=max_ctx, eos_id=hp.eos_id,
-                   kv_dtype=kv_dtype)
+                   kv_dtype=kv_dtype, **kw)
 
     def close(self):
         self.moe.close()
@@ -354,6 +410,8 @@ class DecodeModel:
         c, hx, s = self.cfg, _hx(), _stream(stream)
         H = c.n_embd
         x, x2 = self.x, self.x2
+        if self.budget:
+            self._make_room(pos, stream)
         _ok(hx.hoard_hx_embed(self.embd_type, _ptr(self.embd), H, c.n_vocab, _ptr(self.seq[pos:pos + 1]), _ptr(x), s),
             "embed")
         for il, L in enumerate(self.layers):
@@ -364,6 +422,22 @@ class DecodeModel:
         _ok(hx.hoard_hx_gemv(self.out_type, _ptr(self.out_w), c.n_vocab, H, _ptr(self.q8), None, _ptr(self.logits), s),
             "gemv")
         _ok(hx.hoard_hx_argmax(_ptr(self.logits), c.n_vocab, _ptr(next_tok), s), "argmax")
+        self.n_rows += 1
+
+    # ---- bounded cache ----
+    def _make_room(self, pos: int, stream=None):
+        """Before the token at position pos is stored: a full cache is brought down to its budget."""
+        b = self.budget
+        if self.n_rows < b.rows:
+            return
+        for i in range(len(self.kv_index)):
+            self.ops.evict(self._heads(self.kc[i]), self._heads(self.vc[i]), self.kv_acc[i], self.kv_pos[i], self.n_rows,
+                           b.n_keep, n_sink=b.n_sink, recent_from=pos - b.n_recent, stream=stream)
+        self.n_rows = b.n_keep
+
+    def _heads(self, t):
+        """A cache as [row][KV head][head_dim]."""
+        return t.view(self.n_cache, self.cfg.n_head_kv, self.cfg.head_dim)
 
     def _layer_attention(self, il, L, x, x2, hx, s, pos=None, bufs=None):
         """Graph A's attention part of layer il: x2 = Wo att + x (or the delta-net block's output
@@ -382,34 +456,79 @@ class DecodeModel:
         mode = QK_MODE[c.qk_norm]
         qn, kn = (L["q_norm"], L["k_norm"]) if mode else (None, None)
         scale = 1.0 / math.sqrt(hd)
+        qs = 2 * hd if c.attn_gate else hd           # a q head, with its gate
+        pd = None if pos is not None else self.pos_dev
+        if self.budget:
+            # the token's row is not its position
+            k3, v3 = self._heads(kc), self._heads(vc)
+            row_dev = None if pos is not None else self.rows_dev
+            i = self.kv_index[il]
+            rot = self.ops.store(self._q_view(q), k.view(1, c.n_head_kv, hd), v.view(1, c.n_head_kv, hd), k3, v3,
+                                 self.all_pos[pos:pos + 1] if pd is None else pd, self.n_rows, q_norm=qn, k_norm=kn, mode=mode,
+                                 eps=c.eps, rope_dim=c.n_rot, freq_base=c.freq_base, q_out=q_rot.view(1, c.n_head, hd),
+                                 row0_dev=row_dev, acc=self.kv_acc[i], row_pos=self.kv_pos[i], stream=s)
+            self.ops.tree_attention(rot, k3, v3, self.n_rows, gate=self._gate_view(q), acc=self.kv_acc[i],
+                                    out=att.view(1, c.n_head, hd), n_past_dev=row_dev, stream=s)
+        else:
+            self._store(q, k, v, q_rot, kc, vc, qn, kn, mode, hx, s, pos)
+            if self.ops:
+                args = dict(gate=self._gate_view(q), out=att.view(1, c.n_head, hd), n_past_dev=pd, stream=s)
+                rot, k3, v3, n = q_rot.view(1, c.n_head, hd), self._heads(kc), self._heads(vc), pos or 0
+                if self.blocks:
+                    bc, bounds = self.blocks, self.bounds[self.kv_index[il]]
+                    self.ops.block_attention(rot, k3, v3, bounds, n, n_sink=bc.n_sink, n_local=bc.n_local, n_sel=bc.n_sel,
+                                             **args)
+                    # the row just stored may complete a block
+                    if pos is None:
+                        self.ops.block_bounds(k3, bounds, row1_dev=pd, stream=s)
+                    elif (pos + 1) % bc.block == 0:
+                        self.ops.block_bounds(k3, bounds, pos, pos + 1, stream=s)
+                else:
+                    self.ops.tree_attention(rot, k3, v3, n, **args)
+            elif c.attn_gate or c.n_rot != hd:
+                n_pos = pos + 1 if pos is not None else self.max_ctx
+                gate = _ptr(q) + 4 * hd if c.attn_gate else None
+                _ok(hx.hoard_hx_attention_ex(_ptr(q_rot), _ptr(kc), _ptr(vc), c.n_head, c.n_head_kv, hd, n_pos, _ptr(pd),
+                                             scale, gate, qs, _ptr(att), self.kv_type, s), "attention")
+            elif pos is None:
+                _ok(hx.hoard_hx_attention_at(_ptr(q_rot), _ptr(kc), _ptr(vc), c.n_head, c.n_head_kv, hd,
+                                             _ptr(self.pos_dev), self.max_ctx, scale, _ptr(att), self.kv_type, s),
+                    "attention")
+            else:
+                _ok(hx.hoard_hx_attention(_ptr(q_rot), _ptr(kc), _ptr(vc), c.n_head, c.n_head_kv, hd, pos + 1, scale,
+                                          _ptr(att), self.kv_type, s), "attention")
+        _ok(hx.hoard_hx_quant_q8(_ptr(att), self.nq, _ptr(self.q8), s), "quant")
+        ty, wo = L["o"]
+        _ok(hx.hoard_hx_gemv(ty, _ptr(wo), H, self.nq, _ptr(self.q8), _ptr(x), _ptr(x2), s), "gemv")
+
+    def _store(self, q, k, v, q_rot, kc, vc, qn, kn, mode, hx, s, pos):
+        """QK norm, RoPE, and k, v to the cache row of the token's position."""
+        c, hd = self.cfg, self.cfg.head_dim
         if c.attn_gate or c.n_rot != hd:
             # fused q + gate rows ([q | gate] per head), partial rotary dims
             qs = 2 * hd if c.attn_gate else hd
             pd = None if pos is not None else _ptr(self.pos_dev)
-            p0 = pos if pos is not None else 0
             _ok(hx.hoard_hx_qknorm_rope_store_ex(_ptr(q), _ptr(k), _ptr(v), _ptr(qn), _ptr(kn), mode, c.eps, c.n_head,
-                                                 c.n_head_kv, hd, qs, c.n_rot, p0, pd, self.max_ctx, c.freq_base,
-                                                 _ptr(q_rot), _ptr(kc), _ptr(vc), self.kv_type, s), "qk rope")
-            n_pos = pos + 1 if pos is not None else self.max_ctx
-            gate = _ptr(q) + 4 * hd if c.attn_gate else None
-            _ok(hx.hoard_hx_attention_ex(_ptr(q_rot), _ptr(kc), _ptr(vc), c.n_head, c.n_head_kv, hd, n_pos, pd, scale,
-                                         gate, qs, _ptr(att), self.kv_type, s), "attention")
+                                                 c.n_head_kv, hd, qs, c.n_rot, pos if pos is not None else 0, pd,
+                                                 self.max_ctx, c.freq_base, _ptr(q_rot), _ptr(kc), _ptr(vc), self.kv_type,
+                                                 s), "qk rope")
         elif pos is None:
             _ok(hx.hoard_hx_qknorm_rope_store_at(_ptr(q), _ptr(k), _ptr(v), _ptr(qn), _ptr(kn), mode, c.eps, c.n_head,
                                                  c.n_head_kv, hd, _ptr(self.pos_dev), self.max_ctx, c.freq_base,
                                                  _ptr(q_rot), _ptr(kc), _ptr(vc), self.kv_type, s), "qk rope")
-            _ok(hx.hoard_hx_attention_at(_ptr(q_rot), _ptr(kc), _ptr(vc), c.n_head, c.n_head_kv, hd,
-                                         _ptr(self.pos_dev), self.max_ctx, scale, _ptr(att), self.kv_type, s),
-                "attention")
         else:
             _ok(hx.hoard_hx_qknorm_rope_store(_ptr(q), _ptr(k), _ptr(v), _ptr(qn), _ptr(kn), mode, c.eps, c.n_head,
                                               c.n_head_kv, hd, pos, c.freq_base, _ptr(q_rot), _ptr(kc), _ptr(vc),
                                               self.kv_type, s), "qk rope")
-            _ok(hx.hoard_hx_attention(_ptr(q_rot), _ptr(kc), _ptr(vc), c.n_head, c.n_head_kv, hd, pos + 1, scale,
-                                      _ptr(att), self.kv_type, s), "attention")
-        _ok(hx.hoard_hx_quant_q8(_ptr(att), self.nq, _ptr(self.q8), s), "quant")
-        ty, wo = L["o"]
-        _ok(hx.hoard_hx_gemv(ty, _ptr(wo), H, self.nq, _ptr(self.q8), _ptr(x), _ptr(x2), s), "gemv")
+
+    def _q_view(self, q):
+        """One token's q projection as [1][n_head][head_dim] (heads of a fused q + gate projection lie apart)."""
+        c = self.cfg
+        return q.view(1, c.n_head, -1)[:, :, :c.head_dim]
+
+    def _gate_view(self, q):
+        c = self.cfg
+        return q.view(1, c.n_head, -1)[:, :, c.head_dim:] if c.attn_gate else None
 
     def _layer_gdn(self, il, L, x, x2, hx, s, pos=None):
         """A gated delta-net block (src/run_qwen35.cpp:508-553): x2 = W_out gdn(RMSNorm(x) * attn_norm) + x."""
@@ -428,7 +547,9 @@ class DecodeModel:
         _ok(hx.hoard_hx_gemv(ty, _ptr(wo), H, self.gdn_vd, _ptr(self.q8), _ptr(x), _ptr(x2), s), "gemv")
 
     def reset_state(self):
-        """Zeroes the delta-net states (the start of a sequence; src/run_qwen35.cpp:366-373)."""
+        """Zeroes the delta-net states (the start of a sequence; src/run_qwen35.cpp:366-373) and empties a bounded
+        cache."""
+        self.n_rows = 0
         if hasattr(self, "gdn_state"):
             self.gdn_state.zero_()
 
@@ -448,6 +569,8 @@ class DecodeModel:
             "gemv")
         _ok(hx.hoard_hx_argmax_at(_ptr(self.logits), c.n_vocab, _ptr(self.seq), _ptr(self.pos_dev), self.seq.numel(), s),
             "argmax")
+        if self.budget:
+            self.rows_dev.add_(1)
 
     def prefill(self, prompt, stream=None):
         """Runs the prompt tokens but the last through the step (their KV entries), then sets the
@@ -458,6 +581,8 @@ class DecodeModel:
         for p in range(T - 1):
             self.step(p, self.scratch_tok, stream)
         self.pos_dev.fill_(T - 1)
+        if self.budget:
+            self.rows_dev.fill_(self.n_rows)
 
     def capture(self):
         """Captures one decode step (position in device memory) as a CUDA graph."""
@@ -476,14 +601,18 @@ class DecodeModel:
             raise ValueError("prompt + n_gen must fit max_ctx")
         g = self.capture()
         self.prefill(prompt)
-        for _ in range(n_gen):
+        for i in range(n_gen):
+            if self.budget and self.n_rows == self.budget.rows:
+                self._make_room(T - 1 + i)
+                self.rows_dev.fill_(self.n_rows)
             g.replay()
+            self.n_rows += 1
         torch.cuda.synchronize(self.dev)
         self.moe.sync_status()
         return self.seq[T:T + n_gen].tolist()
 
     def forward_batch(self, tokens, base: int, stream=None) -> torch.Tensor:
-        """One forward over m <= MAX_BATCH consecutive tokens at positions base .. base+m-1 (causal:
+        """One forward over m <= max_batch consecutive tokens at positions base .. base+m-1 (causal:
         token i attends to positions <= base+i; K/V stored for all m), the MoE layers batched (T = m).
         Returns the logits [m][vocab]; row i predicts position base+i+1. hoard's verify pass,
         src/run_specloop.cpp:76-150."""
@@ -491,22 +620,24 @@ class DecodeModel:
         m, H, hd = len(tokens), c.n_embd, c.head_dim
         if c.full_attn_interval > 0:
             raise ValueError("batched forward of a hybrid (delta-net) model is not supported: its state is sequential")
-        if not 1 <= m <= MAX_BATCH or base + m > self.max_ctx:
-            raise ValueError("batch must be 1..MAX_BATCH tokens inside max_ctx")
+        if self.budget:
+            raise ValueError("batched forward over a bounded cache is not supported: its rows are not positions")
+        if not 1 <= m <= self.max_batch or base + m > self.max_ctx:
+            raise ValueError("batch must be 1..max_batch tokens inside max_ctx")
         self.seq[base:base + m].copy_(torch.tensor(tokens, dtype=torch.int32))
         if not hasattr(self, "_xb"):
             z = lambda *sh: torch.zeros(*sh, dtype=torch.float32, device=self.dev)
-            self._xb, self._x2b, self._curb = z(MAX_BATCH, H), z(MAX_BATCH, H), z(MAX_BATCH, H)
-            self._qb, self._kb, self._vb = z(MAX_BATCH, self.nq), z(MAX_BATCH, self.nkv), z(MAX_BATCH, self.nkv)
-            self._attb, self._lgb = z(MAX_BATCH, self.nq), z(MAX_BATCH, c.n_vocab)
+            self._xb, self._x2b, self._curb = z(self.max_batch, H), z(self.max_batch, H), z(self.max_batch, H)
+            self._qb, self._kb, self._vb = z(self.max_batch, self.nq), z(self.max_batch, self.nkv), z(self.max_batch, self.nkv)
+            self._attb, self._lgb = z(self.max_batch, self.nq), z(self.max_batch, c.n_vocab)
         xb, x2b, cur = self._xb, self._x2b, self._curb
         for i in range(m):
             _ok(hx.hoard_hx_embed(self.embd_type, _ptr(self.embd), H, c.n_vocab, _ptr(self.seq[base + i:base + i + 1]),
                                   _ptr(xb[i]), s), "embed")
         if not hasattr(self, "_qrb"):
-            self._qrb = torch.zeros(MAX_BATCH, self.nq, dtype=torch.float32, device=self.dev)
+            self._qrb = torch.zeros(self.max_batch, self.nq, dtype=torch.float32, device=self.dev)
             self._qkv_yb = [_parr([self._qb[i].data_ptr(), self._kb[i].data_ptr(), self._vb[i].data_ptr()])
-                            for i in range(MAX_BATCH)]
+                            for i in range(self.max_batch)]
         for il, L in enumerate(self.layers):
             for i in range(m):
                 bufs = (self._qb[i], self._kb[i], self._vb[i], self._qrb[i], self._attb[i], self._qkv_yb[i])
@@ -525,8 +656,10 @@ class DecodeModel:
         accept the matching prefix, then run the corrected token. Greedy and lossless: the result
         equals generate()'s. Returns (tokens, {"rounds", "proposed", "accepted"})."""
         T, k_full = len(prompt), self.cfg.n_expert_used
-        if T < 1 or T + n_gen + k_draft + 1 > self.max_ctx or not 1 <= k_draft <= MAX_BATCH:
-            raise ValueError("prompt + n_gen + k_draft must fit max_ctx, 1 <= k_draft <= MAX_BATCH")
+        if self.budget:
+            raise ValueError("speculative decode over a bounded cache is not supported: its rows are not positions")
+        if T < 1 or T + n_gen + k_draft + 1 > self.max_ctx or not 1 <= k_draft <= self.max_batch:
+            raise ValueError("prompt + n_gen + k_draft must fit max_ctx, 1 <= k_draft <= max_batch")
         self.seq[:T].copy_(torch.tensor(prompt, dtype=torch.int32))
         for p in range(T):
             self.step(p, self.scratch_tok)
@@ -566,6 +699,135 @@ class DecodeModel:
             corrected = int(torch.argmax(last).item())
             out.append(corrected)
             self.seq[cur] = corrected
+            self.step(cur, self.scratch_tok)
+            pred = self.logits.clone()
+            cur += 1
+        self.moe.sync_status()
+        return out[:n_gen], stats
+
+    # ---- trees of drafted tokens ----
+    def forward_tree(self, tokens, parents, base: int, stream=None) -> torch.Tensor:
+        """One forward over a tree of m <= max_batch drafted tokens after `base` past positions: parents[i] is the
+        drafted token that token i follows (an earlier index), or -1 for the last past token. Token i takes position
+        base + its depth, its k and v cache row base + i; it attends to the past, its ancestors and itself. The layers'
+        attention is one call for all tokens, and so are the MoE layers (T = m). Returns the logits [m][vocab]; row i
+        predicts what follows token i. With parents = [-1, 0, 1, ..] it is forward_batch."""
+        c, hx, s = self.cfg, _hx(), _stream(stream)
+        m, H, hd = len(tokens), c.n_embd, c.head_dim
+        words, depth = cache.tree_visibility(parents)
+        if c.full_attn_interval > 0:
+            raise ValueError("batched forward of a hybrid (delta-net) model is not supported: its state is sequential")
+        if self.budget:
+            raise ValueError("batched forward over a bounded cache is not supported: its rows are not positions")
+        if len(parents) != m or m > self.max_batch or base < 0 or base + m > self.max_ctx:
+            raise ValueError("a tree has a parent for each of its 1..max_batch tokens, inside max_ctx")
+        if self._tree_ops is None:
+            self._tree_ops = cache.CacheOps(**self._ops_args, max_tokens=self.max_batch, max_acc_tokens=0)
+            z = lambda *sh: torch.zeros(*sh, dtype=torch.float32, device=self.dev)
+            B = self.max_batch
+            self._tq, self._tk, self._tv = z(B, self.nqp), z(B, self.nkv), z(B, self.nkv)
+            self._tx, self._tx2, self._trot, self._tatt = z(B, H), z(B, H), z(B, self.nq), z(B, self.nq)
+            self._tlg = z(B, c.n_vocab)
+            self._tqkv = [_parr([self._tq[i].data_ptr(), self._tk[i].data_ptr(), self._tv[i].data_ptr()]) for i in range(B)]
+        vis = torch.tensor(words, dtype=torch.int64).to(self.dev)
+        pos = torch.tensor([base + d for d in depth], dtype=torch.int32).to(self.dev)
+        tok = torch.tensor(list(tokens), dtype=torch.int32).to(self.dev)
+        x, x2 = self._tx, self._tx2
+        for i in range(m):
+            _ok(hx.hoard_hx_embed(self.embd_type, _ptr(self.embd), H, c.n_vocab, _ptr(tok[i:i + 1]), _ptr(x[i]), s), "embed")
+        q = self._tq[:m].view(m, c.n_head, -1)
+        mode = QK_MODE[c.qk_norm]
+        for il, L in enumerate(self.layers):
+            for i in range(m):
+                _ok(hx.hoard_hx_rmsnorm_q8(_ptr(x[i]), H, c.eps, _ptr(L["attn_norm"]), _ptr(self.q8), s), "rmsnorm_q8")
+                _ok(hx.hoard_hx_gemv_multi(3, L["qkv_types"], L["qkv_w"], self.qkv_N, H, _ptr(self.q8), None, self._tqkv[i],
+                                           s), "gemv qkv")
+            j = self.kv_index[il]
+            k3, v3 = self._heads(self.kc[j]), self._heads(self.vc[j])
+            rot = self._tree_ops.store(q[:, :, :hd], self._tk[:m].view(m, c.n_head_kv, hd),
+                                       self._tv[:m].view(m, c.n_head_kv, hd), k3, v3, pos, base, q_norm=L.get("q_norm"),
+                                       k_norm=L.get("k_norm"), mode=mode, eps=c.eps, rope_dim=c.n_rot,
+                                       freq_base=c.freq_base, q_out=self._trot[:m].view(m, c.n_head, hd), stream=s)
+            args = dict(vis=vis, gate=q[:, :, hd:] if c.attn_gate else None, out=self._tatt[:m].view(m, c.n_head, hd), stream=s)
+            if self.blocks:
+                bc = self.blocks
+                self._tree_ops.block_attention(rot, k3, v3, self.bounds[j], base, n_sink=bc.n_sink, n_local=bc.n_local,
+                                               n_sel=bc.n_sel, **args)
+            else:
+                self._tree_ops.tree_attention(rot, k3, v3, base, **args)
+            ty, wo = L["o"]
+            for i in range(m):
+                _ok(hx.hoard_hx_quant_q8(_ptr(self._tatt[i]), self.nq, _ptr(self.q8), s), "quant")
+                _ok(hx.hoard_hx_gemv(ty, _ptr(wo), H, self.nq, _ptr(self.q8), _ptr(x[i]), _ptr(x2[i]), s), "gemv")
+            self.moe.layers(il, 1, x2[:m], stream=stream)
+            x, x2 = x2, x
+        for i in range(m):
+            _ok(hx.hoard_hx_rmsnorm_q8(_ptr(x[i]), H, c.eps, _ptr(self.out_norm), _ptr(self.q8), s), "rmsnorm_q8")
+            _ok(hx.hoard_hx_gemv(self.out_type, _ptr(self.out_w), c.n_vocab, H, _ptr(self.q8), None, _ptr(self._tlg[i]), s),
+                "gemv")
+        return self._tlg[:m].clone()
+
+    def accept(self, base: int, path, stream=None):
+        """After forward_tree at `base`: the k and v of the drafted tokens path[0], path[1], .. (a root and its accepted
+        descendants) become cache rows base, base + 1, .."""
+        for j in range(len(self.kv_index)):
+            k3, v3 = self._heads(self.kc[j]), self._heads(self.vc[j])
+            self._tree_ops.take(k3, v3, base, path, stream=stream)
+            if self.blocks and path:
+                self._tree_ops.block_bounds(k3, self.bounds[j], base, base + len(path), stream=stream)
+
+    def tree_generate(self, prompt, n_gen: int, depth: int = 4, width: int = 2):
+        """speculative_generate with a tree: at each of `depth` levels the draft (this model at its top-1 expert) offers its
+        `width` best tokens and goes on from the best; one forward_tree verifies all of them, the longest path that the
+        full model agrees with is accepted, then the corrected token runs. Greedy and lossless. Returns (tokens,
+        {"rounds", "proposed", "accepted"})."""
+        T, k_full = len(prompt), self.cfg.n_expert_used
+        if self.budget or self.cfg.full_attn_interval > 0:
+            raise ValueError("a tree of drafts needs a cache whose rows are positions, and no delta-net state")
+        if (T < 1 or depth < 1 or width < 1 or depth * width > self.max_batch
+                or T + n_gen + depth * width + 1 > self.max_ctx):
+            raise ValueError("prompt + n_gen + the tree must fit max_ctx, depth * width <= max_batch")
+        self.seq[:T].copy_(torch.tensor(prompt, dtype=torch.int32))
+        self.reset_state()
+        for p in range(T):
+            self.step(p, self.scratch_tok)
+        pred = self.logits.clone()
+        cur, out, stats = T, [], {"rounds": 0, "proposed": 0, "accepted": 0}
+        while len(out) < n_gen:
+            tokens, parents, lg, parent = [], [], pred, -1
+            self.moe.set_top_k(1)
+            try:
+                for d in range(depth):
+                    best = torch.topk(lg, width).indices.tolist()
+                    first = len(tokens)
+                    tokens += best
+                    parents += [parent] * width
+                    parent = first
+                    if d + 1 < depth:
+                        self.seq[cur + d] = best[0]
+                        self.step(cur + d, self.scratch_tok)
+                        lg = self.logits.clone()
+            finally:
+                self.moe.set_top_k(k_full)
+            V = self.forward_tree(tokens, parents, cur)
+            path, at, want = [], -1, int(torch.argmax(pred).item())
+            while True:
+                hit = [i for i, (t, p) in enumerate(zip(tokens, parents)) if p == at and t == want]
+                if not hit:
+                    break
+                at = hit[0]
+                path.append(at)
+                want = int(torch.argmax(V[at]).item())
+            self.accept(cur, path)
+            stats["rounds"] += 1
+            stats["proposed"] += len(tokens)
+            stats["accepted"] += len(path)
+            out += [tokens[i] for i in path]
+            cur += len(path)
+            if len(out) >= n_gen:
+                break
+            out.append(want)
+            self.seq[cur] = want
             self.step(cur, self.scratch_tok)
             pred = self.logits.clone()
             cur += 1
