@@ -33,7 +33,8 @@ class Desc(ctypes.Structure):
 # hoard_kv_query: q and its token and head strides, k_cache, v_cache, visible, gate and its strides, out, m, n_past,
 # n_past_dev
 _QUERY = struct.Struct("@PqqPPPPqqPiiP")
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_F32, _NO_STRIDE = torch.float32, (0, 0)
 _bound = False
 
 
@@ -91,6 +92,7 @@ class CacheOps:
         self._q = ctypes.create_string_buffer(_QUERY.size)
         self._dp, self._qp = ctypes.addressof(self._d), ctypes.addressof(self._q)
         self._cache_shape, self._cache_stride = (max_rows, n_head_kv, head_dim), None
+        self._head_shape = (n_head, head_dim)
         n = _kv().hoard_kv_ws_bytes(self._dp)
         if n < 0:
             raise HoardError(-1, "hoard_kv_ws_bytes: descriptor refused")
@@ -102,7 +104,7 @@ class CacheOps:
     # The checks read each attribute of a tensor once: at the sizes of a decode step they are a good part of a call.
     def _run(self, fn, stream, *args):
         """fn(*args, stream) on this object's device."""
-        if torch.cuda.current_device() != self.device:
+        if _current_device() != self.device:
             with torch.cuda.device(self.device):
                 return self._run(fn, stream, *args)
         if stream is None:
@@ -140,20 +142,26 @@ class CacheOps:
         return x.data_ptr()
 
     def _query(self, q, k_cache, v_cache, n_past, vis, gate, out, n_past_dev):
-        m = len(q)
-        shape = (m, self.n_head, self.head_dim)
-        qs = self._heads(q, shape, "q")
-        self._caches(k_cache, v_cache)
+        dev, shape, qs, ks = self.device, q.shape, q.stride(), k_cache.stride()
+        if (shape[1:] != self._head_shape or q.dtype is not _F32 or q.get_device() != dev or qs[2] != 1):
+            raise ValueError(f"q is a [m, {self.n_head}, {self.head_dim}] float32 tensor on device {dev} with contiguous heads")
+        if ks != self._cache_stride or k_cache.shape != self._cache_shape or k_cache.dtype is not self.kv_dtype or \
+                k_cache.get_device() != dev or v_cache.stride() != ks or v_cache.shape != self._cache_shape or \
+                v_cache.dtype is not self.kv_dtype or v_cache.get_device() != dev:
+            self._caches(k_cache, v_cache)
+        m = shape[0]
         if gate is None:
-            gp, gs = 0, (0, 0)
+            gp, gs = 0, _NO_STRIDE
         else:
             gs = self._heads(gate, shape, "gate")
             gp = gate.data_ptr()
         if out is None:
-            out = torch.empty(shape, dtype=torch.float32, device=q.device)
+            out = torch.empty(shape, dtype=_F32, device=q.device)
+        elif out.shape != shape or out.dtype is not _F32 or out.get_device() != dev or not out.is_contiguous():
+            raise ValueError(f"out is a contiguous {list(shape)} float32 tensor on device {dev}")
         _QUERY.pack_into(self._q, 0, q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(),
                          0 if vis is None else self._contiguous(vis, (m,), torch.int64, "vis"), gp, gs[0], gs[1],
-                         self._contiguous(out, shape, torch.float32, "out"), m, n_past,
+                         out.data_ptr(), m, n_past,
                          0 if n_past_dev is None else self._contiguous(n_past_dev, (1,), torch.int32, "n_past_dev"))
         return out
 

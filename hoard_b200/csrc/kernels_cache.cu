@@ -460,6 +460,19 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
     if ((int)blockIdx.x < n_rows) {
         const int at = blockIdx.x / col_blocks, prob = at / a.R, row = at - prob * a.R;
         const int64_t part = (int64_t)prob * a.splits * a.R + row;       // + split * R
+        // this CTA's float4 columns, shared out over split groups. The first round of sums is on its way before the
+        // factors are known (what a split without weight left there is not used)
+        const int v4 = (a.hd / 4 + col_blocks - 1) / col_blocks, groups = CB / v4, gi = tid / v4;
+        const int lc = tid - gi * v4, c = (blockIdx.x - at * col_blocks) * v4 + lc;
+        const bool mine = gi < groups && 4 * c < a.hd;
+        const float* po = a.part_o + part * hdt + 4 * c;
+        float4 u[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int s = gi + k * groups;
+            u[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (mine && s < a.splits) u[k] = *reinterpret_cast<const float4*>(po + (int64_t)s * a.R * hdt);
+        }
         const float2 ml = tid < a.splits ? a.part_ml[part + (int64_t)tid * a.R] : make_float2(-INFINITY, 0.f);
         const float wm = warp_max(ml.x);
         if (lane == 0) s_red[0][warp] = wm;
@@ -475,28 +488,26 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
         float l = s_red[1][0];
 #pragma unroll
         for (int w = 1; w < CB / 32; ++w) l += s_red[1][w];
-        // this CTA's float4 columns, shared out over split groups
-        const int v4 = (a.hd / 4 + col_blocks - 1) / col_blocks, groups = CB / v4, gi = tid / v4;
-        const int lc = tid - gi * v4, c = (blockIdx.x - at * col_blocks) * v4 + lc;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (gi < groups && 4 * c < a.hd) {
-            const float* po = a.part_o + part * hdt + 4 * c;
-            for (int s0 = gi; s0 < a.splits; s0 += 8 * groups) {
-                float4 u[8];
-                float w[8];
+        if (mine) {
+            for (int s0 = gi;;) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int s = s0 + k * groups;
-                    w[k] = s < a.splits ? s_f[s] : 0.f;
-                    u[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (w[k] != 0.f) u[k] = *reinterpret_cast<const float4*>(po + (int64_t)s * a.R * hdt);
+                    const float w = s < a.splits ? s_f[s] : 0.f;
+                    if (w != 0.f) {
+                        v.x += w * u[k].x;
+                        v.y += w * u[k].y;
+                        v.z += w * u[k].z;
+                        v.w += w * u[k].w;
+                    }
                 }
+                s0 += 8 * groups;
+                if (s0 >= a.splits) break;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    v.x += w[k] * u[k].x;
-                    v.y += w[k] * u[k].y;
-                    v.z += w[k] * u[k].z;
-                    v.w += w[k] * u[k].w;
+                    const int s = s0 + k * groups;
+                    if (s < a.splits) u[k] = *reinterpret_cast<const float4*>(po + (int64_t)s * a.R * hdt);
                 }
             }
             s_o[tid] = v;

@@ -12,7 +12,9 @@
 //   warps 1-3    copy K and V tiles into a ring (cp.async, rows past the end as zeros)
 //   warps 4-7, 8-11   two softmax groups, even and odd tiles: each has its own running maximum, total and f32 sums
 //                (head_dim registers per thread) and the two are joined at the end.
-// The products of one group's tile run while the other group works on its own: PV(j), S(j+2), PV(j+1), S(j+3), ..
+// The products of one group's tile run while the other group works on its own: PV(j), S(j+NSB), PV(j+1), .. Three
+// tiles of S are in flight for f16 (two for bf16, whose terms leave no room), so that a group finds its next scores
+// ready; the tile of a steady state took 1500 cycles with two and 1170 are the products'.
 // The tensor cores truncate as they accumulate, so a tile's O leaves tensor memory after every tile and is added
 // with rounding, sums scaled to a risen maximum in the same multiply-add.
 // The last tile is the tokens' own rows, with their masks. k_cache_combine joins the splits.
@@ -124,19 +126,20 @@ template <typename KT, int HD> struct TcPlan {
     static constexpr int RING = STAGES * STAGE;
     static_assert(Q_OFF + TM * (HD + Q_PAD) * 4 <= RING, "staged q over the ring's later stages");
     static_assert(TM * (HD + 4) * 4 <= RING, "join buffer");
-    // tensor memory, in columns: Q terms, two tiles of S (P's terms over it), O
+    // tensor memory, in columns: Q terms, tiles of S (P's terms over it; what fits beside the other two), O
+    static constexpr int NSB = TN == 2 ? 3 : 2;
     static constexpr int Q_COLS = HD / 2, P_COLS = TK / 2;
     static constexpr int SP = TN * P_COLS > TK ? TN * P_COLS : TK;
-    static constexpr int C_Q = 0, C_S = TN * Q_COLS, C_O = C_S + 2 * SP;
+    static constexpr int C_Q = 0, C_S = TN * Q_COLS, C_O = C_S + NSB * SP;
     static_assert(C_O + HD <= 512, "tensor memory");
 };
 
 template <typename KT, int HD>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const CacheAttn a) {
     using P = TcPlan<KT, HD>;
-    constexpr int TN = P::TN, ST = P::STAGES;
+    constexpr int TN = P::TN, ST = P::STAGES, NSB = P::NSB;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[ST], empty[ST], s_full[2], p_full[2], o_full[2], o_empty, q_full, done;
+    __shared__ uint64_t full[ST], empty[ST], s_full[NSB], p_full[NSB], o_full[2], o_empty, q_full, done;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_give_up;
     __shared__ float s_mx[2][TM], s_tot[2][TM];
@@ -151,11 +154,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
             mbar_init(&full[i], LOADERS);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NSB; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], GROUP);
-            mbar_init(&o_full[i], 1);
         }
+        for (int i = 0; i < 2; ++i) mbar_init(&o_full[i], 1);
         mbar_init(&o_empty, GROUP);
         mbar_init(&q_full, 2 * GROUP);
         mbar_init(&done, 1);
@@ -208,11 +211,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
                         ph_s ^= 1;
                     }
                 };
-                score(0);
-                if (T > 1) score(1);
+                for (int j = 0; j < NSB && j < T; ++j) score(j);
+                int b = 0, ph_b = 0;                   // buffer of S(j), the phase of its uses
                 for (int j = 0; j < T && ok; ++j) {
-                    const int b = j & 1;
-                    ok = wait(&p_full[b], (j >> 1) & 1) && (j == 0 || wait(&o_empty, b ^ 1));
+                    ok = wait(&p_full[b], ph_b) && (j == 0 || wait(&o_empty, (j - 1) & 1));
                     if (!ok) break;
                     tc_after();
                     const uint64_t vd = desc_sw128(ring + st_o * P::STAGE + (HD / 64) * P::SUB, P::SUB);
@@ -222,10 +224,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
                         for (int k = 0; k < TK / 16; ++k)
                             tc_mma(tmem + P::C_O, tmem + P::C_S + b * P::SP + u * P::P_COLS + 8 * k, vd + (k * 2048 >> 4),
                                    tc_idesc<KT>(HD, true), u != TN - 1 || k != 0, elected);
-                    tc_commit(&o_full[b], elected);
+                    tc_commit(&o_full[j & 1], elected);
                     tc_commit(&empty[st_o], elected);
                     if (++st_o == ST) st_o = 0;
-                    if (j + 2 < T) score(b);
+                    if (j + NSB < T) score(b);
+                    if (++b == NSB) {
+                        b = 0;
+                        ph_b ^= 1;
+                    }
                 }
                 // nothing of this warp's is in flight when tensor memory is freed
                 tc_commit(&done, elected);
@@ -366,9 +372,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
             return __all_sync(0xffffffffu, wait_or_give_up(bar, parity, &s_give_up)) != 0;
         };
         for (int j = grp; j < T; j += 2) {
-            if (!(ok = group_wait(&s_full[grp], (j >> 1) & 1))) break;
+            const int buf = j % NSB;
+            if (!(ok = group_wait(&s_full[buf], (j / NSB) & 1))) break;
             tc_after();
-            const uint32_t sp = tmem + lanes + P::C_S + grp * P::SP;
+            const uint32_t sp = tmem + lanes + P::C_S + buf * P::SP;
             uint32_t sr[TK];
             tc_ld32(sp, sr);
             tc_ld32(sp + 32, sr + 32);
@@ -447,7 +454,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
                 }
             }
             tc_before();
-            mbar_arrive(&p_full[grp]);
+            mbar_arrive(&p_full[buf]);
             if (!(ok = group_wait(&o_full[grp], (j >> 1) & 1))) break;
             tc_after();
             if (!odd) {
