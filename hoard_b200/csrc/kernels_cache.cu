@@ -18,6 +18,10 @@
 #include "async_copy.cuh"
 #include "kv_terms.cuh"
 
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
 namespace hoard {
 
 namespace {
@@ -56,6 +60,7 @@ template <int N> __device__ __forceinline__ void cp_wait() {
 // Warps and ring slots of one CTA (one CTA per SM). A slot is the K or the V of 16 rows; eight warps with all but one
 // of their slots in flight keep 128 to 160 KiB per SM on the way.
 constexpr int W = 8;
+constexpr int MAX_CLUSTER = 4;           // CTAs of a cluster: with a CTA per SM, eight rarely fit in a GPC at once
 template <int HD> struct Plan {
     static constexpr int NS = HD == 256 ? 3 : 6;
     static constexpr int SLOT = KV_CHUNK * HD * 2;                 // bytes
@@ -81,6 +86,8 @@ __global__ void __launch_bounds__(W * 32, 1) k_cache_attention(const CacheAttn a
     __shared__ float s_scale[RT];                      // per query row: scale, log2(e) and the row's power of two
     __shared__ uint64_t s_vis[RT];
     __shared__ float s_m[W][RT], s_l[W][RT];
+    __shared__ float2 s_ml[RT];                        // the CTA's maxima and totals
+    __shared__ float s_fac[MAX_CLUSTER][RT], s_top[RT], s_inv[RT];
     pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, tile = blockIdx.y, prob = blockIdx.z;
@@ -405,17 +412,38 @@ __global__ void __launch_bounds__(W * 32, 1) k_cache_attention(const CacheAttn a
             }
         }
     __syncthreads();
-    const bool whole = a.splits == 1 && !a.logits;     // nothing to join with: the output itself
-    const int64_t part = ((int64_t)prob * a.splits + split) * a.R;
+    // the rows' maxima and totals over the warps, then the sums: to the output where nothing is to be joined, to the
+    // partial results, or for the cluster in place of the first warp's
+    const bool single = a.cluster && a.splits == 1;
+    if (tid < RT) {
+        float top = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][tid]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) l += s_m[w][tid] == -INFINITY ? 0.f : s_l[w][tid] * ex2f(s_m[w][tid] - top);
+        s_ml[tid] = make_float2(top, l);
+        s_top[tid] = top;
+        s_inv[tid] = l == 0.f ? 0.f : 1.f / l;
+        if (!a.cluster && tile * RT + tid < a.R)
+            a.part_ml[((int64_t)prob * a.splits + split) * a.R + tile * RT + tid] = make_float2(top, l);
+    }
+    if (single) __syncthreads();
+    auto put = [&](int r, int d, float4 v) {           // the output of row r of the tile, dims d ..
+        const int row = tile * RT + r, tt = row / a.g, t = t0 + tt, h = kv * a.g + row - tt * a.g;
+        const float inv = s_inv[r];
+        float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+        if (a.gate) {
+            const float* gp = a.gate + t * a.gate_ts + h * a.gate_hs + d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] *= sigmoid_f(gp[i]);
+        }
+        store4(a.out + ((int64_t)t * a.n_head + h) * a.hd + d, y);
+    };
+    float* sums = joined;
     for (int x = tid; x < RT * (HD / 4); x += W * 32) {
         const int r = x / (HD / 4), d = (x - r * (HD / 4)) * 4;
         const int row = tile * RT + r;
-        if (row >= a.R) continue;
-        float top = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][r]);
-#pragma unroll
-        for (int w = 0; w < W; ++w) l += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * ex2f(s_m[w][r] - top);
+        if (row >= a.R || d >= a.hd) continue;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -425,22 +453,78 @@ __global__ void __launch_bounds__(W * 32, 1) k_cache_attention(const CacheAttn a
             v.z += u.z;
             v.w += u.w;
         }
-        if (whole) {
-            if (d >= a.hd) continue;
-            const int t = t0 + row / a.g, h = kv * a.g + row % a.g;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-            if (a.gate) {
-                const float* gp = a.gate + t * a.gate_ts + h * a.gate_hs + d;
+        if (single) put(r, d, v);
+        else if (a.cluster) *reinterpret_cast<float4*>(sums + r * OP + d) = v;
+        else *reinterpret_cast<float4*>(a.part_o + ((((int64_t)prob * a.splits + split) * a.R) + row) * HD + d) = v;
+    }
+    if (!a.cluster) return;
+
+    // ---- the splits are the CTAs of a cluster: each has every split's maximum and total of the rows, joins its share of
+    // the rows' sums and, with weights to accumulate, adds those of its own cache rows ----
+    cg::cluster_group cl = cg::this_cluster();
+    if (!single) {
+        cl.sync();
+        if (tid < RT) {
+            float2 ml[MAX_CLUSTER];
+            float top = -INFINITY, l = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] *= sigmoid_f(gp[i]);
+            for (int c = 0; c < MAX_CLUSTER; ++c) {
+                ml[c] = make_float2(-INFINITY, 0.f);
+                if (c < a.splits) ml[c] = *cl.map_shared_rank(&s_ml[tid], c);
+                top = fmaxf(top, ml[c].x);
             }
-            store4(a.out + ((int64_t)t * a.n_head + h) * a.hd + d, y);
-        } else {
-            *reinterpret_cast<float4*>(a.part_o + (part + row) * HD + d) = v;
-            if (d == 0) a.part_ml[part + row] = make_float2(top, l);
+#pragma unroll
+            for (int c = 0; c < MAX_CLUSTER; ++c) {
+                const float f = ml[c].x == -INFINITY ? 0.f : ex2f(ml[c].x - top);
+                s_fac[c][tid] = f;
+                l += f == 0.f ? 0.f : f * ml[c].y;
+            }
+            s_top[tid] = top;
+            s_inv[tid] = l == 0.f ? 0.f : 1.f / l;
+        }
+        const int share = (RT + a.splits - 1) / a.splits, r0 = split * share;
+        for (int x0 = 0; x0 < share * (HD / 4); x0 += W * 32) {
+            const int x = x0 + tid, rr = x / (HD / 4), r = r0 + rr, d = (x - rr * (HD / 4)) * 4;
+            const bool mine = rr < share && r < RT && tile * RT + r < a.R && d < a.hd;
+            float4 u[MAX_CLUSTER];
+#pragma unroll
+            for (int c = 0; c < MAX_CLUSTER; ++c)
+                if (mine && c < a.splits) u[c] = *reinterpret_cast<const float4*>(cl.map_shared_rank(sums, c) + r * OP + d);
+            if (x0 == 0) __syncthreads();              // the factors are known
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (mine) {
+#pragma unroll
+                for (int c = 0; c < MAX_CLUSTER; ++c) {
+                    const float f = s_fac[c][r];
+                    if (c < a.splits && f != 0.f) {
+                        v.x += f * u[c].x;
+                        v.y += f * u[c].y;
+                        v.z += f * u[c].z;
+                        v.w += f * u[c].w;
+                    }
+                }
+                put(r, d, v);
+            }
         }
     }
+    if (!BLOCKS && a.logits) {                         // one row tile: these are all the query rows of the KV head
+        const float* lg = a.logits + (int64_t)kv * a.R * a.logits_ld;
+        float* acc = a.acc + (int64_t)kv * a.max_rows;
+        const int c0 = c_first - warp;                 // this CTA's first chunk
+        for (int x = tid; x < (c_end - c0) * KV_CHUNK; x += W * 32) {
+            const int c = c0 + x / KV_CHUNK, j = chunk_row(c) + x % KV_CHUNK;
+            if (j >= chunk_end(c)) continue;
+            const float before = acc[j];
+            float lv[RT], w = 0.f;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) lv[r] = r < a.R ? lg[(int64_t)r * a.logits_ld + j] : -INFINITY;
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                if (r < a.R && s_inv[r] != 0.f) w += ex2f(lv[r] - (s_top[r] - Terms<KT>::P_EXP)) * s_inv[r];
+            acc[j] = before + w;
+        }
+    }
+    if (!single) cl.sync();                            // no CTA leaves while its sums may be read
 }
 
 // ---- joins the splits of every query row, and with acc adds the rows' weights to the accumulated ones -------
@@ -593,8 +677,9 @@ cudaError_t attention_go(const CacheAttn& a, cudaStream_t s) {
     static SmemLimit limit;
     cudaError_t e = limit.raise((const void*)k_cache_attention<KT, HD, NT, BLOCKS>, smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_cache_attention<KT, HD, NT, BLOCKS>, dim3(a.splits, a.row_tiles, a.problems),
-                      W * 32, smem, s, a);
+    const dim3 grid(a.splits, a.row_tiles, a.problems);
+    if (!a.cluster) return launch_pdl(k_cache_attention<KT, HD, NT, BLOCKS>, grid, W * 32, smem, s, a);
+    return launch_pdl_cluster(k_cache_attention<KT, HD, NT, BLOCKS>, a.splits, grid, W * 32, smem, s, a);
 }
 template <typename KT, int HD, int NT> cudaError_t attention_form(const CacheAttn& a, cudaStream_t s) {
     return a.list ? attention_go<KT, HD, NT, true>(a, s) : attention_go<KT, HD, NT, false>(a, s);
@@ -617,15 +702,24 @@ int cache_tile_dims(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 // read the cache half as often: with 16 rows of 4 heads of 128, 8 against 16 take 9.1 / 9.9 us over 4000 cache
 // rows, 14.5 / 14.2 over 16000, 35.5 / 30.1 over 60000; with 16 heads 9.2 / 9.8 over 1000, 15.5 / 14.0 over 4000.
 // The two cross where a warp of a full grid has about five chunks.
-// Splits: one CTA per SM over problems and tiles, each warp with a chunk; but a second kernel to join them costs
-// 3 us, about four chunks of a warp, so up to that many one CTA takes them all (`join`: it runs anyway).
-void cache_plan(CacheAttn& a, int n_chunks, bool join) {
+// Splits: up to four are the CTAs of a cluster, which joins them itself (about 1 us where there is more than one);
+// more are joined by a second kernel (3 us). A chunk of a warp is 0.8 us. So: two chunks of a warp in one CTA; up to
+// three and a half in four; else one CTA per SM over problems and tiles, each warp with a chunk. (Clusters of eight
+// waited for SMs: 3460 rows of 4 heads 11.7 us, against 8.2 with 28 splits.)
+// Weights are accumulated by the cluster too, where one tile holds all query rows of a KV head.
+void cache_plan(CacheAttn& a, int n_chunks) {
     const int64_t w = W, tiles8 = (a.R + 7) / 8;
     a.tile_rows = a.R > 8 && a.problems * tiles8 * n_chunks > 5 * w * KV_SMS ? 16 : 8;
+    if (a.logits && a.R > 8 && a.R <= 16) a.tile_rows = 16;
     a.row_tiles = (a.R + a.tile_rows - 1) / a.tile_rows;
     const int64_t most = KV_SMS / ((int64_t)a.problems * a.row_tiles), useful = (n_chunks + w - 1) / w;
     a.splits = (int)(most < useful ? most : useful);
-    if (a.splits < 1 || (!join && n_chunks <= 4 * w)) a.splits = 1;
+    if (a.splits < 1) a.splits = 1;
+    const int wide = most >= 4 ? 4 : most >= 2 ? 2 : 1;
+    int in_cluster = 1;                                // fewest CTAs (1, 2, 4) that leave a warp two chunks
+    while (in_cluster < wide && n_chunks > 2 * w * in_cluster) in_cluster *= 2;
+    a.cluster = (!a.logits || a.row_tiles == 1) && (a.splits <= in_cluster || 2 * n_chunks <= 7 * w * in_cluster);
+    if (a.cluster) a.splits = in_cluster;
 }
 
 // Splits for the tensor-core form: one CTA per SM over KV heads and tiles of 128 query rows, each with TC_MIN_TILES
@@ -641,7 +735,7 @@ cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s) {
     const cudaError_t e = a.tc_splits ? launch_cache_attention_tc(a, s)
                           : a.bf16    ? attention_type<__nv_bfloat16>(a, s)
                                       : attention_type<__half>(a, s);
-    if (e != cudaSuccess || (a.splits == 1 && !a.logits)) return e;
+    if (e != cudaSuccess || (a.tc_splits ? a.splits == 1 : a.cluster)) return e;
     const int rows = a.n_past_dev ? a.max_rows : a.n_past + a.m;
     const int per = (rows + ACC_ROWS - 1) / ACC_ROWS;                  // accumulating CTAs of a KV head
     const int n_rows = a.problems * a.R;

@@ -28,6 +28,27 @@ struct SmemLimit {
     }
 };
 
+// a programmatic dependent launch in clusters of `cl` CTAs along x
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), int cl, dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                                      Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cl;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // The cache and the query side of one attention call. Strides in elements (caches) and floats (q, gate).
 struct CacheAttn {
     const float* q;
@@ -46,6 +67,7 @@ struct CacheAttn {
     // its query heads, or with a block list a (token, KV head) with R = g.
     int problems, R, tile_rows, row_tiles, splits;
     int tc_splits;                       // splits of the tensor-core form, 0 where it does not run
+    bool cluster;                        // the splits are a cluster's CTAs and are joined by it
     // partial results of each (problem, split, query row): unnormalised sums, running maxima and totals
     float* part_o;                       // [problems][splits][R][tile dims]
     float2* part_ml;                     // [problems][splits][R]
@@ -59,7 +81,7 @@ struct CacheAttn {
 };
 
 int cache_tile_dims(int hd);             // dims of the instantiation that runs a head_dim
-void cache_plan(CacheAttn& a, int n_chunks, bool join);                  // sets tile_rows, row_tiles, splits
+void cache_plan(CacheAttn& a, int n_chunks);                             // sets tile_rows, row_tiles, splits, cluster
 int cache_tc_splits(int hd, int n_kv, int R, int64_t past_rows);
 cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s);
 cudaError_t launch_cache_attention_tc(const CacheAttn& a, cudaStream_t s);

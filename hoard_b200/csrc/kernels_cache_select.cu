@@ -715,27 +715,6 @@ __global__ void __launch_bounds__(32) k_cache_take(char* kc, char* vc, int64_t r
 
 }  // namespace
 
-// a programmatic dependent launch in clusters of `cl` CTAs along x
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_cluster(void (*kernel)(KArgs...), int cl, dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                                  Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = cl;
-    at[1].val.clusterDim.y = 1;
-    at[1].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 cudaError_t launch_cache_evict(const CacheEvict& e, cudaStream_t s) {
     const int most = e.n_keep < e.n_rows - e.n_keep ? e.n_keep : e.n_rows - e.n_keep;      // moves
     if (e.n_rows <= EV_SINGLE) {
@@ -750,7 +729,7 @@ cudaError_t launch_cache_evict(const CacheEvict& e, cudaStream_t s) {
         cudaError_t rc = limit.raise((const void*)k_evict_choose<CL>, EV_KEYS * 4);
         if (rc != cudaSuccess) return rc;
         const int n = (e.n_rows + CL - 1) / CL;
-        rc = launch_cluster(k_evict_choose<CL>, CL, dim3(CL, e.n_kv), SEL_THREADS, n <= EV_KEYS ? (size_t)n * 4 : 0, s, e,
+        rc = launch_pdl_cluster(k_evict_choose<CL>, CL, dim3(CL, e.n_kv), SEL_THREADS, n <= EV_KEYS ? (size_t)n * 4 : 0, s, e,
                             false);
         if (rc != cudaSuccess) return rc;
     }
@@ -800,7 +779,7 @@ cudaError_t launch_cache_select(const CacheSelect& asked, cudaStream_t s) {
     static SmemLimit limit;
     e = limit.raise((const void*)k_block_choose<CL>, 128 * 1024);
     if (e != cudaSuccess) return e;
-    return launch_cluster(k_block_choose<CL>, CL, dim3(CL, c.n_kv, c.m), SEL_THREADS, (size_t)((n_cand + CL - 1) / CL) * 8, s,
+    return launch_pdl_cluster(k_block_choose<CL>, CL, dim3(CL, c.n_kv, c.m), SEL_THREADS, (size_t)((n_cand + CL - 1) / CL) * 8, s,
                           c, nb_cap);
 }
 
