@@ -608,11 +608,15 @@ __global__ void __launch_bounds__(SC_THREADS) k_block_score(const CacheSelect c,
 // ---- selection: one CTA or cluster per (KV head, token) -------------------------------------------------------
 // Key of a score max_h (u_h - top_h) <= 0: the bits of its magnitude, turned over; NaN lowest.
 constexpr int BS_MAX_G = 64;
-constexpr int BS_SINGLE = 8192;          // candidates up to which one CTA chooses alone
+// Candidates up to which one CTA chooses, and above which a cluster's eight form the keys for it, if the clusters of all
+// problems fit on the GPU at once: 4086 candidates x 8 heads 14 us alone, 11.5 with a cluster; 1557 candidates of 32
+// problems 10 alone, 17 with clusters.
+constexpr int BS_ONE = 8192, BS_ALONE = 1024;
 __device__ __forceinline__ unsigned long long score_key(double v) {
     return v != v ? 0ull : 0x7FFFFFFFFFFFFFFFull - (unsigned long long)__double_as_longlong(fabs(v));
 }
-template <int CLN>
+// CLN > 1 and GATHER: the cluster's CTAs form the keys, the first of them chooses; without GATHER all choose together.
+template <int CLN, bool GATHER>
 __global__ void __launch_bounds__(SEL_THREADS) k_block_choose(const CacheSelect c, int nb_cap) {
     pdl_enter();
     extern __shared__ unsigned long long s_keys[];
@@ -640,37 +644,47 @@ __global__ void __launch_bounds__(SEL_THREADS) k_block_choose(const CacheSelect 
         return;
     }
     if (n_take == 0) return;
-    const int i0 = (int)((int64_t)n_cand * rank / CLN), i1 = (int)((int64_t)n_cand * (rank + 1) / CLN), n = i1 - i0;
+    int i0 = (int)((int64_t)n_cand * rank / CLN), n = (int)((int64_t)n_cand * (rank + 1) / CLN) - i0;
     const int64_t row0 = ((int64_t)kv * c.m + t) * c.g;
+    // four blocks by eight heads of loads in flight per thread, the first of them while the maxima are formed
+    const double* u = c.u + row0 * nb_cap + i0;
+    double v[4][8];
+    auto load = [&](int i, int h0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int h = 0; h < 8; ++h)
+                v[k][h] = i + k * SEL_THREADS < n && h0 + h < c.g ? u[(h0 + h) * (int64_t)nb_cap + i + k * SEL_THREADS] : 0.0;
+    };
+    load(tid, 0);
     const int tops = (n_cand + SC_TOP - 1) / SC_TOP, top_cap = (nb_cap + SC_TOP - 1) / SC_TOP;
     for (int h = warp; h < c.g; h += SEL_WARPS) {
         const double* p = c.u_top + (row0 + h) * top_cap;
         double mx = -INFINITY;
         for (int i = lane; i < tops; i += 8 * 32) {
-            double v[8];
+            double w[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = i + 32 * k < tops ? p[i + 32 * k] : -INFINITY;
+            for (int k = 0; k < 8; ++k) w[k] = i + 32 * k < tops ? p[i + 32 * k] : -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) mx = fmax(mx, v[k]);
+            for (int k = 0; k < 8; ++k) mx = fmax(mx, w[k]);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         if (lane == 0) s_top[h] = mx;
     }
-    __syncthreads();
-    // four blocks by eight heads of loads in flight per thread
-    const double* u = c.u + row0 * nb_cap + i0;
+    unsigned long long* keys = s_keys;
+    if constexpr (GATHER) {
+        cg::this_cluster().sync();                     // the first CTA runs, its memory can be written
+        keys = cg::this_cluster().map_shared_rank(s_keys, 0) + i0;
+    } else {
+        __syncthreads();
+    }
     for (int i = tid; i < n; i += 4 * SEL_THREADS) {
         double best[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) best[k] = -INFINITY;
         for (int h0 = 0; h0 < c.g; h0 += 8) {
-            double v[4][8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int h = 0; h < 8; ++h)
-                    v[k][h] = i + k * SEL_THREADS < n && h0 + h < c.g ? u[(h0 + h) * (int64_t)nb_cap + i + k * SEL_THREADS] : 0.0;
+            if (i != tid || h0) load(i, h0);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -679,19 +693,27 @@ __global__ void __launch_bounds__(SEL_THREADS) k_block_choose(const CacheSelect 
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (i + k * SEL_THREADS < n) s_keys[i + k * SEL_THREADS] = score_key(best[k]);
+            if (i + k * SEL_THREADS < n) keys[i + k * SEL_THREADS] = score_key(best[k]);
     }
-    __syncthreads();
+    constexpr int SEL = GATHER ? 1 : CLN;              // CTAs that choose
+    if constexpr (GATHER) {
+        cg::this_cluster().sync();
+        if (rank) return;
+        i0 = 0;
+        n = n_cand;
+    } else {
+        __syncthreads();
+    }
     auto key = [&](int i) { return s_keys[i]; };
-    const Threshold th = select_threshold<CLN, 63>(ss, key, n, n_take);
-    ranked<CLN>(
+    const Threshold th = select_threshold<SEL, 63>(ss, key, n, n_take);
+    ranked<SEL>(
         ss, [&](int i) { return th.in(s_keys[i], i); }, n, [](unsigned) {},
         [&](int i, unsigned r) {
             const int b = cd.first + i0 + i;
             list[cd.first + r] = b;
             if (sel) sel[r] = b;
         });
-    if constexpr (CLN > 1) cg::this_cluster().sync();  // no CTA leaves while its counts may be read
+    if constexpr (SEL > 1) cg::this_cluster().sync();  // no CTA leaves while its counts may be read
 }
 
 // ---- the accepted path of a tree: thread = a 16-byte column of the K or V rows of a KV head. Rows ascend and
@@ -770,17 +792,23 @@ cudaError_t launch_cache_select(const CacheSelect& asked, cudaStream_t s) {
         e = launch_pdl(fn, grid, SC_THREADS, score_smem(c.hd, nb), s, c, nb_cap);
         if (e != cudaSuccess) return e;
     }
-    if (n_cand <= BS_SINGLE) {
+    if (n_cand <= BS_ONE && (n_cand <= BS_ALONE || c.n_kv * c.m * CL > KV_SMS)) {
         static SmemLimit limit;
-        e = limit.raise((const void*)k_block_choose<1>, BS_SINGLE * 8);
+        e = limit.raise((const void*)k_block_choose<1, false>, BS_ONE * 8);
         if (e != cudaSuccess) return e;
-        return launch_pdl(k_block_choose<1>, dim3(1, c.n_kv, c.m), SEL_THREADS, (size_t)n_cand * 8, s, c, nb_cap);
+        return launch_pdl(k_block_choose<1, false>, dim3(1, c.n_kv, c.m), SEL_THREADS, (size_t)n_cand * 8, s, c, nb_cap);
+    }
+    const dim3 grid(CL, c.n_kv, c.m);
+    if (n_cand <= BS_ONE) {
+        static SmemLimit limit;
+        e = limit.raise((const void*)k_block_choose<CL, true>, BS_ONE * 8);
+        if (e != cudaSuccess) return e;
+        return launch_pdl_cluster(k_block_choose<CL, true>, CL, grid, SEL_THREADS, (size_t)n_cand * 8, s, c, nb_cap);
     }
     static SmemLimit limit;
-    e = limit.raise((const void*)k_block_choose<CL>, 128 * 1024);
+    e = limit.raise((const void*)k_block_choose<CL, false>, 128 * 1024);
     if (e != cudaSuccess) return e;
-    return launch_pdl_cluster(k_block_choose<CL>, CL, dim3(CL, c.n_kv, c.m), SEL_THREADS, (size_t)((n_cand + CL - 1) / CL) * 8, s,
-                          c, nb_cap);
+    return launch_pdl_cluster(k_block_choose<CL, false>, CL, grid, SEL_THREADS, (size_t)((n_cand + CL - 1) / CL) * 8, s, c, nb_cap);
 }
 
 cudaError_t launch_cache_take(void* kc, void* vc, int64_t rs, int64_t hs, int n_kv, int hd, int row0,
