@@ -6,7 +6,7 @@ names and take torch CUDA tensors. Caches are [max_rows][n_head_kv][head_dim] te
 head strides that are multiples of 8 elements (a [n_head_kv][max_rows][head_dim] buffer passes as its transpose).
 Wrong tensors raise ValueError, refused arguments HoardError; nothing is launched then. One CacheOps is driven by one
 host thread at a time, and its calls share one workspace: calls on streams that may overlap, captured graphs among
-them, need a CacheOps each.
+them, need a CacheOps each. A result that a call allocates belongs to the stream of the call; `out` may be `q` itself.
 """
 from __future__ import annotations
 
@@ -71,6 +71,14 @@ def tree_visibility(parents):
     return [w - (1 << 64) if w >> 63 else w for w in words], depths
 
 
+def _ints(*values):
+    """The values, if C's int holds them (ctypes would cut them off)."""
+    for v in values:
+        if not -2**31 <= v < 2**31:
+            raise ValueError(f"{v} is not an int of 32 bits")
+    return values
+
+
 class CacheOps:
     """The cache operators for one head layout and cache shape on one device.
 
@@ -90,15 +98,15 @@ class CacheOps:
         self._d = Desc(n_head, n_head_kv, head_dim, KV_TYPES[kv_dtype], max_rows, max_tokens, max_acc_tokens, block, 0, 0,
                        1.0 / math.sqrt(head_dim) if scale is None else scale)
         self._q = ctypes.create_string_buffer(_QUERY.size)
-        self._dp, self._qp = ctypes.addressof(self._d), ctypes.addressof(self._q)
+        # pointers that stay, as ctypes takes them fastest
+        self._dp, self._qp = (ctypes.c_void_p(ctypes.addressof(x)) for x in (self._d, self._q))
         self._cache_shape, self._cache_stride = (max_rows, n_head_kv, head_dim), None
-        self._head_shape = (n_head, head_dim)
         n = _kv().hoard_kv_ws_bytes(self._dp)
         if n < 0:
             raise HoardError(-1, "hoard_kv_ws_bytes: descriptor refused")
         self.device = torch.cuda.current_device() if device is None else device
         self._ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", self.device))
-        self._wsp = self._ws.data_ptr()
+        self._wsp = ctypes.c_void_p(self._ws.data_ptr())
 
     # ---- plumbing ----
     # The checks read each attribute of a tensor once: at the sizes of a decode step they are a good part of a call.
@@ -107,13 +115,18 @@ class CacheOps:
         if _current_device() != self.device:
             with torch.cuda.device(self.device):
                 return self._run(fn, stream, *args)
-        if stream is None:
-            stream = _raw_stream(self.device)
-        elif hasattr(stream, "cuda_stream"):
-            stream = stream.cuda_stream
-        rc = fn(*args, stream)
+        rc = fn(*args, _raw_stream(self.device) if stream is None else getattr(stream, "cuda_stream", stream))
         if rc != 0:
             raise HoardError(rc, f"{fn.__name__} failed ({lib().hoard_strerror(rc).decode()})")
+
+    def _new(self, shape, stream):
+        """A float32 tensor of the call's stream."""
+        if stream is None:
+            return torch.empty(shape, dtype=_F32, device=self._ws.device)
+        if not hasattr(stream, "cuda_stream"):
+            stream = torch.cuda.ExternalStream(stream, device=self._ws.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=_F32, device=self._ws.device)
 
     def _caches(self, k_cache, v_cache=None):
         """Checks the caches and sets the descriptor's strides to theirs."""
@@ -126,6 +139,8 @@ class CacheOps:
                                     or v_cache.get_device() != dev or v_cache.stride() != s):
             raise ValueError("the V cache has the K cache's shape, type, device and strides")
         if s != self._cache_stride:
+            if not s[0] or not s[1]:               # expanded: its rows or heads are the same memory
+                raise ValueError("caches have a row and a head of memory for each of theirs")
             self._d.row_stride, self._d.head_stride = s[0], s[1]
             self._cache_stride = s
 
@@ -141,9 +156,10 @@ class CacheOps:
             raise ValueError(f"{what} is a contiguous {list(shape)} {dtype} tensor on device {self.device}")
         return x.data_ptr()
 
-    def _query(self, q, k_cache, v_cache, n_past, vis, gate, out, n_past_dev):
+    def _query(self, q, k_cache, v_cache, n_past, vis, gate, out, n_past_dev, stream):
         dev, shape, qs, ks = self.device, q.shape, q.stride(), k_cache.stride()
-        if (shape[1:] != self._head_shape or q.dtype is not _F32 or q.get_device() != dev or qs[2] != 1):
+        if (len(qs) != 3 or shape[1] != self.n_head or shape[2] != self.head_dim or q.dtype is not _F32
+                or q.get_device() != dev or qs[2] != 1):
             raise ValueError(f"q is a [m, {self.n_head}, {self.head_dim}] float32 tensor on device {dev} with contiguous heads")
         if ks != self._cache_stride or k_cache.shape != self._cache_shape or k_cache.dtype is not self.kv_dtype or \
                 k_cache.get_device() != dev or v_cache.stride() != ks or v_cache.shape != self._cache_shape or \
@@ -156,13 +172,16 @@ class CacheOps:
             gs = self._heads(gate, shape, "gate")
             gp = gate.data_ptr()
         if out is None:
-            out = torch.empty(shape, dtype=_F32, device=q.device)
+            out = self._new(shape, stream)
         elif out.shape != shape or out.dtype is not _F32 or out.get_device() != dev or not out.is_contiguous():
             raise ValueError(f"out is a contiguous {list(shape)} float32 tensor on device {dev}")
-        _QUERY.pack_into(self._q, 0, q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(),
-                         0 if vis is None else self._contiguous(vis, (m,), torch.int64, "vis"), gp, gs[0], gs[1],
-                         out.data_ptr(), m, n_past,
-                         0 if n_past_dev is None else self._contiguous(n_past_dev, (1,), torch.int32, "n_past_dev"))
+        try:
+            _QUERY.pack_into(self._q, 0, q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(),
+                             0 if vis is None else self._contiguous(vis, (m,), torch.int64, "vis"), gp, gs[0], gs[1],
+                             out.data_ptr(), m, n_past,
+                             0 if n_past_dev is None else self._contiguous(n_past_dev, (1,), torch.int32, "n_past_dev"))
+        except struct.error:
+            raise ValueError(f"n_past {n_past} is not an int of 32 bits") from None
         return out
 
     # ---- attention ----
@@ -172,7 +191,7 @@ class CacheOps:
         vis (int64 [m], see tree_visibility): which own rows a token sees; None: those of tokens up to itself. gate: the
         output times sigmoid(gate). acc (float32 [n_head_kv][max_rows]) gets the weights added. n_past_dev (int32 [1]):
         n_past in device memory. Returns out [m][n_head][head_dim]."""
-        out = self._query(q, k_cache, v_cache, n_past, vis, gate, out, n_past_dev)
+        out = self._query(q, k_cache, v_cache, n_past, vis, gate, out, n_past_dev, stream)
         accp = None if acc is None else self._contiguous(acc, (self.n_head_kv, self.max_rows), torch.float32, "acc")
         self._run(_kv().hoard_kv_attention, stream, self._dp, self._qp, accp, self._wsp)
         return out
@@ -182,6 +201,7 @@ class CacheOps:
         bounds [n_head_kv][max_rows // block][2][head_dim]; row1_dev (int32 [1]): those of row *row1_dev alone."""
         self._caches(k_cache)
         p = self._bounds(bounds)
+        row0, row1 = _ints(row0, row1)
         d = None if row1_dev is None else self._contiguous(row1_dev, (1,), torch.int32, "row1_dev")
         self._run(_kv().hoard_kv_block_bounds, stream, self._dp, k_cache.data_ptr(), p, row0, row1, d)
         return bounds
@@ -198,7 +218,8 @@ class CacheOps:
         n_sel others with the largest score, chosen for each token and KV head. sel_out (int32 [m][n_head_kv][n_sel]),
         if given, receives the chosen blocks, ascending, then -1."""
         bp = self._bounds(bounds)
-        out = self._query(q, k_cache, v_cache, n_past, vis, gate, out, n_past_dev)
+        out = self._query(q, k_cache, v_cache, n_past, vis, gate, out, n_past_dev, stream)
+        n_sink, n_local, n_sel = _ints(n_sink, n_local, n_sel)
         sp = None if sel_out is None else self._contiguous(sel_out, (q.shape[0], self.n_head_kv, n_sel), torch.int32,
                                                            "sel_out")
         self._run(_kv().hoard_kv_block_attention, stream, self._dp, self._qp, bp, n_sink, n_local, n_sel, sp, self._wsp)
@@ -211,6 +232,7 @@ class CacheOps:
         n_sink or from recent_from on, then those of the largest acc. acc, row_pos: [n_head_kv][max_rows]; updated in
         place, or written to acc_out / pos_out."""
         self._caches(k_cache, v_cache)
+        n_rows, n_keep, n_sink, recent_from = _ints(n_rows, n_keep, n_sink, recent_from)
         shape = (self.n_head_kv, self.max_rows)
         ap = self._contiguous(acc, shape, torch.float32, "acc")
         pp = self._contiguous(row_pos, shape, torch.int32, "row_pos")
@@ -223,6 +245,7 @@ class CacheOps:
         """hoard_kv_take: rows row0 + path[i] to rows row0 + i (path ascending): the accepted path of a drafted tree."""
         self._caches(k_cache, v_cache)
         n = len(path)
+        row0, *path = _ints(row0, *path)
         self._run(_kv().hoard_kv_take, stream, self._dp, k_cache.data_ptr(), v_cache.data_ptr(), row0,
                   (ctypes.c_int32 * max(1, n))(*path), n)
 
@@ -231,13 +254,13 @@ class CacheOps:
               row_pos=None, stream=None):
         """hoard_kv_store: QK norm and RoPE of m tokens' q [m][n_head][head_dim] and k, at positions pos (int32 [m]), and
         their k, v [m][n_head_kv][head_dim] into cache rows row0.. (row0_dev: in device memory). Returns the rotated q."""
-        m = q.shape[0]
+        m, row0, mode = _ints(q.shape[0], row0, mode)
         shape, kshape = (m, self.n_head, self.head_dim), (m, self.n_head_kv, self.head_dim)
         qs = self._heads(q, shape, "q")
         self._caches(k_cache, v_cache)
         kp, vp = (self._contiguous(x, kshape, torch.float32, w) for x, w in ((k, "k"), (v, "v")))
         if q_out is None:
-            q_out = torch.empty(shape, dtype=torch.float32, device=q.device)
+            q_out = self._new(shape, stream)
         qo = self._contiguous(q_out, shape, torch.float32, "q_out")
         if mode in (1, 2):
             full = mode == 1

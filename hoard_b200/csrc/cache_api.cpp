@@ -38,7 +38,9 @@ bool desc_ok(const hoard_kv_desc* d) {
         return false;
     if (d->block != 0 && d->block != 16 && d->block != 32 && d->block != 64 && d->block != 128) return false;
     if (d->block && d->max_rows / d->block > 131072) return false;
-    if (!(d->scale > 0) || !std::isfinite(d->scale)) return false;
+    // the block form's problems, (token, KV head), are the third dimension of its grid
+    if (d->block && (int64_t)d->max_tokens * d->n_head_kv > 65535) return false;
+    if (!(d->scale > 0) || !std::isfinite(d->scale * LOG2E)) return false;
     // either [row][head][dim]-like (heads inside a row) or [head][row][dim]-like, elements of a head contiguous
     if (d->row_stride == 0 && d->head_stride == 0) return true;
     if (d->row_stride < d->head_dim || d->head_stride < d->head_dim || d->row_stride % 8 || d->head_stride % 8)
@@ -90,11 +92,17 @@ Ws ws_plan(const hoard_kv_desc* d) {
     return w;
 }
 
+// Heads of hd floats, one token's after another's or one head's tokens after another's, none over the next
+bool heads_ok(int64_t ts, int64_t hs, int m, int n_head, int hd) {
+    if (hs < hd || ts < 0) return false;
+    return m == 1 || ts >= hs * (n_head - 1) + hd || (ts >= hd && hs >= ts * (m - 1) + hd);
+}
+
 bool query_ok(const hoard_kv_desc* d, const hoard_kv_query* a) {
     if (!a || !a->q || !a->k_cache || !a->v_cache || !a->out || !aligned16(a->k_cache) || !aligned16(a->v_cache))
         return false;
-    if (a->m < 1 || a->m > d->max_tokens || a->q_head_stride < d->head_dim || a->q_token_stride < 0) return false;
-    if (a->m > 1 && a->q_token_stride < a->q_head_stride * (d->n_head - 1) + d->head_dim) return false;
+    if (a->m < 1 || a->m > d->max_tokens || !heads_ok(a->q_token_stride, a->q_head_stride, a->m, d->n_head, d->head_dim))
+        return false;
     if (a->gate && (a->gate_head_stride < d->head_dim || a->gate_token_stride < 0)) return false;
     if (!a->n_past_dev && (a->n_past < 0 || a->n_past > d->max_rows - a->m)) return false;
     return true;
@@ -273,9 +281,9 @@ int hoard_kv_store(const hoard_kv_desc* d, const float* q, int64_t q_token_strid
                    float* q_out, void* k_cache, void* v_cache, float* acc, int32_t* row_pos, hoard_stream stream) {
     if (!desc_ok(d) || !q || !k || !v || !pos || !q_out || q_out == q || !k_cache || !v_cache || m < 1 ||
         m > HOARD_KV_MAX_TOKENS || mode < 0 || mode > 2 || (mode && (!q_norm || !k_norm)) || rope_dim < 2 ||
-        rope_dim > d->head_dim || rope_dim % 2 || !(freq_base > 0) || q_head_stride < d->head_dim ||
-        (mode == 1 && q_head_stride != d->head_dim) || q_token_stride < 0 ||
-        (m > 1 && q_token_stride < q_head_stride * (d->n_head - 1) + d->head_dim) || (!row0_dev && row0 < 0))
+        rope_dim > d->head_dim || rope_dim % 2 || !(freq_base > 0) ||
+        !heads_ok(q_token_stride, q_head_stride, m, d->n_head, d->head_dim) ||
+        (mode == 1 && q_head_stride != d->head_dim) || (!row0_dev && row0 < 0))
         return HOARD_EINVAL;
     return st(launch_qknorm_rope_store_rows(q, q_token_stride, q_head_stride, k, v, q_norm, k_norm, mode, eps, d->n_head,
                                             d->n_head_kv, d->head_dim, rope_dim, pos, m, row0, row0_dev, d->max_rows,

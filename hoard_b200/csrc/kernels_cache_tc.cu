@@ -320,15 +320,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
         constexpr int HALF = HD / 2;
         float4 xq[HALF / 4];
         {
-            float am = 0.f, all = 0.f;
+            float am = 0.f, odd = 0.f;                 // NaN where the row has an infinity or NaN
 #pragma unroll
             for (int i = 0; i < HALF / 4; ++i) {
                 const float4 x = xq[i] = *reinterpret_cast<const float4*>(sq + row * QP + grp * HALF + 4 * i);
                 am = fmaxf(am, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-                all += (fabsf(x.x) + fabsf(x.y)) + (fabsf(x.z) + fabsf(x.w));
+                odd = fmaf(x.x, 0.f, fmaf(x.y, 0.f, fmaf(x.z, 0.f, fmaf(x.w, 0.f, odd))));
             }
-            // rows with infinities or NaN, or so large that their sum is, are left as they are
-            s_mx[grp][row] = all <= 3.4e38f ? am : INFINITY;
+            s_mx[grp][row] = odd == 0.f ? am : INFINITY;
         }
         named_sync(2, 2 * GROUP);
         const float am = fmaxf(s_mx[0][row], s_mx[1][row]);

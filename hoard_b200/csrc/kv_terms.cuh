@@ -47,14 +47,14 @@ template <typename KT> __device__ __forceinline__ bool odd_pair(uint32_t w) {
     return (e & 0xFFFFu) == (Terms<KT>::INF2 & 0xFFFFu) || (e >> 16) == (Terms<KT>::INF2 >> 16);
 }
 
-// The power of two that brings a row with largest magnitude am (2^e <= am < 2^(e + 1)) to exponent Q_EXP, and its
-// inverse. Rows of zeros, and rows with infinities or NaN (bad), are left as they are.
+// The power of two that brings a row with largest magnitude am (2^e <= am < 2^(e + 1)) to exponent Q_EXP (e kept where
+// the powers are normal numbers), and its inverse. Rows of zeros, and rows with infinities or NaN (bad), are left as they are.
 struct RowScale {
     float up, down;
 };
 template <typename KT> __device__ __forceinline__ RowScale row_scale(float am, bool bad) {
     int e = (int)(__float_as_uint(am) >> 23) - 127;
-    e = bad || am == 0.f ? Terms<KT>::Q_EXP : max(e, -100);
+    e = bad || am == 0.f ? Terms<KT>::Q_EXP : min(max(e, -100), 126);
     return {__uint_as_float((uint32_t)(127 + Terms<KT>::Q_EXP - e) << 23),
             __uint_as_float((uint32_t)(127 - Terms<KT>::Q_EXP + e) << 23)};
 }

@@ -712,6 +712,9 @@ class DecodeModel:
         base + its depth, its k and v cache row base + i; it attends to the past, its ancestors and itself. The layers'
         attention is one call for all tokens, and so are the MoE layers (T = m). Returns the logits [m][vocab]; row i
         predicts what follows token i. With parents = [-1, 0, 1, ..] it is forward_batch."""
+        if stream is not None:                   # the tensors made here belong to the stream that uses them
+            with torch.cuda.stream(torch.cuda.ExternalStream(_stream(stream), device=self.dev)):
+                return self.forward_tree(tokens, parents, base)
         c, hx, s = self.cfg, _hx(), _stream(stream)
         m, H, hd = len(tokens), c.n_embd, c.head_dim
         words, depth = cache.tree_visibility(parents)

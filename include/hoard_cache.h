@@ -35,7 +35,8 @@ typedef struct hoard_kv_desc {
     int max_rows;           /* rows of the caches */
     int max_tokens;         /* most query tokens of a call, 1 .. HOARD_KV_MAX_TOKENS (sizes the workspace) */
     int max_acc_tokens;     /* most query tokens of a call that accumulates weights, 0 .. max_tokens */
-    int block;              /* rows of a block for the block operators: 16, 32, 64 or 128; 0: not used */
+    int block;              /* rows of a block for the block operators: 16, 32, 64 or 128 (max_rows / block at most
+                               131072, n_head_kv * max_tokens 65535); 0: not used */
     int64_t row_stride, head_stride; /* in elements, multiples of 8; both 0: [row][n_head_kv][head_dim] */
     float scale;            /* of the scores, finite and > 0 */
 } hoard_kv_desc;
@@ -46,13 +47,13 @@ int64_t hoard_kv_ws_bytes(const hoard_kv_desc* d);
 /* The query side of an attention call. */
 typedef struct hoard_kv_query {
     const float* q;              /* head h of token t at q + t * q_token_stride + h * q_head_stride */
-    int64_t q_token_stride, q_head_stride;       /* in floats; head_stride >= head_dim */
+    int64_t q_token_stride, q_head_stride;       /* in floats; token after token or head after head, none overlapping */
     const void* k_cache;         /* 16-byte aligned */
     const void* v_cache;
     const uint64_t* visible;     /* [m]: bit i of word t: token t sees token i's row. NULL: rows of tokens <= t */
     const float* gate;           /* optional: head h of token t's output times sigmoid(gate[...]) */
     int64_t gate_token_stride, gate_head_stride;
-    float* out;                  /* [m][n_head][head_dim] */
+    float* out;                  /* [m][n_head][head_dim]; may be q where q has this layout */
     int m, n_past;
     const int32_t* n_past_dev;   /* optional, overrides n_past */
 } hoard_kv_query;
@@ -87,7 +88,7 @@ int hoard_kv_block_bounds(const hoard_kv_desc* d, const void* k_cache, void* bou
  * max over the KV head's query heads of U_h(b) - max_b' U_h(b'), U_h(b) = sum_d max(q_d kmin_d, q_d kmax_d), an
  * upper bound of q . k over the block's keys; formed and compared in 64 bits, the NaN of a NaN in q ranking
  * lowest and infinite keys counting as one step above the largest finite value.
- * bounds have to be those of the complete blocks of [0, n_past). sel_out (optional, [m][n_head_kv][n_sel]):
+ * What keys of NaN count as is not defined. bounds have to be those of the complete blocks of [0, n_past). sel_out (optional, [m][n_head_kv][n_sel]):
  * the chosen blocks in ascending order, then -1. */
 int hoard_kv_block_attention(const hoard_kv_desc* d, const hoard_kv_query* a, const void* bounds, int n_sink,
                              int n_local, int n_sel, int32_t* sel_out, void* ws, hoard_stream stream);

@@ -43,7 +43,8 @@ def test_header_symbols_exported():
                                  dict(max_acc_tokens=5), dict(max_acc_tokens=-1), dict(block=8), dict(block=48),
                                  dict(row_stride=100, head_stride=128), dict(row_stride=256, head_stride=64),
                                  dict(row_stride=250, head_stride=128), dict(row_stride=128, head_stride=128),
-                                 dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan"))])
+                                 dict(n_head=4096, n_head_kv=1024, max_tokens=64, max_acc_tokens=0),
+                                 dict(scale=3e38), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan"))])
 def test_descriptor_refused(bad):
     d = desc(**bad)
     assert cache._kv().hoard_kv_ws_bytes(ref(d)) == -1
@@ -55,7 +56,7 @@ def test_descriptor_accepted():
     L = cache._kv()
     assert L.hoard_kv_ws_bytes(None) == -1
     for ok in (dict(), dict(row_stride=512, head_stride=128), dict(row_stride=128, head_stride=12800), dict(block=0), dict(head_dim=8),
-               dict(max_tokens=64, max_acc_tokens=0)):
+               dict(max_tokens=64, max_acc_tokens=0), dict(n_head=4096, n_head_kv=1024, max_tokens=63, max_acc_tokens=0)):
         assert L.hoard_kv_ws_bytes(ref(desc(**ok))) > 0
     # a workspace for more tokens is not smaller
     sizes = [L.hoard_kv_ws_bytes(ref(desc(max_tokens=t, max_acc_tokens=0))) for t in (1, 4, 16, 64)]
@@ -64,7 +65,7 @@ def test_descriptor_accepted():
 
 @pytest.mark.parametrize("bad", [dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(k=4104), dict(v=4100), dict(m=0), dict(m=5),
                                  dict(n_past=-1), dict(n_past=100), dict(m=2, n_past=99), dict(qh=64), dict(qt=-1),
-                                 dict(m=2, qt=512), dict(gate=4096, gh=64), dict(gate=4096, gh=128, gt=-1)])
+                                 dict(m=2, qt=512), dict(m=2, qt=128, qh=255), dict(m=2, qt=64, qh=4096), dict(gate=4096, gh=64), dict(gate=4096, gh=128, gt=-1)])
 def test_query_refused(bad):
     d, q = desc(), query(**bad)
     L = cache._kv()

@@ -135,6 +135,35 @@ def test_extreme_magnitudes(scale_q, scale_k):
     assert rel(ops.tree_attention(q, k, v, 198), ref.attention(q, k, v, 198)[0]) < TOL
 
 
+@pytest.mark.parametrize("m,n_past", [(2, 198), (20, 900)])
+def test_queries_near_the_largest_float(m, n_past):
+    """1.5 * 2^127 beside 2^120, over keys that bring the scores back to ordinary size."""
+    q, k, v, r = case(8, 2, 64, BF16, n_past + m, m)
+    q, k = q * 2.0**120, (k.float() * 2.0**-120).to(BF16)
+    q[:, :, 0] = 1.5 * 2.0**127 * torch.sign(q[:, :, 0])
+    k[:, :, 0] = (r(n_past + m, 2) * 2.0**-124).to(BF16)
+    ops = cache.CacheOps(n_head=8, n_head_kv=2, head_dim=64, kv_dtype=BF16, max_rows=n_past + m, max_tokens=m)
+    assert rel(ops.tree_attention(q, k, v, n_past), ref.attention(q, k, v, n_past)[0]) < TOL
+
+
+@pytest.mark.parametrize("m,n_past", [(3, 40), (3, 3000), (20, 900)])
+def test_head_major_queries_and_output_in_place(m, n_past):
+    """q as [n_head][m][head_dim]'s transpose; out the same tensor as q: results to the bit."""
+    q, k, v, r = case(8, 2, 128, F16, n_past + m, m)
+    gate = r(8, m, 128).transpose(0, 1)
+    ops = cache.CacheOps(n_head=8, n_head_kv=2, head_dim=128, kv_dtype=F16, max_rows=n_past + m, max_tokens=m, block=16)
+    bounds = torch.zeros(2, (n_past + m) // 16, 2, 128, dtype=F16, device=DEV)
+    ops.block_bounds(k, bounds, 0, n_past)
+    major = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert major.stride()[1] == m * 128
+    for call in (lambda q, **kw: ops.tree_attention(q, k, v, n_past, gate=gate, **kw),
+                 lambda q, **kw: ops.block_attention(q, k, v, bounds, n_past, n_sink=1, n_local=1, n_sel=2, **kw)):
+        want = call(q)
+        assert torch.equal(call(major), want)
+        x = q.clone()
+        assert call(x, out=x) is x and torch.equal(x, want)
+
+
 @pytest.mark.parametrize("m,n_past", [(1, 77), (20, 900)])
 def test_strides_gate_and_layouts(m, n_past):
     """q and gate inside wider rows, a cache laid out [head][row][dim], an output that is given."""
@@ -373,8 +402,10 @@ def test_other_stream():
     s.wait_stream(torch.cuda.current_stream())
     out = torch.empty_like(want)
     ops.tree_attention(q, k, v, 580, out=out, stream=s)
+    got = ops.tree_attention(q, k, v, 580, stream=s)                     # allocated on the stream of the call
+    raw = ops.tree_attention(q, k, v, 580, stream=s.cuda_stream)
     s.synchronize()
-    assert torch.equal(out, want)
+    assert torch.equal(out, want) and torch.equal(got, want) and torch.equal(raw, want)
 
 
 def test_long_cache_offsets_pass_32_bits():
@@ -437,3 +468,24 @@ def test_wrong_tensors_are_refused():
         ops.take(k, v, 60, [0, 5])
     with pytest.raises(HoardError):
         ops.evict(k, v, torch.zeros(2, 64, device=DEV), torch.zeros(2, 64, dtype=torch.int32, device=DEV), 10, 11)
+
+
+def test_expanded_caches_and_wide_integers_are_refused():
+    ops = cache.CacheOps(n_head=8, n_head_kv=2, head_dim=128, kv_dtype=F16, max_rows=64, block=16)
+    k = torch.zeros(64, 2, 128, dtype=F16, device=DEV)
+    q = torch.zeros(1, 8, 128, device=DEV)
+    acc, pos = torch.zeros(2, 64, device=DEV), torch.zeros(2, 64, dtype=torch.int32, device=DEV)
+    bounds = torch.zeros(2, 4, 2, 128, dtype=F16, device=DEV)
+    for flat in (k[:1, :1].expand(64, 2, 128), k[:, :1].expand(64, 2, 128), k[:1].expand(64, 2, 128)):
+        with pytest.raises(ValueError):
+            ops.tree_attention(q, flat, flat, 3)
+        with pytest.raises(ValueError):
+            ops.take(flat, flat, 0, [1])
+    big = 2**32 + 1
+    for call in (lambda: ops.tree_attention(q, k, k, big), lambda: ops.evict(k, k, acc, pos, big, 1),
+                 lambda: ops.evict(k, k, acc, pos, 5, 1, recent_from=2**31), lambda: ops.take(k, k, 0, [big]),
+                 lambda: ops.take(k, k, big, [1]), lambda: ops.block_bounds(k, bounds, 0, big),
+                 lambda: ops.block_attention(q, k, k, bounds, 40, n_sink=1, n_local=1, n_sel=big),
+                 lambda: ops.store(q, q[:, :2], q[:, :2], k, k, pos[0, :1], big)):
+        with pytest.raises(ValueError):
+            call()

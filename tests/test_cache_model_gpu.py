@@ -61,6 +61,11 @@ def test_forward_tree_matches_its_paths(cfg, kv, weights):
     tokens = prompt_of(cfg, 21, seed=9)
     parents = [-1, -1, 0, 0, 1, 2, 2, 5, 5, 7, 4, 10, 11, -1, 13, 14, 15, 16, 17, 18, 19]
     out = m.forward_tree(tokens, parents, len(prompt))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    again = m.forward_tree(tokens, parents, len(prompt), stream=side)
+    side.synchronize()
+    assert torch.equal(again, out)
     for leaf in (3, 6, 8, 9, 12, 20):
         path = []
         i = leaf
