@@ -163,9 +163,7 @@ int hoard_kv_attention(const hoard_kv_desc* d, const hoard_kv_query* a, float* a
         c.logits_ld = w.logits_ld;
     }
     const int64_t past = c.n_past_dev ? c.max_rows - c.m : c.n_past;
-    if (!acc) c.tc_splits = cache_tc_splits(c.hd, c.n_kv, c.R, past);
-    if (c.tc_splits) c.splits = c.tc_splits;
-    else cache_plan(c, chunks_of(c, past));
+    cache_plan(c, chunks_of(c, past), past);
     return st(launch_cache_attention(c, (cudaStream_t)stream));
 }
 
@@ -253,7 +251,7 @@ int hoard_kv_block_attention(const hoard_kv_desc* d, const hoard_kv_query* a, co
     c.block = d->block;
     int64_t blocks = (int64_t)s.n_sink + s.n_local + n_sel;
     if (blocks > nb_most) blocks = nb_most;
-    cache_plan(c, chunks_of(c, blocks * d->block));
+    cache_plan(c, chunks_of(c, blocks * d->block), blocks * d->block);
     return st(launch_cache_attention(c, (cudaStream_t)stream));
 }
 

@@ -18,6 +18,7 @@
 #include "async_copy.cuh"
 #include "kv_terms.cuh"
 
+#include <cmath>
 #include <cooperative_groups.h>
 
 namespace cg = cooperative_groups;
@@ -697,38 +698,67 @@ template <typename KT> cudaError_t attention_type(const CacheAttn& a, cudaStream
 
 int cache_tile_dims(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
-// Query rows of a tile and splits of the chunks, for P problems of R rows over n_chunks chunks.
-// Rows: 8 or 16. Tiles of 8 have the shorter code and epilogue (one call over 40 rows 4.1 us against 5.7), tiles of 16
-// read the cache half as often: with 16 rows of 4 heads of 128, 8 against 16 take 9.1 / 9.9 us over 4000 cache
-// rows, 14.5 / 14.2 over 16000, 35.5 / 30.1 over 60000; with 16 heads 9.2 / 9.8 over 1000, 15.5 / 14.0 over 4000.
-// The two cross where a warp of a full grid has about five chunks.
-// Splits: up to four are the CTAs of a cluster, which joins them itself (about 1 us where there is more than one);
-// more are joined by a second kernel (3 us). A chunk of a warp is 0.8 us. So: two chunks of a warp in one CTA; up to
-// three and a half in four; else one CTA per SM over problems and tiles, each warp with a chunk. (Clusters of eight
-// waited for SMs: 3460 rows of 4 heads 11.7 us, against 8.2 with 28 splits.)
-// Weights are accumulated by the cluster too, where one tile holds all query rows of a KV head.
-void cache_plan(CacheAttn& a, int n_chunks) {
-    const int64_t w = W, tiles8 = (a.R + 7) / 8;
-    a.tile_rows = a.R > 8 && a.problems * tiles8 * n_chunks > 5 * w * KV_SMS ? 16 : 8;
-    if (a.logits && a.R > 8 && a.R <= 16) a.tile_rows = 16;
-    a.row_tiles = (a.R + a.tile_rows - 1) / a.tile_rows;
-    const int64_t most = KV_SMS / ((int64_t)a.problems * a.row_tiles), useful = (n_chunks + w - 1) / w;
-    a.splits = (int)(most < useful ? most : useful);
-    if (a.splits < 1) a.splits = 1;
-    const int wide = most >= 4 ? 4 : most >= 2 ? 2 : 1;
-    int in_cluster = 1;                                // fewest CTAs (1, 2, 4) that leave a warp two chunks
-    while (in_cluster < wide && n_chunks > 2 * w * in_cluster) in_cluster *= 2;
-    a.cluster = (!a.logits || a.row_tiles == 1) && (a.splits <= in_cluster || 2 * n_chunks <= 7 * w * in_cluster);
-    if (a.cluster) a.splits = in_cluster;
-}
+// The plan of a call: query rows of a tile (8 or 16), splits of the chunks and who joins them, or the tensor-core form.
+// The choice is by time, from what the parts were measured to take in microseconds (f16; bf16 a tenth more):
+//
+//   - a CTA's start and end, and a chunk of each of its warps (a CTA has as many in turn as its fullest warp):
+//     tiles of 16 cost more of both and halve the reads of the cache where there are more than 8 rows
+//   - joining: nothing for one CTA; 1.2 for a cluster of 2 or 4, which joins in shared memory; a second kernel takes 2.5
+//     and, up to 128 query rows, 0.01 for each
+//   - the tensor-core form: its start, 1 / 256 for each query row (staged, split into terms, stored) and a tile of 64 cache
+//     rows. It takes 128 query rows at once, so that its time hardly depends on them
+//
+// Both sides, measured: 4 heads of 128 with 32 rows each over 250 cache rows: one CTA 7.4, cluster of 4 6.4, second kernel
+// 8.4; over 1000 with 8 rows: 10.5 for 2 CTAs, 8.0 for a cluster of 4, 7.4 for eight splits; heads of 256 over 1400: cluster
+// 13.3, sixteen splits 9.0. Tiles of 8 against 16: 4 heads of 128 with 64 rows 11.0 / 12.1 over 2000 cache rows, 47 / 34 over
+// 16000. Tensor cores against the best of these: 4 heads of 128 with 24 rows 13.2 / 11.5 over 4000 cache rows, 15.1 / 15.0
+// over 8000, 35.5 / 58.0 over 64000; with 512 rows 20.3 / 15.6 over 600, 31.8 / 115 over 8000; 16 heads with 33 rows 13.1 /
+// 11.7 over 600, 15.3 / 18.9 over 2000. Up to 16 rows a tile of 16 reads the cache once as well, and they are not asked for.
+struct TileCost {
+    float base, chunk;
+};
+constexpr TileCost TILE_COST[3][2] = {{{2.7f, 1.3f}, {4.3f, 1.15f}}, {{3.2f, 1.4f}, {4.4f, 1.8f}}, {{3.9f, 2.6f}, {5.5f, 3.9f}}};
+constexpr TileCost TC_COST[2] = {{8.6f, 0.7f}, {10.f, 1.f}};
+// CTAs up to which clusters of four all run at once (a CTA per SM, and SMs of a GPC left over)
+constexpr int CLUSTERED_CTAS = 128;
 
-// Splits for the tensor-core form: one CTA per SM over KV heads and tiles of 128 query rows, each with TC_MIN_TILES
-// tiles of 64 rows at least; 0: the other form runs the call.
-int cache_tc_splits(int hd, int n_kv, int R, int64_t past_rows) {
-    if (cache_tile_dims(hd) > 128 || R <= TC_MIN_R || past_rows < TC_MIN_PAST) return 0;
-    const int64_t tiles = (past_rows + 63) / 64 + 1, few = (tiles + TC_MIN_TILES - 1) / TC_MIN_TILES;
-    const int64_t most = KV_SMS / ((int64_t)n_kv * ((R + 127) / 128));
-    return (int)(most < 1 ? 1 : most < few ? most : few);
+inline int64_t up_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+void cache_plan(CacheAttn& a, int n_chunks, int64_t past_rows) {
+    const int dims = cache_tile_dims(a.hd), di = dims == 64 ? 0 : dims == 128 ? 1 : 2;
+    const int64_t rows = (int64_t)a.problems * a.R;
+    const float second = 2.5f + 0.01f * (rows < 128 ? rows : 128);
+    float best = INFINITY;
+    a.tc_splits = 0;
+    for (int rt = 8; rt <= (a.R > 8 ? 16 : 8); rt += 8) {
+        const TileCost& cost = TILE_COST[di][rt / 16];
+        const int64_t row_tiles = up_div(a.R, rt), ctas = a.problems * row_tiles, useful = up_div(n_chunks, W);
+        const int64_t fit = KV_SMS / ctas, most = useful < fit ? useful : fit;
+        auto offer = [&](int64_t splits, bool cluster, float join) {
+            const int64_t waves = up_div(ctas * splits, KV_SMS);
+            const float t = join + waves * (cost.base + cost.chunk * up_div(up_div(n_chunks, splits), W));
+            if (t >= best) return;
+            best = t;
+            a.tile_rows = rt;
+            a.row_tiles = (int)row_tiles;
+            a.splits = (int)splits;
+            a.cluster = cluster;
+        };
+        // the weights of a call that accumulates are added by the cluster if one tile has all rows of a KV head
+        const bool joins = !a.logits || row_tiles == 1;
+        offer(1, joins, joins ? 0.f : second);
+        if (joins && ctas * 2 <= CLUSTERED_CTAS) offer(2, true, 1.2f);
+        if (joins && ctas * 4 <= CLUSTERED_CTAS) offer(4, true, 1.2f);
+        if (most > 1) offer(most, false, second);
+    }
+    if (a.logits || a.list || a.R <= TC_MIN_R || di == 2) return;
+    // one CTA per SM over KV heads and tiles of 128 query rows, two tiles of cache rows each at least
+    const int64_t tiles = up_div(past_rows, 64) + 1, ctas = a.problems * up_div(a.R, 128);
+    int64_t splits = KV_SMS / ctas;
+    if (splits > up_div(tiles, 2)) splits = up_div(tiles, 2);
+    if (splits < 1) splits = 1;
+    const float t = TC_COST[di].base + rows * (1.f / 256) + TC_COST[di].chunk * up_div(tiles, splits) * up_div(ctas * splits, KV_SMS);
+    if (t < best) a.tc_splits = a.splits = (int)splits;
 }
 
 cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s) {

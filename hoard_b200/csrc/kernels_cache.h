@@ -9,8 +9,7 @@ namespace hoard {
 
 constexpr int KV_SMS = 148;              // B200: one split CTA per SM
 constexpr int KV_CHUNK = 16;             // rows of one step of a warp (the M of m16n8k16)
-// The tensor-core form runs where a KV head has more query rows and the past more rows than these.
-constexpr int TC_MIN_R = 32, TC_MIN_PAST = 512, TC_MIN_TILES = 2;
+constexpr int TC_MIN_R = 16;             // the tensor-core form runs where a KV head has more query rows than these
 
 // Dynamic shared memory above 48 KiB has to be allowed once for each kernel and device; asking again costs a
 // launch's time in every call.
@@ -81,8 +80,8 @@ struct CacheAttn {
 };
 
 int cache_tile_dims(int hd);             // dims of the instantiation that runs a head_dim
-void cache_plan(CacheAttn& a, int n_chunks);                             // sets tile_rows, row_tiles, splits, cluster
-int cache_tc_splits(int hd, int n_kv, int R, int64_t past_rows);
+// sets tile_rows, row_tiles, splits, cluster, tc_splits for n_chunks chunks (past_rows rows of the past among them) a problem
+void cache_plan(CacheAttn& a, int n_chunks, int64_t past_rows);
 cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s);
 cudaError_t launch_cache_attention_tc(const CacheAttn& a, cudaStream_t s);
 
