@@ -474,16 +474,21 @@ __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __r
     }
 }
 
-// ---- scores: u[kv][row][b - first] = sum_d max(q_d kmin_d, q_d kmax_d) = sum_d q_d (q_d > 0 ? kmax_d : kmin_d) ----
+// ---- scores: u[kv][row][b - first] = sum_d max(q_d kmin_d, q_d kmax_d) = sum_d q+_d kmax_d + q-_d kmin_d ----
 // In 64 bits, because the scores decide which rows are read: products of 24 and 11 (or 8) bits are exact, and
-// sums differ from the true ones in the 16th digit. A CTA takes NB x 32 blocks (NB per lane) and eight query rows; its
-// warps share out the dims, eight at a time, and their sums are added in warp order. u_top receives the rows' maxima
-// over the CTA's blocks.
-// Bound by instruction issue, so nothing but the multiply-add is done per product except a select: a bound's f64 is
-// made from its bits by shifting them under the exponent field (two or three integer instructions, where the
-// conversion instruction runs at a quarter of the multiply-add's rate), which is its value times 2^-1008 (f16) or
-// 2^-896 (bf16), subnormals included; q is scaled up to make up for all but 2^-128 of it, which cancels in nothing but
-// the comparison of scores. Infinite bounds thereby count as one step above the largest finite value.
+// sums differ from the true ones in the 16th digit. The positive and the negative part of q are two products by f64
+// matrix instructions (m8n8k4: eight query rows, four dims, eight blocks); a multiply-add with a select of the bound does
+// half the arithmetic, but spends the issue slots on selects and on reading q again for every product. A warp takes eight
+// query rows and eight blocks of a CTA's 32, 128 dims; more dims take four more warps, whose sums are added. The bounds come
+// from memory as a lane needs them, and which dim a step's k-th place holds is free as long as both operands
+// agree. u_top receives the rows' maxima over the 32 blocks.
+// Bound by the f64 pipe (64 multiply-adds a clock and SM, 5.7 us for 1557 blocks of 64 query rows and 4 KV heads of 128) and
+// by the bounds' way from L2, once for every eight query rows: 12.7 us there; with multiply-adds and selects 20.4. CTAs
+// that keep q for further blocks hold it as f64 in 64 registers, and their loads wait for one another: 16.5.
+// A bound's f64 is made from its bits by shifting them under the exponent field (two or three integer instructions), which
+// is its value times 2^-1008 (f16) or 2^-896 (bf16), subnormals included; q is scaled up to make up for all but
+// 2^-128 of it, which cancels in nothing but the comparison of scores. Infinite bounds thereby count as one step above the
+// largest finite value.
 struct Candidates {
     int n_past, nb, first, last;
 };
@@ -506,102 +511,95 @@ template <typename KT> __device__ __forceinline__ int2 high_words(uint32_t w) {
     return make_int2(((int)(w << 16) >> Shift<KT>::N) & Shift<KT>::MASK, ((int)w >> Shift<KT>::N) & Shift<KT>::MASK);
 }
 
-constexpr int SC_THREADS = 256, SC_ROWS = 8;
-constexpr int SC_TOP = 32;               // blocks of an entry of u_top
-constexpr int score_smem(int hd, int nb) {
-    return SC_ROWS * hd * 8 + SC_ROWS * hd * 4 + 8 * SC_ROWS * 32 * 8 + nb * 32 * (hd + 4) * 4;
+constexpr int SC_ROWS = 8, SC_TOP = 32;  // query rows and blocks of a CTA; an entry of u_top has as many blocks
+constexpr int SC_WARPS = SC_TOP / 8;     // warps of 128 dims
+__device__ __forceinline__ void mma884(double* c, double a, double b) {
+    asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};"
+                 : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
-template <typename KT, int NB>
-__global__ void __launch_bounds__(SC_THREADS) k_block_score(const CacheSelect c, int nb_cap) {
+template <typename KT, int PARTS>
+__global__ void __launch_bounds__(32 * SC_WARPS * PARTS, PARTS == 1 ? 5 : 2) k_block_score(const CacheSelect c, int nb_cap) {
     pdl_enter();
-    extern __shared__ __align__(16) uint8_t s_raw[];
+    __shared__ double s_top[SC_WARPS][SC_ROWS];
+    __shared__ double2 s_sum[PARTS == 1 ? 1 : SC_WARPS * 32];
     const Candidates cd = candidates(c);
-    const int n_cand = cd.last - cd.first, b0 = blockIdx.x * 32 * NB, kv = blockIdx.y, row0 = blockIdx.z * SC_ROWS;
+    const int n_cand = cd.last - cd.first, b0 = blockIdx.x * SC_TOP, kv = blockIdx.y, row0 = blockIdx.z * SC_ROWS;
     if (n_cand <= c.n_sel || b0 >= n_cand) return;     // every candidate is taken: no scores needed
-    const int R = c.m * c.g, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    double* sq = reinterpret_cast<double*>(s_raw);                              // [SC_ROWS][hd]
-    double* red = sq + SC_ROWS * c.hd;                                          // [8 warps][SC_ROWS][32]
-    int* sm = reinterpret_cast<int*>(red + 8 * SC_ROWS * 32);                   // [SC_ROWS][hd]: -1 where q > 0
-    // [32 NB][hd + 4] words: 16-byte reads of eight lanes fall in eight bank groups
-    uint32_t* sb = reinterpret_cast<uint32_t*>(sm + SC_ROWS * c.hd);
-    const int n = min(32 * NB, n_cand - b0), c4 = c.hd / 4, c8 = c.hd / 8;
-    const uint32_t* src = reinterpret_cast<const uint32_t*>(c.bounds) +
-                          ((int64_t)kv * nb_cap + cd.first + b0) * c.hd;      // hd words a block
-    for (int b = warp; b < n; b += 8)
-        for (int p = lane; p < c4; p += 32) cp_async16(sb + b * (c.hd + 4) + 4 * p, src + b * c.hd + 4 * p);
-    cp_async_commit();
-    {
-        const int row = row0 + warp;                   // a warp converts a query row
-        const int t = row / c.g;
-        const float* q = c.q + t * c.q_ts + (kv * c.g + row - t * c.g) * c.q_hs;
-        const double up = __hiloint2double((1023 + Shift<KT>::Q_EXP) << 20, 0);
-        float x[8];
+    const int R = c.m * c.g, tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) % SC_WARPS, part = tid / (32 * SC_WARPS);
+    // lane = (row of q, place k) and (block, place k) of the operands, (row, two blocks) of the sums
+    const int j = lane & 3, i8 = lane >> 2, row = row0 + i8, c8 = c.hd / 8, t = row / c.g;
+    const float* q = c.q + (row < R ? t * c.q_ts + (kv * c.g + row - t * c.g) * c.q_hs : 0);
+    const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+    const uint4* src = reinterpret_cast<const uint4*>(c.bounds) +
+                       ((int64_t)kv * nb_cap + cd.first + min(b0 + 8 * warp + i8, n_cand - 1)) * 2 * c8;
+    uint4 lo[4], hi[4];
+    float x[4][8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = row < R && k * 32 + lane < c.hd ? q[k * 32 + lane] : 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k * 32 + lane < c.hd) {
-                sq[warp * c.hd + k * 32 + lane] = (double)x[k] * up;
-                sm[warp * c.hd + k * 32 + lane] = x[k] > 0.f ? -1 : 0;
-            }
-    }
-    cp_async_wait_all();
-    __syncthreads();
-    double acc[NB][SC_ROWS];
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int r = 0; r < SC_ROWS; ++r) acc[i][r] = 0.0;
-    const uint32_t* mine[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) mine[i] = sb + min(32 * i + lane, n - 1) * (c.hd + 4);
-    for (int p = warp; p < c8; p += 8) {
-        uint32_t lw[NB][4], hw[NB][4];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const uint4 l4 = *reinterpret_cast<const uint4*>(mine[i] + 4 * p);
-            const uint4 h4 = *reinterpret_cast<const uint4*>(mine[i] + c.hd / 2 + 4 * p);
-            lw[i][0] = l4.x, lw[i][1] = l4.y, lw[i][2] = l4.z, lw[i][3] = l4.w;
-            hw[i][0] = h4.x, hw[i][1] = h4.y, hw[i][2] = h4.z, hw[i][3] = h4.w;
+    for (int i = 0; i < 4; ++i) {                      // this lane's pieces of eight dims: j, j + 4, .. of the warp's 128
+        const int p = part * 16 + 4 * i + j;
+        lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+        if (p < c8) {
+            lo[i] = src[p];
+            hi[i] = src[c8 + p];
         }
+        const bool there = row < R && p < c8;
+        if (wide) {
+            const float4 a = there ? *reinterpret_cast<const float4*>(q + 8 * p) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 b = there ? *reinterpret_cast<const float4*>(q + 8 * p + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[i][0] = a.x, x[i][1] = a.y, x[i][2] = a.z, x[i][3] = a.w;
+            x[i][4] = b.x, x[i][5] = b.y, x[i][6] = b.z, x[i][7] = b.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[i][k] = there ? q[8 * p + k] : 0.f;
+        }
+    }
+    const double up = __hiloint2double((1023 + Shift<KT>::Q_EXP) << 20, 0);
+    double pos[2] = {0.0, 0.0}, neg[2] = {0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lw[4] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w}, hw[4] = {hi[i].x, hi[i].y, hi[i].z, hi[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            int2 lo[NB], hi[NB];
+            const int2 l = high_words<KT>(lw[k]), h = high_words<KT>(hw[k]);
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                lo[i] = high_words<KT>(lw[i][k]);
-                hi[i] = high_words<KT>(hw[i][k]);
-            }
-#pragma unroll
-            for (int r = 0; r < SC_ROWS; ++r) {
-                const double2 q = *reinterpret_cast<const double2*>(sq + r * c.hd + 8 * p + 2 * k);
-                const int2 up = *reinterpret_cast<const int2*>(sm + r * c.hd + 8 * p + 2 * k);
-#pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    acc[i][r] = fma(q.x, __hiloint2double((hi[i].x & up.x) | (lo[i].x & ~up.x), 0), acc[i][r]);
-                    acc[i][r] = fma(q.y, __hiloint2double((hi[i].y & up.y) | (lo[i].y & ~up.y), 0), acc[i][r]);
-                }
+            for (int e = 0; e < 2; ++e) {
+                // the part of q of one sign: the high word of the other's becomes 0, and what the low word leaves is below
+                // 2^-1022, so that its products are 0
+                const double d = (double)x[i][2 * k + e] * up;
+                const int dh = __double2hiint(d), dl = __double2loint(d);
+                mma884(pos, __hiloint2double(max(dh, 0), dl), __hiloint2double(e ? h.y : h.x, 0));
+                mma884(neg, __hiloint2double(min(dh, 0), dl), __hiloint2double(e ? l.y : l.x, 0));
             }
         }
     }
-    const int row = row0 + warp;
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        if (i) __syncthreads();
-#pragma unroll
-        for (int r = 0; r < SC_ROWS; ++r) red[(warp * SC_ROWS + r) * 32 + lane] = acc[i][r];
+    double sum[2] = {pos[0] + neg[0], pos[1] + neg[1]}, top = -INFINITY;
+    if constexpr (PARTS > 1) {
+        if (part) s_sum[warp * 32 + lane] = make_double2(sum[0], sum[1]);
         __syncthreads();
-        double s = 0.0;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) s += red[(w * SC_ROWS + warp) * 32 + lane];     // thread = (row, block)
-        const int left = n - 32 * i;
-        if (row < R && left > 0) {
-            if (lane < left) c.u[((int64_t)kv * R + row) * nb_cap + b0 + 32 * i + lane] = s;
-            double top = lane < left ? s : -INFINITY;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (lane == 0) c.u_top[((int64_t)kv * R + row) * ((nb_cap + SC_TOP - 1) / SC_TOP) + blockIdx.x * NB + i] = top;
+        if (!part) {
+            sum[0] += s_sum[warp * 32 + lane].x;
+            sum[1] += s_sum[warp * 32 + lane].y;
         }
+    }
+    if (!part) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int b = b0 + 8 * warp + 2 * j + e;
+            if (row < R && b < n_cand) {
+                c.u[((int64_t)kv * R + row) * nb_cap + b] = sum[e];
+                top = fmax(top, sum[e]);
+            }
+        }
+        top = fmax(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmax(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (j == 0) s_top[warp][i8] = top;
+    }
+    __syncthreads();
+    if (tid < SC_ROWS && row0 + tid < R) {
+        top = s_top[0][tid];
+#pragma unroll
+        for (int w = 1; w < SC_WARPS; ++w) top = fmax(top, s_top[w][tid]);
+        c.u_top[((int64_t)kv * R + row0 + tid) * ((nb_cap + SC_TOP - 1) / SC_TOP) + blockIdx.x] = top;
     }
 }
 
@@ -780,16 +778,11 @@ cudaError_t launch_cache_select(const CacheSelect& asked, cudaStream_t s) {
     if (n_cand < 0) n_cand = 0;
     cudaError_t e;
     if (n_cand > c.n_sel && c.n_sel > 0) {
-        // one block per lane where that fits the GPU at once (two CTAs per SM), else two: half the reads of q per product
-        const int row_groups = (c.m * c.g + SC_ROWS - 1) / SC_ROWS, chunks = (n_cand + 31) / 32;
-        const int nb = chunks * c.n_kv * row_groups <= 2 * KV_SMS ? 1 : 2;
-        const dim3 grid((chunks + nb - 1) / nb, c.n_kv, row_groups);
-        auto fn = c.bf16 ? (nb == 1 ? k_block_score<__nv_bfloat16, 1> : k_block_score<__nv_bfloat16, 2>)
-                         : (nb == 1 ? k_block_score<__half, 1> : k_block_score<__half, 2>);
-        static SmemLimit limit[4];
-        e = limit[2 * c.bf16 + nb - 1].raise((const void*)fn, score_smem(256, nb));
-        if (e != cudaSuccess) return e;
-        e = launch_pdl(fn, grid, SC_THREADS, score_smem(c.hd, nb), s, c, nb_cap);
+        const int parts = c.hd <= 128 ? 1 : 2;
+        const dim3 grid((n_cand + SC_TOP - 1) / SC_TOP, c.n_kv, (c.m * c.g + SC_ROWS - 1) / SC_ROWS);
+        auto fn = c.bf16 ? (parts == 1 ? k_block_score<__nv_bfloat16, 1> : k_block_score<__nv_bfloat16, 2>)
+                         : (parts == 1 ? k_block_score<__half, 1> : k_block_score<__half, 2>);
+        e = launch_pdl(fn, grid, 32 * SC_WARPS * parts, 0, s, c, nb_cap);
         if (e != cudaSuccess) return e;
     }
     if (n_cand <= BS_ONE && (n_cand <= BS_ALONE || c.n_kv * c.m * CL > KV_SMS)) {
