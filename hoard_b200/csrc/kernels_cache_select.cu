@@ -30,6 +30,7 @@ struct Select {
     unsigned hist[2][BINS];
     unsigned warp[2][SEL_WARPS];         // one value per warp, alternately (a scan's values may still be read)
     unsigned seg[CL], found[3];          // cluster: segment totals; bin, count in it, count above it
+    uint2 bits[2][SEL_WARPS];            // OR and AND of the keys of the last bin, alternately
     unsigned ex[2];                      // this CTA's totals, for prefixes over the cluster
 };
 
@@ -178,49 +179,81 @@ __device__ __forceinline__ void find_bin(Select& s, const unsigned* hist, unsign
 
 // The `need` largest of the keys, the lower index where equal: afterwards this CTA's i-th key is in if
 // (key >> shift) > prefix, or == prefix and i <= cut. key(i): this CTA's i-th key.
-struct Threshold {
-    unsigned long long prefix;
+template <typename K> struct Threshold {
+    K prefix;
     int shift, cut;
-    __device__ __forceinline__ bool in(unsigned long long key, int i) const {
-        const unsigned long long k = key >> shift;
+    __device__ __forceinline__ bool in(K key, int i) const {
+        const K k = key >> shift;
         return k > prefix || (k == prefix && i <= cut);
     }
 };
-template <int CLN, int BITS, typename Key>
-__device__ __forceinline__ Threshold select_threshold(Select& s, Key key, int n_local, int need) {
+template <int CLN, int BITS, typename K, typename Key>
+__device__ __forceinline__ Threshold<K> select_threshold(Select& s, Key key, int n_local, int need) {
+    // weights are often equal (rows that nothing looked at): one CTA sees that in the second pass
+    constexpr bool SAME = CLN == 1 && BITS <= 32;
     const int tid = threadIdx.x;
     for (int i = tid; i < 2 * BINS; i += SEL_THREADS) s.hist[0][i] = 0;
     __syncthreads();
-    Threshold th{0, BITS, 0x7fffffff};
+    Threshold<K> th{0, BITS, 0x7fffffff};
     for (int pass = 0;; ++pass) {
         const int width = min(DIGIT, th.shift);
         th.shift -= width;
         unsigned* hist = s.hist[pass & 1];
+        unsigned any = 0, every = ~0u;                 // bits of the bin's keys
         for (int i = tid; i < n_local; i += SEL_THREADS) {
-            const unsigned long long k = key(i);
+            const K k = key(i);
             const unsigned d = (unsigned)(k >> th.shift) & ((1u << width) - 1);
-            if (pass == 0 || (k >> (th.shift + width)) == th.prefix) atomicAdd(&hist[d], 1u);
+            if (pass == 0 || (k >> (th.shift + width)) == th.prefix) {
+                atomicAdd(&hist[d], 1u);
+                any |= (unsigned)k;
+                every &= (unsigned)k;
+            }
+        }
+        if (SAME && pass) {
+            any = __reduce_or_sync(0xffffffffu, any);
+            every = __reduce_and_sync(0xffffffffu, every);
+            if ((tid & 31) == 0) s.bits[pass & 1][tid >> 5] = make_uint2(any, every);
         }
         unsigned bin, in_bin, above;
         find_bin<CLN>(s, hist, (unsigned)need, bin, in_bin, above);
         th.prefix = th.prefix << width | bin;
         need -= (int)above;
+        if (SAME && pass) {                            // the bin's keys are one key: no more digits to look at
+            any = 0, every = ~0u;
+#pragma unroll
+            for (int w = 0; w < SEL_WARPS; ++w) {
+                const uint2 b = s.bits[pass & 1][w];
+                any |= b.x;
+                every &= b.y;
+            }
+            if (any == every) {
+                th.prefix = any;
+                th.shift = 0;
+            }
+        }
         if (in_bin == (unsigned)need) return th;
         if (th.shift == 0) break;
         // the next pass's counts are zero already; these are made so for the pass after it
         for (int i = tid; i < BINS; i += SEL_THREADS) hist[i] = 0;
     }
     // more equal keys than are wanted: the index of the need-th of them
-    unsigned mine = 0, total, before, all;
-    for (int i = tid; i < n_local; i += SEL_THREADS) mine += key(i) == th.prefix;
-    block_scan(s, 0, mine, total);
-    cluster_sums<CLN>(s, 0, total, before, all);
-    if (before + total <= (unsigned)need) return th;   // uniform over the CTA
-    th.cut = -1;
-    if (before >= (unsigned)need) return th;
+    unsigned total, before = 0;
+    if constexpr (CLN > 1) {
+        unsigned mine = 0, all;
+        for (int i = tid; i < n_local; i += SEL_THREADS) mine += key(i) == th.prefix;
+        block_scan(s, 0, mine, total);
+        cluster_sums<CLN>(s, 0, total, before, all);
+        if (before + total <= (unsigned)need) return th;             // uniform over the CTA
+        th.cut = -1;
+        if (before >= (unsigned)need) return th;
+    } else {
+        th.cut = -1;
+    }
     for (int i0 = 0; i0 < n_local; i0 += SPAN) {
         unsigned mask = 0, at;
-        for (int k = 0; k < 32 && i0 + k * SEL_THREADS < n_local; ++k) {
+        const int strips = min(32, (n_local - i0 + SEL_THREADS - 1) / SEL_THREADS);
+#pragma unroll 4
+        for (int k = 0; k < strips; ++k) {
             const int i = i0 + k * SEL_THREADS + tid;
             mask |= (unsigned)(i < n_local && key(i) == th.prefix) << k;
         }
@@ -252,21 +285,25 @@ __device__ __forceinline__ void ranked(Select& s, Flag flag, int n_local, Begin 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto flags = [&](int i0) {
         unsigned mask = 0;
-        for (int k = 0; k < 32 && i0 + k * SEL_THREADS < n_local; ++k) {
+        const int strips = min(32, (n_local - i0 + SEL_THREADS - 1) / SEL_THREADS);
+#pragma unroll 4
+        for (int k = 0; k < strips; ++k) {
             const int i = i0 + k * SEL_THREADS + tid;
             mask |= (unsigned)(i < n_local && flag(i)) << k;
         }
         return mask;
     };
     auto report = [&](int i0, unsigned mask, unsigned before) {
-        for (int k = 0; k < 32 && i0 + k * SEL_THREADS < n_local; ++k) {
+        const int strips = min(32, (n_local - i0 + SEL_THREADS - 1) / SEL_THREADS);
+#pragma unroll 4
+        for (int k = 0; k < strips; ++k) {
             const unsigned b = __ballot_sync(0xffffffffu, mask >> k & 1);
             if (mask >> k & 1)
                 emit(i0 + k * SEL_THREADS + tid, before + s.hist[0][k * SEL_WARPS + warp] + __popc(b & ((1u << lane) - 1)));
         }
     };
     unsigned total, before, all, at;
-    if (n_local <= SPAN) {
+    if (CLN == 1 || n_local <= SPAN) {
         const unsigned mask = flags(0);
         strip_scan(s, mask, at, total);
         cluster_sums<CLN>(s, 1, total, before, all);
@@ -293,47 +330,59 @@ __device__ __forceinline__ void ranked(Select& s, Flag flag, int n_local, Begin 
 
 // ---- eviction -------------------------------------------------------------------------------------------------
 // Key of a row: protected rows above everything; weights in order; NaN below everything. -0 equals +0.
-constexpr int EV_KEYS = 40960;           // keys that a CTA holds in shared memory (160 KiB)
-constexpr int EV_SINGLE = 32768;         // rows up to which one CTA chooses alone
-constexpr int EV_FUSED = 512;            // moves up to which that CTA makes them itself
+constexpr int EV_KEYS = 40960;           // keys that a CTA of a cluster holds in shared memory (160 KiB)
+// Rows up to which one CTA chooses alone. One against a cluster, 4 / 16 heads: 13.7 / 15.2 us against 15.2 / 19.5 for 8000
+// rows, 17.8 / 19.2 against 15.5 / 19.7 for 12000, 47 / 66 against 23 / 43 for 30000.
+constexpr int EV_SINGLE = 10240;
+// Moves up to which that CTA makes them itself: an SM moves some 35 bytes a clock, a second kernel starts in 1.5 us. At
+// most 76 of 4 heads of 128: 7.7 us against 7.9, 256: 10.4 against 9.1, 504: 13.2 against 7.9.
+constexpr int EV_FUSED = 64;
 __device__ __forceinline__ unsigned evict_key(float acc, int pos, int n_sink, int recent_from) {
     if (pos < n_sink || pos >= recent_from) return 0xFFFFFFFFu;
     if (acc != acc) return 0u;
     const unsigned b = __float_as_uint(acc + 0.f);
     return b >> 31 ? ~b : b | 0x80000000u;
 }
-// Moves i0, i0 + 1, .. of N: K and V rows by 16-byte pieces, all N loads before the first store. Rows read are at or
+// Moves i0 .. i1 - 1, at most N: K and V rows by 16-byte pieces, all loads before the first store. Rows read are at or
 // above n_keep, rows written below it.
 template <int N>
 __device__ __forceinline__ void move_rows(const CacheEvict& e, int kv, const int32_t* to, const int32_t* from, int i0,
-                                          int n) {
+                                          int i1) {
+    static_assert(N <= 32, "a lane for each row's weight and position");
     const int lane = threadIdx.x & 31, c16 = e.hd / 8;
     const int64_t hb = (int64_t)kv * e.max_rows;
-    int t[N], f[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        t[k] = i0 + k < n ? to[i0 + k] : -1;
-        f[k] = i0 + k < n ? from[i0 + k] : 0;
+    const bool mine = lane < i1 - i0;                  // lane k: row k's weight and position
+    int t1 = -1, f1 = 0, p1 = 0;
+    float a1 = 0.f;
+    if (mine) {
+        t1 = to[i0 + lane];
+        f1 = from[i0 + lane];
+        a1 = e.acc[hb + f1];
+        p1 = e.pos[hb + f1];
     }
-    for (int p = lane; p < 2 * c16; p += 32) {
+    for (int p = lane; p < (2 * c16 + 31) / 32 * 32; p += 32) {
         char* c = static_cast<char*>(p < c16 ? e.kc : e.vc) + (int64_t)kv * e.hs * 2 + (p < c16 ? p : p - c16) * 16;
         uint4 v[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (t[k] >= 0) v[k] = *reinterpret_cast<const uint4*>(c + (int64_t)f[k] * e.rs * 2);
+        for (int k = 0; k < N; ++k) {
+            const int f = __shfl_sync(0xffffffffu, f1, k);
+            if (i0 + k < i1 && p < 2 * c16) v[k] = *reinterpret_cast<const uint4*>(c + (int64_t)f * e.rs * 2);
+        }
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (t[k] >= 0) *reinterpret_cast<uint4*>(c + (int64_t)t[k] * e.rs * 2) = v[k];
+        for (int k = 0; k < N; ++k) {
+            const int t = __shfl_sync(0xffffffffu, t1, k);
+            if (i0 + k < i1 && p < 2 * c16) *reinterpret_cast<uint4*>(c + (int64_t)t * e.rs * 2) = v[k];
+        }
     }
-    if (lane < N && i0 + lane < n) {
-        const int tt = to[i0 + lane], ff = from[i0 + lane];
-        e.acc_out[hb + tt] = e.acc[hb + ff];
-        e.pos_out[hb + tt] = e.pos[hb + ff];
+    if (mine) {
+        e.acc_out[hb + t1] = a1;
+        e.pos_out[hb + t1] = p1;
     }
 }
 // Grid (CLN, n_kv). Lists the rows to fill and the rows to move (ascending both), copies acc and pos of the rows below
-// n_keep to their outputs, and makes the moves itself where there are few (to, from then sit in shared memory).
-template <int CLN>
+// n_keep to their outputs, and makes the moves itself where there are few (to, from then sit in shared memory). HELD: a CTA's keys fit in shared memory;
+// otherwise they are formed again each time.
+template <int CLN, bool HELD>
 __global__ void __launch_bounds__(SEL_THREADS) k_evict_choose(const CacheEvict e, const bool fused) {
     pdl_enter();
     extern __shared__ unsigned s_key[];
@@ -344,13 +393,12 @@ __global__ void __launch_bounds__(SEL_THREADS) k_evict_choose(const CacheEvict e
     const int32_t* pos = e.pos + (int64_t)kv * e.max_rows;
     const int first = (int)((int64_t)e.n_rows * rank / CLN), last = (int)((int64_t)e.n_rows * (rank + 1) / CLN);
     const int n = last - first;
-    const bool held = CLN == 1 || n <= EV_KEYS;
     // rows that stay are copied where the outputs are other buffers; rows that are filled are written again, later
     float* acc_out = e.acc_out + (int64_t)kv * e.max_rows;
     int32_t* pos_out = e.pos_out + (int64_t)kv * e.max_rows;
     const bool copy = e.acc_out != e.acc || e.pos_out != e.pos;
     auto fresh = [&](int i) { return evict_key(acc[first + i], pos[first + i], e.n_sink, e.recent_from); };
-    if (held) {
+    if constexpr (HELD) {
         for (int i0 = tid; i0 < n; i0 += 8 * SEL_THREADS) {
             float a[8];
             int p[8];
@@ -378,8 +426,8 @@ __global__ void __launch_bounds__(SEL_THREADS) k_evict_choose(const CacheEvict e
         }
     }
     __syncthreads();
-    auto key = [&](int i) { return held ? s_key[i] : fresh(i); };
-    const Threshold th = select_threshold<CLN, 32>(sel, key, n, e.n_keep);
+    auto key = [&](int i) { return HELD ? s_key[i] : fresh(i); };
+    const Threshold<unsigned> th = select_threshold<CLN, 32, unsigned>(sel, key, n, e.n_keep);
     // rows to fill (below n_keep, not kept) come before rows to move (at or above n_keep, kept), as many of each
     int32_t* to = CLN == 1 && fused ? s_to : e.to + (int64_t)kv * e.max_rows;
     int32_t* from = CLN == 1 && fused ? s_from : e.from + (int64_t)kv * e.max_rows;
@@ -397,7 +445,10 @@ __global__ void __launch_bounds__(SEL_THREADS) k_evict_choose(const CacheEvict e
     if constexpr (CLN == 1) {
         if (fused) {
             __syncthreads();
-            for (int i = (tid >> 5) * 8; i < moves; i += SEL_WARPS * 8) move_rows<8>(e, kv, s_to, s_from, i, moves);
+            // as many rows a warp as the warps have in common, up to 16 at once
+            const int per = min(16, (moves + SEL_WARPS - 1) / SEL_WARPS);
+            for (int i = (tid >> 5) * per; i < moves; i += SEL_WARPS * per)
+                move_rows<16>(e, kv, s_to, s_from, i, min(i + per, moves));
         }
     } else {
         cg::this_cluster().sync();                     // no CTA leaves while its counts may be read
@@ -407,7 +458,7 @@ __global__ void __launch_bounds__(256) k_evict_move(const CacheEvict e) {
     pdl_enter();
     const int kv = blockIdx.y, i = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 4, n = e.n_moves[kv];
     if (i >= n) return;
-    move_rows<4>(e, kv, e.to + (int64_t)kv * e.max_rows, e.from + (int64_t)kv * e.max_rows, i, n);
+    move_rows<4>(e, kv, e.to + (int64_t)kv * e.max_rows, e.from + (int64_t)kv * e.max_rows, i, min(i + 4, n));
 }
 
 // ---- bounds of complete blocks: one CTA per (block, KV head) --------------------------------------------------
@@ -703,7 +754,7 @@ __global__ void __launch_bounds__(SEL_THREADS) k_block_choose(const CacheSelect 
         __syncthreads();
     }
     auto key = [&](int i) { return s_keys[i]; };
-    const Threshold th = select_threshold<SEL, 63>(ss, key, n, n_take);
+    const Threshold<unsigned long long> th = select_threshold<SEL, 63, unsigned long long>(ss, key, n, n_take);
     ranked<SEL>(
         ss, [&](int i) { return th.in(s_keys[i], i); }, n, [](unsigned) {},
         [&](int i, unsigned r) {
@@ -740,17 +791,17 @@ cudaError_t launch_cache_evict(const CacheEvict& e, cudaStream_t s) {
     if (e.n_rows <= EV_SINGLE) {
         const bool fused = most <= EV_FUSED;
         static SmemLimit limit;
-        cudaError_t rc = limit.raise((const void*)k_evict_choose<1>, EV_SINGLE * 4);
+        cudaError_t rc = limit.raise((const void*)k_evict_choose<1, true>, EV_SINGLE * 4);
         if (rc != cudaSuccess) return rc;
-        rc = launch_pdl(k_evict_choose<1>, dim3(1, e.n_kv), SEL_THREADS, (size_t)e.n_rows * 4, s, e, fused);
+        rc = launch_pdl(k_evict_choose<1, true>, dim3(1, e.n_kv), SEL_THREADS, (size_t)e.n_rows * 4, s, e, fused);
         if (rc != cudaSuccess || fused) return rc;
     } else {
         static SmemLimit limit;
-        cudaError_t rc = limit.raise((const void*)k_evict_choose<CL>, EV_KEYS * 4);
+        cudaError_t rc = limit.raise((const void*)k_evict_choose<CL, true>, EV_KEYS * 4);
         if (rc != cudaSuccess) return rc;
         const int n = (e.n_rows + CL - 1) / CL;
-        rc = launch_pdl_cluster(k_evict_choose<CL>, CL, dim3(CL, e.n_kv), SEL_THREADS, n <= EV_KEYS ? (size_t)n * 4 : 0, s, e,
-                            false);
+        rc = n <= EV_KEYS ? launch_pdl_cluster(k_evict_choose<CL, true>, CL, dim3(CL, e.n_kv), SEL_THREADS, (size_t)n * 4, s, e, false)
+                          : launch_pdl_cluster(k_evict_choose<CL, false>, CL, dim3(CL, e.n_kv), SEL_THREADS, 0, s, e, false);
         if (rc != cudaSuccess) return rc;
     }
     if (most == 0) return cudaSuccess;
