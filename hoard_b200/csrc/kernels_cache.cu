@@ -58,18 +58,22 @@ __device__ __forceinline__ void cp16z(unsigned dst, const void* src, bool there)
 template <int N> __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// Warps and ring slots of one CTA (one CTA per SM). A slot is the K or the V of 16 rows; eight warps with all but one
-// of their slots in flight keep 128 to 160 KiB per SM on the way.
-constexpr int W = 8;
+// Warps and ring slots of one CTA (one CTA per SM). A slot is the K or the V of 16 rows; the warps with all but one of their
+// slots in flight keep 128 to 170 KiB per SM on the way. Eight warps; tiles of 8 rows of 64 dims have registers and slots for
+// twelve: 8 heads over 100000 cache rows 63.3 us with 8, 39.0 with 12, 37.9 with 16; over 40 rows 4.1, 4.5, 4.7. At 128 dims
+// twelve are slower over few rows and no faster over many (4 heads, 8 rows: 7.8 / 9.0 over 2300, 36.7 / 39.1 over
+// 100000), at 256 dims slower everywhere (9.2 / 10.8, 39.6 / 41.5).
 constexpr int MAX_CLUSTER = 4;           // CTAs of a cluster: with a CTA per SM, eight rarely fit in a GPC at once
-template <int HD> struct Plan {
-    static constexpr int NS = HD == 256 ? 3 : 6;
+constexpr int plan_warps(int hd, int nt) { return hd == 64 && nt == 1 ? 12 : 8; }
+template <int HD, int NT> struct Plan {
+    static constexpr int W = plan_warps(HD, NT), NS = HD == 256 ? 3 : W == 12 ? 8 : 6;
     static constexpr int SLOT = KV_CHUNK * HD * 2;                 // bytes
     static constexpr int RING = W * NS * SLOT;
 };
 template <typename KT, int HD, int NT> constexpr int q_bytes() { return HD / 16 * NT * Terms<KT>::N * 32 * 8; }
 template <typename KT, int HD, int NT> constexpr int attn_smem() {
-    return Plan<HD>::RING + q_bytes<KT, HD, NT>();
+    constexpr int ring = Plan<HD, NT>::RING + q_bytes<KT, HD, NT>(), join = Plan<HD, NT>::W * 8 * NT * (HD + 4) * 4;
+    return ring > join ? ring : join;
 }
 
 __device__ __forceinline__ int past_rows(const CacheAttn& a) {
@@ -77,8 +81,8 @@ __device__ __forceinline__ int past_rows(const CacheAttn& a) {
 }
 
 template <typename KT, int HD, int NT, bool BLOCKS>
-__global__ void __launch_bounds__(W * 32, 1) k_cache_attention(const CacheAttn a) {
-    constexpr int NS = Plan<HD>::NS, SLOT = Plan<HD>::SLOT, TN = Terms<KT>::N;
+__global__ void __launch_bounds__(Plan<HD, NT>::W * 32, 1) k_cache_attention(const CacheAttn a) {
+    constexpr int W = Plan<HD, NT>::W, NS = Plan<HD, NT>::NS, SLOT = Plan<HD, NT>::SLOT, TN = Terms<KT>::N;
     constexpr int KS = HD / 16;                        // K steps of q . K = M tiles of V^T
     constexpr int RT = 8 * NT;                         // query rows of the tile
     constexpr int PITCH = HD * 2;                      // bytes of a staged row
@@ -95,7 +99,7 @@ __global__ void __launch_bounds__(W * 32, 1) k_cache_attention(const CacheAttn a
     const int n_past = past_rows(a);
     const int kv = BLOCKS ? prob / a.m : prob;
     const int t0 = BLOCKS ? prob - kv * a.m : 0;       // first token of the problem's rows
-    uint32_t* qf = reinterpret_cast<uint32_t*>(smem + Plan<HD>::RING);
+    uint32_t* qf = reinterpret_cast<uint32_t*>(smem + Plan<HD, NT>::RING);
 
     // chunks of this CTA: past rows (or the listed blocks' rows), then the tokens' own rows
     const int sub_shift = BLOCKS ? __ffs(a.block / KV_CHUNK) - 1 : 0;         // chunks of a block: a power of two
@@ -138,12 +142,12 @@ __global__ void __launch_bounds__(W * 32, 1) k_cache_attention(const CacheAttn a
 
     // the tile's q rows as fragments of the B operand: [K step][8-row tile][term][lane] of 8 bytes. A warp takes
     // every W-th row and loads all of them before it uses the first
-    constexpr int QR = RT / W;
+    constexpr int QR = (RT + W - 1) / W;
     float x[QR][HD / 32];
 #pragma unroll
     for (int i = 0; i < QR; ++i) {
         const int row = tile * RT + warp + i * W;      // row = (token - t0) * g + head of the KV head
-        const bool live = row < a.R;
+        const bool live = warp + i * W < RT && row < a.R;
         const int t = t0 + (live ? row / a.g : 0), h = kv * a.g + (live ? row % a.g : 0);
         const float* q = a.q + t * a.q_ts + h * a.q_hs;
 #pragma unroll
@@ -156,6 +160,7 @@ __global__ void __launch_bounds__(W * 32, 1) k_cache_attention(const CacheAttn a
 #pragma unroll
     for (int i = 0; i < QR; ++i) {
         const int r = warp + i * W;
+        if (RT % W && r >= RT) break;
         float am = 0.f;
         bool bad = false;
 #pragma unroll
@@ -675,6 +680,7 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
 template <typename KT, int HD, int NT, bool BLOCKS>
 cudaError_t attention_go(const CacheAttn& a, cudaStream_t s) {
     constexpr int smem = attn_smem<KT, HD, NT>();
+    constexpr int W = Plan<HD, NT>::W;
     static SmemLimit limit;
     cudaError_t e = limit.raise((const void*)k_cache_attention<KT, HD, NT, BLOCKS>, smem);
     if (e != cudaSuccess) return e;
@@ -717,7 +723,7 @@ int cache_tile_dims(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 struct TileCost {
     float base, chunk;
 };
-constexpr TileCost TILE_COST[3][2] = {{{2.7f, 1.3f}, {4.3f, 1.15f}}, {{3.2f, 1.4f}, {4.4f, 1.8f}}, {{3.9f, 2.6f}, {5.5f, 3.9f}}};
+constexpr TileCost TILE_COST[3][2] = {{{3.4f, 1.15f}, {4.3f, 1.15f}}, {{3.2f, 1.4f}, {4.4f, 1.8f}}, {{3.9f, 2.6f}, {5.5f, 3.9f}}};
 constexpr TileCost TC_COST[2] = {{8.6f, 0.7f}, {10.f, 1.f}};
 // CTAs up to which clusters of four all run at once (a CTA per SM, and SMs of a GPC left over)
 constexpr int CLUSTERED_CTAS = 128;
@@ -732,6 +738,7 @@ void cache_plan(CacheAttn& a, int n_chunks, int64_t past_rows) {
     a.tc_splits = 0;
     for (int rt = 8; rt <= (a.R > 8 ? 16 : 8); rt += 8) {
         const TileCost& cost = TILE_COST[di][rt / 16];
+        const int W = plan_warps(dims, rt / 8);
         const int64_t row_tiles = up_div(a.R, rt), ctas = a.problems * row_tiles, useful = up_div(n_chunks, W);
         const int64_t fit = KV_SMS / ctas, most = useful < fit ? useful : fit;
         auto offer = [&](int64_t splits, bool cluster, float join) {
