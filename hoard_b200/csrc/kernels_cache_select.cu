@@ -658,9 +658,10 @@ __global__ void __launch_bounds__(32 * SC_WARPS * PARTS, PARTS == 1 ? 5 : 2) k_b
 // Key of a score max_h (u_h - top_h) <= 0: the bits of its magnitude, turned over; NaN lowest.
 constexpr int BS_MAX_G = 64;
 // Candidates up to which one CTA chooses, and above which a cluster's eight form the keys for it, if the clusters of all
-// problems fit on the GPU at once: 4086 candidates x 8 heads 14 us alone, 11.5 with a cluster; 1557 candidates of 32
-// problems 10 alone, 17 with clusters.
-constexpr int BS_ONE = 8192, BS_ALONE = 1024;
+// problems fit on the GPU at once: BS_ALONE and BS_MORE for each problem, because many clusters start later. Alone against a
+// cluster (all of a call, 128 dims): 8 problems 18.9 / 20.7 us for 1089 candidates, 21.3 / 21.5 for 1557, 25.1 / 23.5 for 3120;
+// 16 problems 22.5 / 25.3 for 1557, 30.4 / 30.6 for 3120, 46.7 / 42.1 for 6245.
+constexpr int BS_ONE = 8192, BS_ALONE = 1024, BS_MORE = 128;
 __device__ __forceinline__ unsigned long long score_key(double v) {
     return v != v ? 0ull : 0x7FFFFFFFFFFFFFFFull - (unsigned long long)__double_as_longlong(fabs(v));
 }
@@ -836,7 +837,7 @@ cudaError_t launch_cache_select(const CacheSelect& asked, cudaStream_t s) {
         e = launch_pdl(fn, grid, 32 * SC_WARPS * parts, 0, s, c, nb_cap);
         if (e != cudaSuccess) return e;
     }
-    if (n_cand <= BS_ONE && (n_cand <= BS_ALONE || c.n_kv * c.m * CL > KV_SMS)) {
+    if (n_cand <= BS_ONE && (n_cand <= BS_ALONE + BS_MORE * c.n_kv * c.m || c.n_kv * c.m * CL > KV_SMS)) {
         static SmemLimit limit;
         e = limit.raise((const void*)k_block_choose<1, false>, BS_ONE * 8);
         if (e != cudaSuccess) return e;
