@@ -10,6 +10,11 @@
 // between warps), with its own running maximum and total, and the partial results are joined once at the
 // end of the CTA and once after all CTAs (k_cache_combine).
 //
+// Bound by: latency over short caches (one CTA's chain of loads, products and joins: 4.5 us over 40 rows), the warps' chains of
+// products over middle ones (a 16-row chunk of a warp 1.1 to 1.4 us at 64 and 128 dims, 2.6 at 256), DRAM over long ones: 16
+// heads of 128, one token each, over 30000 rows 245 MB in 42 us, 5.8 TB/s. At 256 dims the registers allow eight warps, whose
+// chains do not cover the loads: 2 heads over 32769 rows 67 MB in 18.5 us, 3.6 TB/s.
+//
 // Precision. K and V enter the products as they are stored. q (f32) and the weights p (f32) are written as
 // sums of f16 or bf16 terms (kv_terms.cuh), whatever the cache's type is, so a product is f32-accurate; sums, maxima
 // and totals are f32.
@@ -534,9 +539,11 @@ __global__ void __launch_bounds__(Plan<HD, NT>::W * 32, 1) k_cache_attention(con
 }
 
 // ---- joins the splits of every query row, and with acc adds the rows' weights to the accumulated ones -------
-// A CTA per query row (token, head) and block of columns (one block where there are rows enough): the factors 2^(m_s - M) of the splits, one split per thread, then float4
-// columns x split groups, eight partial rows in flight per thread. The CTAs after them take 1024 cache rows of a KV
-// head each: w = sum over the head's query rows of 2^(s - M) / L in row order, four cache rows per thread.
+// A CTA per query row (token, head) and block of columns (one block where there are rows enough): the factors
+// 2^(m_s - M) of the splits, one split per thread, then float4 columns x split groups, eight partial rows in flight per
+// thread. The CTAs after them take 1024 cache rows of a KV head each: w = sum over the head's query rows of
+// 2^(s - M) / L in row order, four cache rows per thread. Bound by latency, three dependent rounds of loads: 3.5 us for 512
+// rows of 33 splits; with a warp per row and its splits in sequence it was 29.
 constexpr int CB = 256, ACC_PER = 4, ACC_ROWS = CB * ACC_PER, ACC_MAX_R = 512;
 static_assert(KV_SMS + 1 <= CB, "one split per thread");
 __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt, int col_blocks, int per) {

@@ -379,6 +379,8 @@ __device__ __forceinline__ void move_rows(const CacheEvict& e, int kv, const int
         e.pos_out[hb + t1] = p1;
     }
 }
+// Bound by barriers and dependent shared loads: 2304 rows 4.3 us to the threshold (two passes, equal weights) and 1.8 for the
+// ranks; 65521 rows by a cluster 3.6 for the keys, 7.8 to the threshold, 5.6 for the ranks.
 // Grid (CLN, n_kv). Lists the rows to fill and the rows to move (ascending both), copies acc and pos of the rows below
 // n_keep to their outputs, and makes the moves itself where there are few (to, from then sit in shared memory). HELD: a CTA's keys fit in shared memory;
 // otherwise they are formed again each time.
@@ -461,7 +463,9 @@ __global__ void __launch_bounds__(256) k_evict_move(const CacheEvict e) {
     move_rows<4>(e, kv, e.to + (int64_t)kv * e.max_rows, e.from + (int64_t)kv * e.max_rows, i, min(i + 4, n));
 }
 
-// ---- bounds of complete blocks: one CTA per (block, KV head) --------------------------------------------------
+// ---- bounds of complete blocks: one CTA per (block, KV head), 16 bytes of a row per thread ----------------------
+// Bound by DRAM and the CTAs' start: 32767 rows x 4 heads of 128, 33.5 MB in 8 us, 4.2 TB/s. CTAs that take several blocks need
+// the next block's loads in registers (spills) and were slower.
 __device__ __forceinline__ __half2 min2(__half2 a, __half2 b) { return __hmin2(a, b); }
 __device__ __forceinline__ __half2 max2(__half2 a, __half2 b) { return __hmax2(a, b); }
 __device__ __forceinline__ __nv_bfloat162 min2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmin2(a, b); }
@@ -655,7 +659,8 @@ __global__ void __launch_bounds__(32 * SC_WARPS * PARTS, PARTS == 1 ? 5 : 2) k_b
 }
 
 // ---- selection: one CTA or cluster per (KV head, token) -------------------------------------------------------
-// Key of a score max_h (u_h - top_h) <= 0: the bits of its magnitude, turned over; NaN lowest.
+// Key of a score max_h (u_h - top_h) <= 0: the bits of its magnitude, turned over; NaN lowest. Bound by latency: 506 candidates
+// of 8 heads 5.7 us (loads 1, maxima 0.7, keys 1.1, threshold 1.9, ranks 1).
 constexpr int BS_MAX_G = 64;
 // Candidates up to which one CTA chooses, and above which a cluster's eight form the keys for it, if the clusters of all
 // problems fit on the GPU at once: BS_ALONE and BS_MORE for each problem, because many clusters start later. Alone against a
