@@ -203,7 +203,7 @@ def test_accumulated_weights(n_head, n_kv, hd, kt, m, n_past):
 
 
 @pytest.mark.parametrize("n_rows,n_keep", [(1, 1), (2, 1), (33, 32), (100, 7), (1000, 999), (2304, 2048), (5000, 600),
-                                           (40000, 37000), (70001, 3000)])
+                                           (10240, 10176), (10240, 10100), (10241, 10177), (40000, 37000), (70001, 3000)])
 @pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
 def test_evict(n_rows, n_keep, kind):
     n_kv, hd, kt = 3, 64, F16
@@ -228,6 +228,23 @@ def test_evict(n_rows, n_keep, kind):
                            w.view(torch.int16 if a.dtype is kt else torch.int32))
         assert torch.equal(b.cpu().view(torch.int16 if a.dtype is kt else torch.int32),
                            w.view(torch.int16 if a.dtype is kt else torch.int32))
+
+
+@pytest.mark.parametrize("n_rows,n_keep", [(140001, 70000), (330001, 5000)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_very_many_rows(n_rows, n_keep, ties):
+    """More rows for each CTA of the cluster than one scan takes, and than its shared memory holds."""
+    g = torch.Generator(device=DEV).manual_seed(n_rows)
+    k, v = (torch.randn(n_rows, 2, 8, generator=g, device=DEV).half() for _ in range(2))
+    acc = torch.exp(2 * torch.randn(2, n_rows, generator=g, device=DEV))
+    if ties:
+        acc = torch.floor(acc).clamp(max=2)
+    pos = torch.arange(n_rows, device=DEV, dtype=torch.int32).repeat(2, 1)
+    want = ref.evict(k, v, acc, pos, n_rows, n_keep, 4, n_rows - 100)
+    ops = cache.CacheOps(n_head=2, n_head_kv=2, head_dim=8, kv_dtype=F16, max_rows=n_rows)
+    ops.evict(k, v, acc, pos, n_rows, n_keep, n_sink=4, recent_from=n_rows - 100)
+    for a, w in zip((k, v, acc, pos), want):
+        assert torch.equal(a.cpu(), w)
 
 
 def test_evict_more_protected_rows_than_are_kept():
