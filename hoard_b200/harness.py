@@ -268,6 +268,8 @@ class DecodeModel:
             raise ValueError(f"max_batch must be 1..{cache.MAX_TOKENS}")
         if blocks is not None and budget is not None:
             raise ValueError("blocks of the cache need its rows in the order of positions: not with a budget")
+        if blocks is not None and max_ctx < blocks.block:
+            raise ValueError("max_ctx holds one block at least")
         if budget is not None and not (0 <= budget.n_sink and 0 <= budget.n_recent and budget.n_slack >= 1
                                        and budget.n_sink + budget.n_recent < budget.n_keep):
             raise ValueError("a budget keeps more rows than its first and last positions, and has slack")
@@ -732,6 +734,7 @@ class DecodeModel:
             self._tx, self._tx2, self._trot, self._tatt = z(B, H), z(B, H), z(B, self.nq), z(B, self.nq)
             self._tlg = z(B, c.n_vocab)
             self._tqkv = [_parr([self._tq[i].data_ptr(), self._tk[i].data_ptr(), self._tv[i].data_ptr()]) for i in range(B)]
+        self._tree_m = m
         vis = torch.tensor(words, dtype=torch.int64).to(self.dev)
         pos = torch.tensor([base + d for d in depth], dtype=torch.int32).to(self.dev)
         tok = torch.tensor(list(tokens), dtype=torch.int32).to(self.dev)
@@ -773,9 +776,13 @@ class DecodeModel:
     def accept(self, base: int, path, stream=None):
         """After forward_tree at `base`: the k and v of the drafted tokens path[0], path[1], .. (a root and its accepted
         descendants) become cache rows base, base + 1, .."""
+        path = list(path)
+        if path and (self._tree_ops is None or path[-1] >= self._tree_m):
+            raise ValueError("a path names tokens of the last forward_tree")
         for j in range(len(self.kv_index)):
             k3, v3 = self._heads(self.kc[j]), self._heads(self.vc[j])
-            self._tree_ops.take(k3, v3, base, path, stream=stream)
+            if path:
+                self._tree_ops.take(k3, v3, base, path, stream=stream)
             if self.blocks and path:
                 self._tree_ops.block_bounds(k3, self.bounds[j], base, base + len(path), stream=stream)
 

@@ -114,6 +114,17 @@ def test_token_that_sees_nothing(kt):
     assert rel(out, want) < TOL and out[0].abs().max() == 0 and out[3].abs().max() == 0
 
 
+@pytest.mark.parametrize("n_past,m", [(30, 5), (900, 20), (900, 64)])
+def test_visibility_bits_beyond_the_tokens(n_past, m):
+    q, k, v, _ = case(8, 2, 128, F16, n_past + m + 64, m)
+    k[n_past + m:], v[n_past + m:] = float("nan"), float("nan")
+    ops = cache.CacheOps(n_head=8, n_head_kv=2, head_dim=128, kv_dtype=F16, max_rows=n_past + m + 64, max_tokens=m)
+    every = torch.full((m,), -1, dtype=torch.int64, device=DEV)
+    just = torch.full((m,), (1 << m) - 1 if m < 64 else -1, dtype=torch.int64, device=DEV)
+    out = ops.tree_attention(q, k, v, n_past, vis=every)
+    assert torch.equal(out, ops.tree_attention(q, k, v, n_past, vis=just)) and torch.isfinite(out).all()
+
+
 @pytest.mark.parametrize("n_past,m", [(30, 3), (900, 20)])
 def test_nan_query_stays_in_its_row(n_past, m):
     q, k, v, _ = case(8, 2, 128, F16, n_past + m, m)

@@ -191,7 +191,7 @@ def test_context_beyond_shared_memory(weights):
 def test_wrong_settings_are_refused(weights):
     for bad in (dict(max_batch=0), dict(max_batch=65), dict(blocks=hx.BlockChoice(), budget=hx.CacheBudget(64)),
                 dict(budget=hx.CacheBudget(n_keep=100, n_sink=50, n_recent=50)), dict(budget=hx.CacheBudget(64, n_slack=0, n_recent=8)),
-                dict(kv_dtype=torch.float32)):
+                dict(kv_dtype=torch.float32), dict(blocks=hx.BlockChoice(block=128))):
         with pytest.raises(ValueError):
             make(OLMOE_S, weights, max_ctx=64, **bad)
     m = make(HYBRID_S, weights, max_ctx=64)
@@ -199,4 +199,12 @@ def test_wrong_settings_are_refused(weights):
         m.forward_tree([1], [-1], 3)
     with pytest.raises(ValueError):
         m.tree_generate([1, 2, 3], 4)
+    m.close()
+    m = make(OLMOE_S, weights, max_ctx=64)
+    with pytest.raises(ValueError):
+        m.accept(3, [0])                                 # no tree yet
+    m.forward_tree([1, 2], [-1, 0], 3)
+    with pytest.raises(ValueError):
+        m.accept(3, [0, 2])
+    m.accept(3, [])
     m.close()
