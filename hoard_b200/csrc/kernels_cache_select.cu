@@ -334,9 +334,10 @@ constexpr int EV_KEYS = 40960;           // keys that a CTA of a cluster holds i
 // Rows up to which one CTA chooses alone. One against a cluster, 4 / 16 heads: 13.7 / 15.2 us against 15.2 / 19.5 for 8000
 // rows, 17.8 / 19.2 against 15.5 / 19.7 for 12000, 47 / 66 against 23 / 43 for 30000.
 constexpr int EV_SINGLE = 10240;
-// Moves up to which that CTA makes them itself: an SM moves some 35 bytes a clock, a second kernel starts in 1.5 us. At
-// most 76 of 4 heads of 128: 7.7 us against 7.9, 256: 10.4 against 9.1, 504: 13.2 against 7.9.
-constexpr int EV_FUSED = 64;
+// Moves up to which that CTA makes them itself, one a warp: an SM moves some 35 bytes a clock, a second kernel starts in
+// 1.5 us. By the CTA against the kernel, heads of 128 / 256 dims: at most 32 moves 6.3 / 7.7 us against 6.3 / 6.6, 64 moves 7.5 / 9.1
+// against 7.2 / 7.5, 256 moves 10.4 / 13.3 against 8.2 / 8.6.
+constexpr int EV_FUSED = 16, EV_MOVES = 2;
 __device__ __forceinline__ unsigned evict_key(float acc, int pos, int n_sink, int recent_from) {
     if (pos < n_sink || pos >= recent_from) return 0xFFFFFFFFu;
     if (acc != acc) return 0u;
@@ -447,20 +448,19 @@ __global__ void __launch_bounds__(SEL_THREADS) k_evict_choose(const CacheEvict e
     if constexpr (CLN == 1) {
         if (fused) {
             __syncthreads();
-            // as many rows a warp as the warps have in common, up to 16 at once
-            const int per = min(16, (moves + SEL_WARPS - 1) / SEL_WARPS);
-            for (int i = (tid >> 5) * per; i < moves; i += SEL_WARPS * per)
-                move_rows<16>(e, kv, s_to, s_from, i, min(i + per, moves));
+            for (int i = tid >> 5; i < moves; i += SEL_WARPS) move_rows<1>(e, kv, s_to, s_from, i, i + 1);
         }
     } else {
         cg::this_cluster().sync();                     // no CTA leaves while its counts may be read
     }
 }
+// EV_MOVES rows a warp: 61440 rows of 256 bytes each in K and V (16 heads) 35.5 us for the whole eviction with 2, 39.2 with 1, 39.3
+// with 4, 43.5 with 8; 240 rows 8.2, 8.0, 8.7, 9.7.
 __global__ void __launch_bounds__(256) k_evict_move(const CacheEvict e) {
     pdl_enter();
-    const int kv = blockIdx.y, i = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 4, n = e.n_moves[kv];
+    const int kv = blockIdx.y, i = (blockIdx.x * 8 + (threadIdx.x >> 5)) * EV_MOVES, n = e.n_moves[kv];
     if (i >= n) return;
-    move_rows<4>(e, kv, e.to + (int64_t)kv * e.max_rows, e.from + (int64_t)kv * e.max_rows, i, min(i + 4, n));
+    move_rows<EV_MOVES>(e, kv, e.to + (int64_t)kv * e.max_rows, e.from + (int64_t)kv * e.max_rows, i, min(i + EV_MOVES, n));
 }
 
 // ---- bounds of complete blocks: one CTA per (block, KV head), 16 bytes of a row per thread ----------------------
@@ -811,7 +811,7 @@ cudaError_t launch_cache_evict(const CacheEvict& e, cudaStream_t s) {
         if (rc != cudaSuccess) return rc;
     }
     if (most == 0) return cudaSuccess;
-    return launch_pdl(k_evict_move, dim3((most + 31) / 32, e.n_kv), 256, 0, s, e);
+    return launch_pdl(k_evict_move, dim3((most + 8 * EV_MOVES - 1) / (8 * EV_MOVES), e.n_kv), 256, 0, s, e);
 }
 
 cudaError_t launch_cache_bounds(const void* kc, int64_t rs, int64_t hs, bool bf16, int n_kv, int hd, int max_rows,
