@@ -463,15 +463,21 @@ __global__ void __launch_bounds__(256) k_evict_move(const CacheEvict e) {
     move_rows<EV_MOVES>(e, kv, e.to + (int64_t)kv * e.max_rows, e.from + (int64_t)kv * e.max_rows, i, min(i + EV_MOVES, n));
 }
 
-// ---- bounds of complete blocks: one CTA per (block, KV head), 16 bytes of a row per thread ----------------------
-// Bound by DRAM and the CTAs' start: 32767 rows x 4 heads of 128, 33.5 MB in 8 us, 4.2 TB/s. CTAs that take several blocks need
-// the next block's loads in registers (spills) and were slower.
+// ---- bounds of complete blocks: 16 bytes of a row per thread, as many (block, KV head) per CTA as its threads take ----
+// Bound by DRAM and the CTAs' start: 120000 rows x 4 heads of 128, 123 MB in 23.4 us, 5.3 TB/s; 32767 rows 8.8 us, 3.8 TB/s.
+// A CTA for each block of 16 rows took 18 us for the latter, now 9.4; eight rows a thread 9.6. CTAs that take one block
+// after another need the next one's loads in registers (spills) and were slower.
 __device__ __forceinline__ __half2 min2(__half2 a, __half2 b) { return __hmin2(a, b); }
 __device__ __forceinline__ __half2 max2(__half2 a, __half2 b) { return __hmax2(a, b); }
 __device__ __forceinline__ __nv_bfloat162 min2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmin2(a, b); }
 __device__ __forceinline__ __nv_bfloat162 max2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2(a, b); }
 
-constexpr int BN_THREADS = 128;
+constexpr int BN_THREADS = 128, BN_ROWS = 16;
+// Threads in a column of a block: BN_ROWS rows each where there are threads enough
+__host__ __device__ inline int bounds_groups(int hd, int block) {
+    const int want = block / BN_ROWS, most = BN_THREADS / (hd / 8);
+    return want < 1 ? 1 : want < most ? want : most;
+}
 template <typename T2>
 __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __restrict__ kc, int64_t rs, int64_t hs,
                                                              int hd, int max_rows, int block, int row0, int row1,
@@ -483,18 +489,19 @@ __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __r
         row0 = max(0, *row1_dev);
         row1 = min(row0 + 1, max_rows);
     }
-    const int b = row0 / block + blockIdx.x, kv = blockIdx.y;
-    if (b >= row1 / block) return;
-    const int cols = hd / 8, groups = BN_THREADS / cols, gi = threadIdx.x / cols, c = threadIdx.x - gi * cols;
+    const int kv = blockIdx.y, cols = hd / 8, groups = bounds_groups(hd, block), per = groups * cols;
+    const int mine = threadIdx.x / per, b0 = row0 / block + blockIdx.x * (BN_THREADS / per), b = b0 + mine;
+    if (b0 >= row1 / block) return;
+    const int gi = (threadIdx.x - mine * per) / cols, c = (threadIdx.x - mine * per) - gi * cols;
+    const bool live = b < row1 / block && mine < BN_THREADS / per;
     union V {
         uint4 u;
         T2 h[4];
     };
     V lo, hi;
-    if (gi < groups) {
+    if (live) {
         const uint16_t* base = kc + (int64_t)b * block * rs + (int64_t)kv * hs + 8 * c;
-        const int r0 = min(gi, block - 1);
-        lo.u = hi.u = *reinterpret_cast<const uint4*>(base + r0 * rs);
+        lo.u = hi.u = *reinterpret_cast<const uint4*>(base + gi * rs);
         for (int r = gi + groups; r < block; r += 8 * groups) {      // eight rows' loads in flight
             V x[8];
 #pragma unroll
@@ -512,11 +519,11 @@ __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __r
         s_hi[threadIdx.x] = hi.u;
     }
     __syncthreads();
-    if (gi == 0) {
+    if (live && gi == 0) {
         for (int g = 1; g < groups; ++g) {
             V x, y;
-            x.u = s_lo[g * cols + c];
-            y.u = s_hi[g * cols + c];
+            x.u = s_lo[threadIdx.x + g * cols];
+            y.u = s_hi[threadIdx.x + g * cols];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 lo.h[i] = min2(lo.h[i], x.h[i]);
@@ -818,7 +825,8 @@ cudaError_t launch_cache_bounds(const void* kc, int64_t rs, int64_t hs, bool bf1
                                 int block, int row0, int row1, const int32_t* row1_dev, void* bounds, cudaStream_t s) {
     const int blocks = row1_dev ? 1 : row1 / block - row0 / block;
     if (blocks <= 0) return cudaSuccess;
-    const dim3 grid(blocks, n_kv);
+    const int at_once = BN_THREADS / (bounds_groups(hd, block) * (hd / 8));
+    const dim3 grid((blocks + at_once - 1) / at_once, n_kv);
     if (bf16)
         return launch_pdl(k_cache_bounds<__nv_bfloat162>, grid, BN_THREADS, 0, s, (const uint16_t*)kc, rs, hs, hd,
                           max_rows, block, row0, row1, row1_dev, (uint16_t*)bounds);
