@@ -464,23 +464,18 @@ __global__ void __launch_bounds__(256) k_evict_move(const CacheEvict e) {
 }
 
 // ---- bounds of complete blocks: 16 bytes of a row per thread, as many (block, KV head) per CTA as its threads take ----
-// Bound by DRAM and the CTAs' start: 120000 rows x 4 heads of 128, 123 MB in 23.4 us, 5.3 TB/s; 32767 rows 8.8 us, 3.8 TB/s.
-// A CTA for each block of 16 rows took 18 us for the latter, now 9.4; eight rows a thread 9.6. CTAs that take one block
-// after another need the next one's loads in registers (spills) and were slower.
+// Bound by DRAM and the CTAs' start: 120000 rows x 4 heads of 128, 123 MB in 23.2 us, 5.3 TB/s; 32767 rows 8.6 us, 3.9 TB/s.
+// A CTA for each block of 16 rows took 18 us for the latter, now 8.8. Sixteen rows a thread leave too few loads under way for
+// keys that are in L2 (2 us more); CTAs that take one block after another need the next one's loads in registers (spills).
 __device__ __forceinline__ __half2 min2(__half2 a, __half2 b) { return __hmin2(a, b); }
 __device__ __forceinline__ __half2 max2(__half2 a, __half2 b) { return __hmax2(a, b); }
 __device__ __forceinline__ __nv_bfloat162 min2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmin2(a, b); }
 __device__ __forceinline__ __nv_bfloat162 max2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2(a, b); }
 
-constexpr int BN_THREADS = 128, BN_ROWS = 16;
-// Threads in a column of a block: BN_ROWS rows each where there are threads enough
-__host__ __device__ inline int bounds_groups(int hd, int block) {
-    const int want = block / BN_ROWS, most = BN_THREADS / (hd / 8);
-    return want < 1 ? 1 : want < most ? want : most;
-}
+constexpr int BN_THREADS = 128, BN_ROWS = 8;
 template <typename T2>
 __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __restrict__ kc, int64_t rs, int64_t hs,
-                                                             int hd, int max_rows, int block, int row0, int row1,
+                                                             int hd, int max_rows, int shift, int row0, int row1,
                                                              const int32_t* __restrict__ row1_dev,
                                                              uint16_t* __restrict__ bounds) {
     pdl_enter();
@@ -489,11 +484,12 @@ __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __r
         row0 = max(0, *row1_dev);
         row1 = min(row0 + 1, max_rows);
     }
-    const int kv = blockIdx.y, cols = hd / 8, groups = bounds_groups(hd, block), per = groups * cols;
-    const int mine = threadIdx.x / per, b0 = row0 / block + blockIdx.x * (BN_THREADS / per), b = b0 + mine;
-    if (b0 >= row1 / block) return;
-    const int gi = (threadIdx.x - mine * per) / cols, c = (threadIdx.x - mine * per) - gi * cols;
-    const bool live = b < row1 / block && mine < BN_THREADS / per;
+    const int kv = blockIdx.y, block = 1 << shift, b0 = (row0 >> shift) + blockIdx.x * blockDim.z;
+    const int b = b0 + threadIdx.z, last = row1 >> shift;
+    if (b0 >= last) return;
+    const int cols = blockDim.x, groups = blockDim.y, c = threadIdx.x, gi = threadIdx.y;
+    const int tid = (threadIdx.z * groups + gi) * cols + c;
+    const bool live = b < last;
     union V {
         uint4 u;
         T2 h[4];
@@ -515,22 +511,22 @@ __global__ void __launch_bounds__(BN_THREADS) k_cache_bounds(const uint16_t* __r
                     hi.h[i] = max2(hi.h[i], x[k].h[i]);
                 }
         }
-        s_lo[threadIdx.x] = lo.u;
-        s_hi[threadIdx.x] = hi.u;
+        s_lo[tid] = lo.u;
+        s_hi[tid] = hi.u;
     }
     __syncthreads();
     if (live && gi == 0) {
         for (int g = 1; g < groups; ++g) {
             V x, y;
-            x.u = s_lo[threadIdx.x + g * cols];
-            y.u = s_hi[threadIdx.x + g * cols];
+            x.u = s_lo[tid + g * cols];
+            y.u = s_hi[tid + g * cols];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 lo.h[i] = min2(lo.h[i], x.h[i]);
                 hi.h[i] = max2(hi.h[i], y.h[i]);
             }
         }
-        uint16_t* out = bounds + ((int64_t)kv * (max_rows / block) + b) * 2 * hd + 8 * c;
+        uint16_t* out = bounds + ((int64_t)kv * (max_rows >> shift) + b) * 2 * hd + 8 * c;
         *reinterpret_cast<uint4*>(out) = lo.u;
         *reinterpret_cast<uint4*>(out + hd) = hi.u;
     }
@@ -825,12 +821,14 @@ cudaError_t launch_cache_bounds(const void* kc, int64_t rs, int64_t hs, bool bf1
                                 int block, int row0, int row1, const int32_t* row1_dev, void* bounds, cudaStream_t s) {
     const int blocks = row1_dev ? 1 : row1 / block - row0 / block;
     if (blocks <= 0) return cudaSuccess;
-    const int at_once = BN_THREADS / (bounds_groups(hd, block) * (hd / 8));
-    const dim3 grid((blocks + at_once - 1) / at_once, n_kv);
+    // threads: 16 bytes of a row, rows of a block (BN_ROWS each where there are threads enough), blocks
+    const int cols = hd / 8, want = block / BN_ROWS, most = BN_THREADS / cols, groups = want < most ? want : most;
+    const int at_once = BN_THREADS / (groups * cols), shift = __builtin_ctz(block);
+    const dim3 grid((blocks + at_once - 1) / at_once, n_kv), threads(cols, groups, at_once);
     if (bf16)
-        return launch_pdl(k_cache_bounds<__nv_bfloat162>, grid, BN_THREADS, 0, s, (const uint16_t*)kc, rs, hs, hd,
-                          max_rows, block, row0, row1, row1_dev, (uint16_t*)bounds);
-    return launch_pdl(k_cache_bounds<__half2>, grid, BN_THREADS, 0, s, (const uint16_t*)kc, rs, hs, hd, max_rows, block,
+        return launch_pdl(k_cache_bounds<__nv_bfloat162>, grid, threads, 0, s, (const uint16_t*)kc, rs, hs, hd,
+                          max_rows, shift, row0, row1, row1_dev, (uint16_t*)bounds);
+    return launch_pdl(k_cache_bounds<__half2>, grid, threads, 0, s, (const uint16_t*)kc, rs, hs, hd, max_rows, shift,
                       row0, row1, row1_dev, (uint16_t*)bounds);
 }
 
