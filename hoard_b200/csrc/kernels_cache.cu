@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(Plan<HD, NT>::W * 32, 1) k_cache_attention(con
     const int sub_shift = BLOCKS ? __ffs(a.block / KV_CHUNK) - 1 : 0;         // chunks of a block: a power of two
     const int n_pc = BLOCKS ? a.list_n[prob] << sub_shift : (n_past + KV_CHUNK - 1) / KV_CHUNK;
     const int n_chunks = n_pc + (a.m + KV_CHUNK - 1) / KV_CHUNK;
-    const int c_end = (int)((int64_t)n_chunks * (split + 1) / gridDim.x);
-    const int c_first = (int)((int64_t)n_chunks * split / gridDim.x) + warp;
+    const Share share_of(n_chunks, gridDim.x);
+    const int c_end = share_of.first(split + 1), c_first = share_of.first(split) + warp;
     const int32_t* list = BLOCKS ? a.list + (int64_t)prob * a.list_cap : nullptr;
     auto chunk_row = [&](int c) {                      // first cache row of chunk c
         if (c >= n_pc) return n_past + (c - n_pc) * KV_CHUNK;

@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     const int n_past = __shfl_sync(0xffffffffu, a.n_past_dev ? max(0, min(*a.n_past_dev, a.max_rows - a.m)) : a.n_past, 0);
     const int n_tiles = (n_past + TK - 1) / TK + 1;    // the last: the tokens' own rows
-    const int t_first = (int)((int64_t)n_tiles * split / a.tc_splits), t_end = (int)((int64_t)n_tiles * (split + 1) / a.tc_splits);
-    const int T = t_end - t_first;
+    const Share share(n_tiles, a.tc_splits);
+    const int t_first = share.first(split), T = share.first(split + 1) - t_first;
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");

@@ -58,6 +58,13 @@ template <typename KT> __device__ __forceinline__ RowScale row_scale(float am, b
     return {__uint_as_float((uint32_t)(127 + Terms<KT>::Q_EXP - e) << 23),
             __uint_as_float((uint32_t)(127 - Terms<KT>::Q_EXP + e) << 23)};
 }
+// n things in `parts` shares that differ by one at most: the first of share i (one 32-bit division, before the first load)
+struct Share {
+    unsigned each, more;
+    __device__ __forceinline__ Share(unsigned n, unsigned parts) : each(n / parts), more(n - each * parts) {}
+    __device__ __forceinline__ int first(unsigned i) const { return (int)(each * i + min(i, more)); }
+};
+
 // four floats to an address of any alignment that floats have
 __device__ __forceinline__ void store4(float* p, const float* v) {
     if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
