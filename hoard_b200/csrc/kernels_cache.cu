@@ -539,28 +539,29 @@ __global__ void __launch_bounds__(Plan<HD, NT>::W * 32, 1) k_cache_attention(con
 }
 
 // ---- joins the splits of every query row, and with acc adds the rows' weights to the accumulated ones -------
-// A CTA per query row (token, head) and block of columns (one block where there are rows enough): the factors
-// 2^(m_s - M) of the splits, one split per thread, then float4 columns x split groups, eight partial rows in flight per
-// thread. The CTAs after them take 1024 cache rows of a KV head each: w = sum over the head's query rows of
-// 2^(s - M) / L in row order, four cache rows per thread. Bound by latency, three dependent rounds of loads: 3.5 us for 512
-// rows of 33 splits; with a warp per row and its splits in sequence it was 29.
+// Grid y: the problem. A CTA per query row (token, head) and block of columns (one block where there are rows enough):
+// the factors 2^(m_s - M) of the splits, one split per thread, then float4 columns x split groups, eight partial rows in
+// flight per thread. The CTAs after them take 1024 cache rows of a KV head each: w = sum over the head's query rows of
+// 2^(s - M) / L in row order, four cache rows per thread. Bound by latency, three dependent rounds of loads: 3 us for 512
+// rows of 33 splits; with a warp per row and its splits in sequence it was 29, and integer divisions before the loads
+// cost 0.6.
 constexpr int CB = 256, ACC_PER = 4, ACC_ROWS = CB * ACC_PER, ACC_MAX_R = 512;
 static_assert(KV_SMS + 1 <= CB, "one split per thread");
-__global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt, int col_blocks, int per) {
+__global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt, int col_shift, int v4, unsigned v4_inv) {
     pdl_enter();
     __shared__ float s_f[CB];
     __shared__ float s_red[2][CB / 32];
     __shared__ float4 s_o[CB];
     __shared__ float s_mr[ACC_MAX_R], s_ir[ACC_MAX_R];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int n_rows = a.problems * a.R * col_blocks;
+    const int prob = blockIdx.y, n_rows = a.R << col_shift;
     if ((int)blockIdx.x < n_rows) {
-        const int at = blockIdx.x / col_blocks, prob = at / a.R, row = at - prob * a.R;
+        const int row = blockIdx.x >> col_shift;
         const int64_t part = (int64_t)prob * a.splits * a.R + row;       // + split * R
         // this CTA's float4 columns, shared out over split groups. The first round of sums is on its way before the
         // factors are known (what a split without weight left there is not used)
-        const int v4 = (a.hd / 4 + col_blocks - 1) / col_blocks, groups = CB / v4, gi = tid / v4;
-        const int lc = tid - gi * v4, c = (blockIdx.x - at * col_blocks) * v4 + lc;
+        const int groups = CB * v4_inv >> 16, gi = tid * v4_inv >> 16;                 // divided by v4
+        const int lc = tid - gi * v4, c = (blockIdx.x - (row << col_shift)) * v4 + lc;
         const bool mine = gi < groups && 4 * c < a.hd;
         const float* po = a.part_o + part * hdt + 4 * c;
         float4 u[8];
@@ -634,7 +635,7 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
     }
     // accumulation
     const int n = past_rows(a) + a.m;
-    const int x = blockIdx.x - n_rows, kv = x / per, j0 = (x - kv * per) * ACC_ROWS;
+    const int kv = prob, j0 = (blockIdx.x - n_rows) * ACC_ROWS;
     if (j0 >= n) return;
     const float* lg = a.logits + (int64_t)kv * a.R * a.logits_ld;
     float* acc = a.acc + (int64_t)kv * a.max_rows;
@@ -783,9 +784,11 @@ cudaError_t launch_cache_attention(const CacheAttn& a, cudaStream_t s) {
     const int rows = a.n_past_dev ? a.max_rows : a.n_past + a.m;
     const int per = (rows + ACC_ROWS - 1) / ACC_ROWS;                  // accumulating CTAs of a KV head
     const int n_rows = a.problems * a.R;
-    const int col_blocks = a.hd % 64 || n_rows > KV_SMS ? 1 : a.hd / 64;
-    return launch_pdl(k_cache_combine, dim3((unsigned)(n_rows * col_blocks + (a.logits ? a.n_kv * per : 0))), CB, 0, s, a,
-                      cache_tile_dims(a.hd), col_blocks, per);
+    const int col_shift = a.hd % 64 || n_rows > KV_SMS || a.hd == 192 ? 0 : a.hd / 128;     // blocks of 64 dims
+    const int v4 = a.hd / 4 >> col_shift;
+    const unsigned v4_inv = (65536 + v4 - 1) / v4;     // exact for x <= 256: x * (v4 - 1) < 65536
+    return launch_pdl(k_cache_combine, dim3((a.R << col_shift) + (a.logits ? per : 0), a.problems), CB, 0, s, a,
+                      cache_tile_dims(a.hd), col_shift, v4, v4_inv);
 }
 
 }  // namespace hoard
