@@ -72,11 +72,9 @@ def tree_visibility(parents):
 
 
 def _ints(*values):
-    """The values, if C's int holds them (ctypes would cut them off)."""
-    for v in values:
-        if not -2**31 <= v < 2**31:
-            raise ValueError(f"{v} is not an int of 32 bits")
-    return values
+    """Refuses what C's int does not hold (ctypes would cut it off)."""
+    if min(values) < -2**31 or max(values) >= 2**31:
+        raise ValueError(f"{values} are not all ints of 32 bits")
 
 
 class CacheOps:
@@ -201,7 +199,7 @@ class CacheOps:
         bounds [n_head_kv][max_rows // block][2][head_dim]; row1_dev (int32 [1]): those of row *row1_dev alone."""
         self._caches(k_cache)
         p = self._bounds(bounds)
-        row0, row1 = _ints(row0, row1)
+        _ints(row0, row1)
         d = None if row1_dev is None else self._contiguous(row1_dev, (1,), torch.int32, "row1_dev")
         self._run(_kv().hoard_kv_block_bounds, stream, self._dp, k_cache.data_ptr(), p, row0, row1, d)
         return bounds
@@ -219,7 +217,7 @@ class CacheOps:
         if given, receives the chosen blocks, ascending, then -1."""
         bp = self._bounds(bounds)
         out = self._query(q, k_cache, v_cache, n_past, vis, gate, out, n_past_dev, stream)
-        n_sink, n_local, n_sel = _ints(n_sink, n_local, n_sel)
+        _ints(n_sink, n_local, n_sel)
         sp = None if sel_out is None else self._contiguous(sel_out, (q.shape[0], self.n_head_kv, n_sel), torch.int32,
                                                            "sel_out")
         self._run(_kv().hoard_kv_block_attention, stream, self._dp, self._qp, bp, n_sink, n_local, n_sel, sp, self._wsp)
@@ -232,7 +230,7 @@ class CacheOps:
         n_sink or from recent_from on, then those of the largest acc. acc, row_pos: [n_head_kv][max_rows]; updated in
         place, or written to acc_out / pos_out."""
         self._caches(k_cache, v_cache)
-        n_rows, n_keep, n_sink, recent_from = _ints(n_rows, n_keep, n_sink, recent_from)
+        _ints(n_rows, n_keep, n_sink, recent_from)
         shape = (self.n_head_kv, self.max_rows)
         ap = self._contiguous(acc, shape, torch.float32, "acc")
         pp = self._contiguous(row_pos, shape, torch.int32, "row_pos")
@@ -245,7 +243,7 @@ class CacheOps:
         """hoard_kv_take: rows row0 + path[i] to rows row0 + i (path ascending): the accepted path of a drafted tree."""
         self._caches(k_cache, v_cache)
         n = len(path)
-        row0, *path = _ints(row0, *path)
+        _ints(row0, *path)
         self._run(_kv().hoard_kv_take, stream, self._dp, k_cache.data_ptr(), v_cache.data_ptr(), row0,
                   (ctypes.c_int32 * max(1, n))(*path), n)
 
@@ -254,7 +252,8 @@ class CacheOps:
               row_pos=None, stream=None):
         """hoard_kv_store: QK norm and RoPE of m tokens' q [m][n_head][head_dim] and k, at positions pos (int32 [m]), and
         their k, v [m][n_head_kv][head_dim] into cache rows row0.. (row0_dev: in device memory). Returns the rotated q."""
-        m, row0, mode = _ints(q.shape[0], row0, mode)
+        m = q.shape[0]
+        _ints(row0, mode)
         shape, kshape = (m, self.n_head, self.head_dim), (m, self.n_head_kv, self.head_dim)
         qs = self._heads(q, shape, "q")
         self._caches(k_cache, v_cache)
