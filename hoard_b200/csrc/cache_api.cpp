@@ -138,6 +138,18 @@ CacheAttn attn_of(const hoard_kv_desc* d, const hoard_kv_query* a) {
 int chunks_of(const CacheAttn& c, int64_t past_rows) {
     return (int)(ceil_div(past_rows, KV_CHUNK) + ceil_div(c.m, KV_CHUNK));
 }
+// A problem is a KV head with the rows of all its tokens, or with a block list one token of it
+void plan_dense(CacheAttn& c) {
+    const int64_t past = c.n_past_dev ? c.max_rows - c.m : c.n_past;
+    c.problems = c.n_kv;
+    c.R = c.m * c.g;
+    cache_plan(c, chunks_of(c, past), past);
+}
+void plan_blocks(CacheAttn& c, int64_t blocks) {
+    c.problems = c.n_kv * c.m;
+    c.R = c.g;
+    cache_plan(c, chunks_of(c, blocks * c.block), blocks * c.block);
+}
 }  // namespace
 
 extern "C" {
@@ -153,8 +165,6 @@ int hoard_kv_attention(const hoard_kv_desc* d, const hoard_kv_query* a, float* a
     const Ws w = ws_plan(d);
     char* b = static_cast<char*>(ws);
     CacheAttn c = attn_of(d, a);
-    c.problems = c.n_kv;
-    c.R = c.m * c.g;
     c.part_o = reinterpret_cast<float*>(b + w.part_o);
     c.part_ml = reinterpret_cast<float2*>(b + w.part_ml);
     if (acc) {
@@ -162,8 +172,7 @@ int hoard_kv_attention(const hoard_kv_desc* d, const hoard_kv_query* a, float* a
         c.logits = reinterpret_cast<float*>(b + w.logits);
         c.logits_ld = w.logits_ld;
     }
-    const int64_t past = c.n_past_dev ? c.max_rows - c.m : c.n_past;
-    cache_plan(c, chunks_of(c, past), past);
+    plan_dense(c);
     return st(launch_cache_attention(c, (cudaStream_t)stream));
 }
 
@@ -241,8 +250,6 @@ int hoard_kv_block_attention(const hoard_kv_desc* d, const hoard_kv_query* a, co
     s.sel_out = sel_out;
     int rc = st(launch_cache_select(s, (cudaStream_t)stream));
     if (rc != HOARD_OK) return rc;
-    c.problems = c.n_kv * c.m;
-    c.R = c.g;
     c.part_o = reinterpret_cast<float*>(b + w.part_o);
     c.part_ml = reinterpret_cast<float2*>(b + w.part_ml);
     c.list = s.list;
@@ -251,7 +258,7 @@ int hoard_kv_block_attention(const hoard_kv_desc* d, const hoard_kv_query* a, co
     c.block = d->block;
     int64_t blocks = (int64_t)s.n_sink + s.n_local + n_sel;
     if (blocks > nb_most) blocks = nb_most;
-    cache_plan(c, chunks_of(c, blocks * d->block), blocks * d->block);
+    plan_blocks(c, blocks);
     return st(launch_cache_attention(c, (cudaStream_t)stream));
 }
 
@@ -288,5 +295,26 @@ int hoard_kv_store(const hoard_kv_desc* d, const float* q, int64_t q_token_strid
                                             freq_base, q_out, k_cache, v_cache, row_stride(d), head_stride(d),
                                             d->kv_type == HOARD_TYPE_BF16, acc, row_pos, (cudaStream_t)stream));
 }
+
+int hoard_kv_attention_form(const hoard_kv_desc* d, int m, int n_past, int n_blocks, int acc, int32_t* form) {
+    if (!desc_ok(d) || !form || m < 1 || m > d->max_tokens || n_past < 0 || n_past > d->max_rows - m) return HOARD_EINVAL;
+    hoard_kv_query a{};
+    a.m = m;
+    a.n_past = n_past;
+    CacheAttn c = attn_of(d, &a);
+    // what is not null says what the call does; nothing is read
+    if (acc) c.logits = reinterpret_cast<float*>(form);
+    if (n_blocks >= 0) c.list = form;
+    c.block = d->block;
+    if (n_blocks >= 0) plan_blocks(c, n_blocks);
+    else plan_dense(c);
+    form[0] = c.tc_splits != 0;
+    form[1] = c.tile_rows;
+    form[2] = c.splits;
+    form[3] = !c.tc_splits && c.cluster;
+    return HOARD_OK;
+}
+
+int hoard_kv_choose_form(int n_cand, int problems) { return choose_form(n_cand, problems); }
 
 }  // extern "C"

@@ -115,6 +115,9 @@ struct CacheSelect {
     int list_cap;
 };
 cudaError_t launch_cache_select(const CacheSelect& c, cudaStream_t s);
+// who chooses among n_cand candidates of each of `problems` problems: one CTA; one CTA, the keys formed by a cluster; a cluster
+enum ChooseForm { CHOOSE_ONE, CHOOSE_GATHER, CHOOSE_CLUSTER };
+ChooseForm choose_form(int n_cand, int problems);
 
 struct TakePath {
     int32_t row[64];
@@ -123,3 +126,10 @@ cudaError_t launch_cache_take(void* kc, void* vc, int64_t rs, int64_t hs, int n_
                               const TakePath& path, int n, cudaStream_t s);
 
 }  // namespace hoard
+
+// The form that a call runs, for tests and measurements, by the rules the calls themselves go by (cache_api.cpp).
+// form: {1 where the tensor-core kernel runs, query rows of a tile, splits, 1 where a cluster (or one CTA) joins them}.
+// n_blocks: blocks that each problem of hoard_kv_block_attention attends, -1 for hoard_kv_attention; acc: weights accumulated
+struct hoard_kv_desc;
+extern "C" int hoard_kv_attention_form(const hoard_kv_desc* d, int m, int n_past, int n_blocks, int acc, int32_t* form);
+extern "C" int hoard_kv_choose_form(int n_cand, int problems);

@@ -832,6 +832,11 @@ cudaError_t launch_cache_bounds(const void* kc, int64_t rs, int64_t hs, bool bf1
                       row0, row1, row1_dev, (uint16_t*)bounds);
 }
 
+ChooseForm choose_form(int n_cand, int problems) {
+    if (n_cand > BS_ONE) return CHOOSE_CLUSTER;
+    return n_cand <= BS_ALONE + BS_MORE * (int64_t)problems || problems * (int64_t)CL > KV_SMS ? CHOOSE_ONE : CHOOSE_GATHER;
+}
+
 cudaError_t launch_cache_select(const CacheSelect& asked, cudaStream_t s) {
     CacheSelect c = asked;
     c.block_shift = __builtin_ctz(c.block);
@@ -848,14 +853,15 @@ cudaError_t launch_cache_select(const CacheSelect& asked, cudaStream_t s) {
         e = launch_pdl(fn, grid, 32 * SC_WARPS * parts, 0, s, c, nb_cap);
         if (e != cudaSuccess) return e;
     }
-    if (n_cand <= BS_ONE && (n_cand <= BS_ALONE + BS_MORE * c.n_kv * c.m || c.n_kv * c.m * CL > KV_SMS)) {
+    const ChooseForm form = choose_form(n_cand, c.n_kv * c.m);
+    if (form == CHOOSE_ONE) {
         static SmemLimit limit;
         e = limit.raise((const void*)k_block_choose<1, false>, BS_ONE * 8);
         if (e != cudaSuccess) return e;
         return launch_pdl(k_block_choose<1, false>, dim3(1, c.n_kv, c.m), SEL_THREADS, (size_t)n_cand * 8, s, c, nb_cap);
     }
     const dim3 grid(CL, c.n_kv, c.m);
-    if (n_cand <= BS_ONE) {
+    if (form == CHOOSE_GATHER) {
         static SmemLimit limit;
         e = limit.raise((const void*)k_block_choose<CL, true>, BS_ONE * 8);
         if (e != cudaSuccess) return e;
