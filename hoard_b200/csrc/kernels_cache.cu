@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(Plan<HD, NT>::W * 32, 1) k_cache_attention(con
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] *= sc[n][i & 1];
+            for (int i = 0; i < 4; ++i) s[n][i] = __fmul_rn(s[n][i], sc[n][i & 1]);      // a score: rounded once, nowhere fused
         if (left < KV_CHUNK || own) {
             const int sh = own ? row0 - n_past : 0;
 #pragma unroll
@@ -318,9 +318,9 @@ __global__ void __launch_bounds__(Plan<HD, NT>::W * 32, 1) k_cache_attention(con
         for (int n = 0; n < NT; ++n) {
             float b[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) b[i] = mx[n][i] == -INFINITY ? 0.f : mx[n][i] - Terms<KT>::P_EXP;
+            for (int i = 0; i < 2; ++i) b[i] = mx[n][i] == -INFINITY ? 0.f : mx[n][i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = ex2f(s[n][i] - b[i & 1]);
+            for (int i = 0; i < 4; ++i) s[n][i] = weight<KT>(s[n][i], b[i & 1]);
             tot[n][0] += s[n][0] + s[n][2];
             tot[n][1] += s[n][1] + s[n][3];
         }
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(Plan<HD, NT>::W * 32, 1) k_cache_attention(con
             for (int r = 0; r < RT; ++r) lv[r] = r < a.R ? lg[(int64_t)r * a.logits_ld + j] : -INFINITY;
 #pragma unroll
             for (int r = 0; r < RT; ++r)
-                if (r < a.R && s_inv[r] != 0.f) w += ex2f(lv[r] - (s_top[r] - Terms<KT>::P_EXP)) * s_inv[r];
+                if (r < a.R && s_inv[r] != 0.f) w += weight<KT>(lv[r], s_top[r]) * s_inv[r];
             acc[j] = before + w;
         }
     }
@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(CB) k_cache_combine(const CacheAttn a, int hdt
         for (int k = 0; k < 4; ++k)
             if (r0 + k < a.R && s_ir[r0 + k] != 0.f)
 #pragma unroll
-                for (int i = 0; i < ACC_PER; ++i) sum[i] += ex2f(s[k][i] - (s_mr[r0 + k] - pe)) * s_ir[r0 + k];
+                for (int i = 0; i < ACC_PER; ++i) sum[i] += ex2f((s[k][i] - s_mr[r0 + k]) + pe) * s_ir[r0 + k];
     }
 #pragma unroll
     for (int i = 0; i < ACC_PER; ++i)

@@ -35,6 +35,7 @@ namespace {
 
 constexpr int TM = 128, TK = 64;                       // query rows, keys of a tile
 constexpr int TC_THREADS = 384, LOADERS = 96, GROUP = 128;
+constexpr float LARGE_SCORE = 1 << 20;                 // steps of f32 up to there: 2^-4
 constexpr int Q_PAD = 4;                               // floats added to a staged q row: rows start in other banks
 
 __device__ __forceinline__ bool wait_or_give_up(uint64_t* bar, unsigned parity, volatile int* give_up) {
@@ -395,9 +396,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < TK; ++i) top = fmaxf(top, __uint_as_float(sr[i]));
-            top = fmaxf(mx, top * sc);
+            top = fmaxf(mx, __fmul_rn(top, sc));
             const float f = top > mx ? ex2f(mx - top) : 1.f;
-            const float b = Terms<KT>::P_EXP - (top == -INFINITY ? 0.f : top);
+            // weights 2^(s sc - top + P_EXP), their exponents by one multiply-add each. Where the roundings of s sc and of top
+            // may come to more than 2^-4, in the order that makes the largest weight 2^P_EXP exactly
+            const float base = top == -INFINITY ? 0.f : top;
+            if (__any_sync(0xffffffffu, fabsf(base) > LARGE_SCORE)) {
+#pragma unroll
+                for (int i = 0; i < TK; ++i)
+                    sr[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(sr[i]), sc), base) + Terms<KT>::P_EXP);
+            } else {
+                const float b = Terms<KT>::P_EXP - base;
+#pragma unroll
+                for (int i = 0; i < TK; ++i) sr[i] = __float_as_uint(fmaf(__uint_as_float(sr[i]), sc, b));
+            }
             mx = top;
             float sum = 0.f;
 #pragma unroll
@@ -405,8 +417,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
                 uint32_t w[TN][16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float p0 = ex2f(fmaf(__uint_as_float(sr[32 * h + 2 * i]), sc, b));
-                    float p1 = ex2f(fmaf(__uint_as_float(sr[32 * h + 2 * i + 1]), sc, b));
+                    float p0 = ex2f(__uint_as_float(sr[32 * h + 2 * i]));
+                    float p1 = ex2f(__uint_as_float(sr[32 * h + 2 * i + 1]));
                     sum += p0 + p1;
 #pragma unroll
                     for (int u = 0; u < TN; ++u) w[u][i] = take_term<KT>(p0, p1);

@@ -80,4 +80,11 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
+// The weight of a score beside the largest one, times 2^P_EXP. The difference is formed first: top - P_EXP rounded at scores of
+// 2^24 and more makes the largest weight 2^16, which is no f16.
+template <typename KT> __device__ __forceinline__ float weight(float s, float top) {
+    if constexpr (Terms<KT>::P_EXP == 0.f) return ex2f(s - top);
+    else return ex2f((s - top) + Terms<KT>::P_EXP);
+}
+
 }  // namespace hoard
