@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(Plan<HD, NT>::W * 32, 1) k_cache_attention(con
         bool bad = false;
 #pragma unroll
         for (int k = 0; k < HD / 32; ++k) {
-            bad |= !(fabsf(x[i][k]) <= 3.4e38f);
+            bad |= !(fabsf(x[i][k]) < INFINITY);
             am = fmaxf(am, fabsf(x[i][k]));
         }
         am = warp_max(am);

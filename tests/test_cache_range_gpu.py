@@ -53,3 +53,20 @@ def test_large_scores_accumulated(n_head, n_kv, hd, m, n_past, kt, sign):
     out = ops.tree_attention(q, k, v, n_past, acc=acc)
     want, add = ref.attention(q, k, v, n_past)
     assert rel(out, want) < TOL and rel(acc, add) < TOL
+
+
+@shapes
+@pytest.mark.parametrize("kt", [F16, BF16])
+@pytest.mark.parametrize("size", [3.4028234663852886e38, 3.401e38])
+def test_queries_of_the_largest_float(s, kt, size):
+    """Up to the largest float itself a query is finite. Its other dims are 0 and keys have levels there, so that equal scores
+    share the weight."""
+    m, n_past, n = s["m"], s["n_past"], s["n_past"] + s["m"]
+    assert kernel_of(s, kt) == s["kernel"]
+    _, k, v, r = case(s["n_head"], s["n_kv"], s["hd"], kt, n, m)
+    k[:, :, 0] = torch.randint(1, 6, (n, s["n_kv"]), device=DEV).to(kt) * 2.0**-24
+    q = torch.zeros(m, s["n_head"], s["hd"], device=DEV)
+    q[:, :, 0] = size * torch.sign(r(m, s["n_head"]))
+    ops = cache.CacheOps(n_head=s["n_head"], n_head_kv=s["n_kv"], head_dim=s["hd"], kv_dtype=kt, max_rows=n, max_tokens=m)
+    out = ops.tree_attention(q, k, v, n_past)
+    assert rel(out, attention64(q, k, v, n_past)) < TOL
