@@ -2,7 +2,9 @@
 //
 // Two f16 terms hold 22 bits of a value, three bf16 terms 24. For f16 the rows of q are scaled by a power of two to
 // [2^13, 2^14) and softmax weights by 2^14, which keeps the terms out of f16's subnormal range; the factors are taken
-// out of the scores (exactly) and cancel between the weighted sum and the total.
+// out of the scores (exactly) and cancel between the weighted sum and the total. bf16 has f32's range, so that rows scaled
+// up could overflow beside large keys: only those below 2^-64 are, to there (their last terms would be subnormal; products with
+// any key stay below 2^65), and those from 2^126 on are scaled below it (rounded to bf16 they could be infinite).
 #pragma once
 #include "common.cuh"
 
@@ -10,12 +12,12 @@ namespace hoard {
 
 template <typename KT> struct Terms;
 template <> struct Terms<__half> {
-    static constexpr int N = 2, Q_EXP = 13;
+    static constexpr int N = 2, Q_MIN = 13, Q_MAX = 13;
     static constexpr float P_EXP = 14.f;
     static constexpr uint32_t INF2 = 0x7C007C00u;        // exponent bits of two values
 };
 template <> struct Terms<__nv_bfloat16> {
-    static constexpr int N = 3, Q_EXP = 0;
+    static constexpr int N = 3, Q_MIN = -64, Q_MAX = 125;
     static constexpr float P_EXP = 0.f;
     static constexpr uint32_t INF2 = 0x7F807F80u;
 };
@@ -47,16 +49,15 @@ template <typename KT> __device__ __forceinline__ bool odd_pair(uint32_t w) {
     return (e & 0xFFFFu) == (Terms<KT>::INF2 & 0xFFFFu) || (e >> 16) == (Terms<KT>::INF2 >> 16);
 }
 
-// The power of two that brings a row with largest magnitude am (2^e <= am < 2^(e + 1)) to exponent Q_EXP (e kept where
-// the powers are normal numbers), and its inverse. Rows of zeros, and rows with infinities or NaN (bad), are left as they are.
+// The power of two that brings a row with largest magnitude am (2^e <= am < 2^(e + 1)) to an exponent of Q_MIN .. Q_MAX, and
+// its inverse (both normal numbers: 2^113 at most). Rows of zeros, and rows with infinities or NaN (bad), are left as they are.
 struct RowScale {
     float up, down;
 };
 template <typename KT> __device__ __forceinline__ RowScale row_scale(float am, bool bad) {
-    int e = (int)(__float_as_uint(am) >> 23) - 127;
-    e = bad || am == 0.f ? Terms<KT>::Q_EXP : min(max(e, -100), 126);
-    return {__uint_as_float((uint32_t)(127 + Terms<KT>::Q_EXP - e) << 23),
-            __uint_as_float((uint32_t)(127 - Terms<KT>::Q_EXP + e) << 23)};
+    const int e = (int)(__float_as_uint(am) >> 23) - 127;
+    const int by = bad || am == 0.f ? 0 : min(min(max(e, Terms<KT>::Q_MIN), Terms<KT>::Q_MAX) - e, 113);
+    return {__uint_as_float((uint32_t)(127 + by) << 23), __uint_as_float((uint32_t)(127 - by) << 23)};
 }
 // n things in `parts` shares that differ by one at most: the first of share i (one 32-bit division, before the first load)
 struct Share {

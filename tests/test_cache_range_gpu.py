@@ -70,3 +70,17 @@ def test_queries_of_the_largest_float(s, kt, size):
     ops = cache.CacheOps(n_head=s["n_head"], n_head_kv=s["n_kv"], head_dim=s["hd"], kv_dtype=kt, max_rows=n, max_tokens=m)
     out = ops.tree_attention(q, k, v, n_past)
     assert rel(out, attention64(q, k, v, n_past)) < TOL
+
+
+@shapes
+@pytest.mark.parametrize("down,up", [(-100, 127), (-60, 127), (-5, 127), (-140, 127), (100, -100), (124, -120)])
+def test_small_queries_beside_large_keys(s, down, up):
+    """bf16 has f32's range: scores of ordinary size from queries and keys of opposite extremes (q of 2^-140 is subnormal in f32)."""
+    assert kernel_of(s, BF16) == s["kernel"]
+    m, n_past, n = s["m"], s["n_past"], s["n_past"] + s["m"]
+    q, k, v, _ = case(s["n_head"], s["n_kv"], s["hd"], BF16, n, m)
+    q, k = q * 2.0**down, (k.float() * 2.0**up).clamp(-3.3e38, 3.3e38).to(BF16)
+    scale = 2.0 ** -(down + up) / s["hd"] ** 0.5
+    ops = cache.CacheOps(n_head=s["n_head"], n_head_kv=s["n_kv"], head_dim=s["hd"], kv_dtype=BF16, max_rows=n, max_tokens=m,
+                         scale=scale)
+    assert rel(ops.tree_attention(q, k, v, n_past), attention64(q, k, v, n_past, scale=scale)) < TOL
