@@ -338,7 +338,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
         named_sync(2, 2 * GROUP);
         const float am = fmaxf(s_mx[0][row], s_mx[1][row]);
         const RowScale rs = row_scale<KT>(am, am == INFINITY);
-        const float sc = a.scale_log2 * rs.down;
+        // a factor that vanishes (a tiny scale beside a row that was scaled up) must not make NaN of a masked -inf; scores vanish
+        // as well with the least normal number
+        const float sc = fmaxf(a.scale_log2 * rs.down, rs.down < 1.f ? 1.17549435e-38f : 0.f);
 #pragma unroll
         for (int h = 0; h < HALF; h += 32) {           // 32 dims are 16 columns
             uint32_t w[TN][16];

@@ -84,3 +84,16 @@ def test_small_queries_beside_large_keys(s, down, up):
     ops = cache.CacheOps(n_head=s["n_head"], n_head_kv=s["n_kv"], head_dim=s["hd"], kv_dtype=BF16, max_rows=n, max_tokens=m,
                          scale=scale)
     assert rel(ops.tree_attention(q, k, v, n_past), attention64(q, k, v, n_past, scale=scale)) < TOL
+
+
+@shapes
+@pytest.mark.parametrize("kt", [F16, BF16])
+def test_scores_that_vanish(s, kt):
+    """A scale and queries so small that their product is 0 in f32: equal weights for the rows that are seen, none for the others."""
+    assert kernel_of(s, kt) == s["kernel"]
+    m, n_past, n = s["m"], s["n_past"], s["n_past"] + s["m"]
+    q, k, v, _ = case(s["n_head"], s["n_kv"], s["hd"], kt, n, m)
+    ops = cache.CacheOps(n_head=s["n_head"], n_head_kv=s["n_kv"], head_dim=s["hd"], kv_dtype=kt, max_rows=n, max_tokens=m, scale=1e-30)
+    vis, _ = tree(m, 6)
+    q = q * (1e-30 if kt is F16 else 1e-37)
+    assert rel(ops.tree_attention(q, k, v, n_past, vis=vis), attention64(q, k, v, n_past, vis, scale=1e-30)) < TOL
