@@ -51,6 +51,10 @@ class BlockChoice:
     n_local: int = 4
     n_sel: int = 32
 
+    def leaves_out(self, rows: int) -> bool:
+        """Whether a past of up to `rows` rows can have blocks that a token does not attend."""
+        return self.n_sink + self.n_local + self.n_sel < -(-rows // self.block)
+
 
 @dataclass
 class CacheBudget:
@@ -713,7 +717,9 @@ class DecodeModel:
         drafted token that token i follows (an earlier index), or -1 for the last past token. Token i takes position
         base + its depth, its k and v cache row base + i; it attends to the past, its ancestors and itself. The layers'
         attention is one call for all tokens, and so are the MoE layers (T = m). Returns the logits [m][vocab]; row i
-        predicts what follows token i. With parents = [-1, 0, 1, ..] it is forward_batch."""
+        predicts what follows token i. With parents = [-1, 0, 1, ..] it is forward_batch, but for the order of the attention's
+        sums. With `blocks` every token attends the blocks that are chosen for a past of `base` rows, its ancestors and itself:
+        where blocks are left out that is not forward_batch's or the step's choice, which goes by the token's own position."""
         if stream is not None:                   # the tensors made here belong to the stream that uses them
             with torch.cuda.stream(torch.cuda.ExternalStream(_stream(stream), device=self.dev)):
                 return self.forward_tree(tokens, parents, base)
@@ -789,14 +795,19 @@ class DecodeModel:
     def tree_generate(self, prompt, n_gen: int, depth: int = 4, width: int = 2):
         """speculative_generate with a tree: at each of `depth` levels the draft (this model at its top-1 expert) offers its
         `width` best tokens and goes on from the best; one forward_tree verifies all of them, the longest path that the
-        full model agrees with is accepted, then the corrected token runs. Greedy and lossless. Returns (tokens,
-        {"rounds", "proposed", "accepted"})."""
+        full model agrees with is accepted, then the corrected token runs. Greedy; the tokens are generate()'s wherever the
+        model's best two logits differ by more than the order of f32 sums moves them (verification sums in another order).
+        With `blocks` only where they hold the whole sequence (see forward_tree). Returns (tokens, {"rounds", "proposed",
+        "accepted"})."""
         T, k_full = len(prompt), self.cfg.n_expert_used
         if self.budget or self.cfg.full_attn_interval > 0:
             raise ValueError("a tree of drafts needs a cache whose rows are positions, and no delta-net state")
         if (T < 1 or depth < 1 or width < 1 or depth * width > self.max_batch
                 or T + n_gen + depth * width + 1 > self.max_ctx):
             raise ValueError("prompt + n_gen + the tree must fit max_ctx, depth * width <= max_batch")
+        if self.blocks and self.blocks.leaves_out(T + n_gen + depth):
+            raise ValueError("a tree of drafts attends the blocks chosen for the past before it: its tokens are generate()'s only "
+                             "where n_sink + n_local + n_sel blocks hold the whole sequence")
         self.seq[:T].copy_(torch.tensor(prompt, dtype=torch.int32))
         self.reset_state()
         for p in range(T):
