@@ -1,11 +1,14 @@
-"""The decode driver's use of the cache operators, beside test_cache_model_gpu.py: what a tree attends where blocks are left out."""
+"""The decode driver's use of the cache operators, beside test_cache_model_gpu.py: what a tree attends where blocks are left out,
+trees whose drafts are accepted, generated tokens against the plain model's logits after any near tie."""
+import dataclasses
+
 import pytest
 import torch
 
 from hoard_b200 import harness as hx
 from tests import cache_ref as ref
 from tests.test_cache_gpu import TOL, rel
-from tests.test_cache_model_gpu import OLMOE_S, QWEN_S, prompt_of
+from tests.test_cache_model_gpu import GAP, OLMOE_S, QWEN_S, prompt_of
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +21,15 @@ def weights():
 
 def make(cfg, weights, **kw):
     return hx.DecodeModel(cfg, weights[cfg.arch], device=0, **kw)
+
+
+def assert_greedy(cfg, weights, prompt, tokens, **kw):
+    """Every generated token is the plain model's best after those before it, or within GAP of it."""
+    m = make(cfg, weights, max_ctx=len(prompt) + len(tokens) + 8, **kw)
+    logits = m.score(prompt + tokens, len(prompt))
+    m.close()
+    got = logits.gather(1, torch.tensor(tokens, device=logits.device)[:, None])[:, 0]
+    assert float((logits.amax(1) - got).max()) < GAP
 
 
 @pytest.mark.parametrize("cfg", [QWEN_S, OLMOE_S])
@@ -45,3 +57,28 @@ def test_forward_tree_over_few_blocks(cfg, weights):
         assert all(len(c) == 1 and c[0] in (0, 1) for t in chosen for c in t) and not seen.all()
         assert rel(out, ref.attention(q, k, v, base, vis, past_seen=seen)[0]) < TOL
     m.close()
+
+
+@pytest.mark.parametrize("cfg", [QWEN_S, OLMOE_S])
+@pytest.mark.parametrize("depth,width", [(4, 3), (1, 8)])
+def test_trees_of_the_model_itself_are_accepted(cfg, depth, width, weights):
+    """With one expert the draft is the full model: its best path is accepted, and the rows that are taken over serve every
+    later round."""
+    cfg, n_gen = dataclasses.replace(cfg, n_expert_used=1), 40
+    prompt = prompt_of(cfg, 33)
+    m = make(cfg, weights, max_ctx=160)
+    got, stats = m.tree_generate(prompt, n_gen, depth=depth, width=width)
+    m.close()
+    assert len(got) == n_gen and stats["accepted"] >= 0.8 * depth * stats["rounds"]
+    assert stats["rounds"] < n_gen / (1 + 0.7 * depth) + 1
+    assert_greedy(cfg, weights, prompt, got)
+
+
+@pytest.mark.parametrize("cfg", [QWEN_S, OLMOE_S])
+def test_tree_generate_is_greedy(cfg, weights):
+    prompt, n_gen = prompt_of(cfg, 33), 40
+    for kw in (dict(), dict(blocks=hx.BlockChoice(block=16, n_sink=1, n_local=1, n_sel=20))):
+        m = make(cfg, weights, max_ctx=160, **kw)
+        got, _ = m.tree_generate(prompt, n_gen, depth=3, width=4)
+        m.close()
+        assert_greedy(cfg, weights, prompt, got)
