@@ -6,7 +6,9 @@ names and take torch CUDA tensors. Caches are [max_rows][n_head_kv][head_dim] te
 head strides that are multiples of 8 elements (a [n_head_kv][max_rows][head_dim] buffer passes as its transpose).
 Wrong tensors raise ValueError, refused arguments HoardError; nothing is launched then. One CacheOps is driven by one
 host thread at a time, and its calls share one workspace: calls on streams that may overlap, captured graphs among
-them, need a CacheOps each. A result that a call allocates belongs to the stream of the call; `out` may be `q` itself.
+them, need a CacheOps each. A CacheOps may be dropped while calls on any stream run (its workspace is given back when they have
+completed), but not before a graph that captured its calls, and a stream that is not torch's own has to outlive it.
+A result that a call allocates belongs to the stream of the call; `out` may be `q` itself.
 """
 from __future__ import annotations
 
@@ -105,6 +107,8 @@ class CacheOps:
         self.device = torch.cuda.current_device() if device is None else device
         self._ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", self.device))
         self._wsp = ctypes.c_void_p(self._ws.data_ptr())
+        # the workspace belongs to the stream that is current now; the others that calls ran on
+        self._home, self._streams = _raw_stream(self.device), set()
 
     # ---- plumbing ----
     # The checks read each attribute of a tensor once: at the sizes of a decode step they are a good part of a call.
@@ -113,7 +117,11 @@ class CacheOps:
         if _current_device() != self.device:
             with torch.cuda.device(self.device):
                 return self._run(fn, stream, *args)
-        rc = fn(*args, _raw_stream(self.device) if stream is None else getattr(stream, "cuda_stream", stream))
+        raw = _raw_stream(self.device) if stream is None else getattr(stream, "cuda_stream", stream)
+        if raw != self._home and raw not in self._streams:
+            self._ws.record_stream(torch.cuda.ExternalStream(raw if raw != 1 else 0, device=self._ws.device))      # 1: cudaStreamLegacy
+            self._streams.add(raw)
+        rc = fn(*args, raw)
         if rc != 0:
             raise HoardError(rc, f"{fn.__name__} failed ({lib().hoard_strerror(rc).decode()})")
 

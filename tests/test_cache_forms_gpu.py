@@ -163,3 +163,28 @@ def test_block_choice_of_each_form(n_cand, n_head, n_kv, hd, m, block, kt, form,
     for h in some:
         want, _ = ref.attention(q[:, h:h + 1], k[:, h // g:h // g + 1], v[:, h // g:h // g + 1], n_past, past_seen=seen[:, h // g:h // g + 1])
         assert rel(out[:, h:h + 1], want) < TOL
+
+
+@pytest.mark.parametrize("given", ["stream", "handle", "current"])
+def test_workspace_of_a_running_call_is_not_given_away(given):
+    """A CacheOps that is dropped while its call on another stream waits: its workspace is nobody else's before that is done."""
+    q, k, v, _ = case(8, 2, 128, F16, 600, 20)
+    ops = cache.CacheOps(n_head=8, n_head_kv=2, head_dim=128, kv_dtype=F16, max_rows=600, max_tokens=20)
+    want = ops.tree_attention(q, k, v, 580)
+    out = torch.empty_like(want)
+    at, size = ops._ws.data_ptr(), ops._ws.numel()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)                   # about 0.2 s, after which the call runs
+        if given == "current":
+            ops.tree_attention(q, k, v, 580, out=out)
+    if given != "current":
+        ops.tree_attention(q, k, v, 580, out=out, stream=side if given == "stream" else side.cuda_stream)
+    del ops
+    held = [torch.empty(size, dtype=torch.uint8, device=DEV) for _ in range(3)]
+    busy = not side.query()
+    assert busy and at not in [x.data_ptr() for x in held]
+    side.synchronize()
+    assert torch.equal(out, want)
+    del held
