@@ -21,8 +21,9 @@ decode kernel).
 Beside the plain step there are three forms of the attention over the cache (hoard_b200/cache.py):
 `tree_generate` verifies a tree of drafted tokens in one forward (`forward_tree`); `blocks=BlockChoice(..)` lets every
 token attend the first, the last and the best-scoring blocks of a long cache; `budget=CacheBudget(..)` keeps a bounded
-number of cache rows per KV head, evicting the positions with the least accumulated attention weight. Contexts too long
-for the one-CTA-per-head attention's shared memory run through the split attention of the same module."""
+number of cache rows per KV head, evicting the positions with the least accumulated attention weight. Positions beyond
+what the one-CTA-per-head attention holds in shared memory (and captured steps of contexts beyond it) run through the split
+attention of the same module."""
 from __future__ import annotations
 
 import ctypes
@@ -39,7 +40,6 @@ Q4_K, Q6_K, F32 = quant.Q4_K, quant.Q6_K, 0
 KV_TYPES = {torch.float16: 1, torch.bfloat16: 30}     # KV cache element -> HOARD_TYPE_F16 / HOARD_TYPE_BF16
 MAX_BATCH = 16          # tokens of one batched (verify) forward
 QK_MODE = {"": 0, "full": 1, "head": 2}
-LONG_CTX = 46000        # cached positions beyond which hoard_hx_attention's scores do not fit in shared memory
 
 
 @dataclass
@@ -68,6 +68,15 @@ class CacheBudget:
     @property
     def rows(self) -> int:
         return self.n_keep + self.n_slack
+
+
+def plain_attention_rows(head_dim: int) -> int:
+    """Most positions that hoard_hx_attention takes: their scores share 200 KiB of shared memory with q and the partial sums of
+    its 512 threads (256 where rows are no multiple of 16 bytes). 0: it does not take the head_dim."""
+    if head_dim < 1 or 256 % head_dim:
+        return 0
+    groups = 512 // (head_dim // 8) if head_dim % 8 == 0 else 256 // head_dim
+    return 200 * 1024 // 4 - head_dim - groups * head_dim
 
 
 def _iarr(vals):
@@ -365,10 +374,17 @@ class DecodeModel:
         self.n_cache = budget.rows if budget else max_ctx         # rows of a layer's cache
         self.kc = torch.zeros(max(1, n_full), self.n_cache, self.nkv, dtype=kv_dtype, device=dev)
         self.vc = torch.zeros_like(self.kc)
-        # the split attention: long contexts, blocks, budgets, and (made when first used) trees
+        # the split attention: blocks, budgets, positions beyond the one-CTA attention's, and (made when first used) trees
         self._ops_args = dict(n_head=cfg.n_head, n_head_kv=cfg.n_head_kv, head_dim=hd, kv_dtype=kv_dtype,
                               max_rows=self.n_cache, block=blocks.block if blocks else 0, device=device)
-        self.ops = cache.CacheOps(**self._ops_args) if blocks or budget or max_ctx > LONG_CTX else None
+        self.plain_rows = plain_attention_rows(hd)
+        self.ops = None
+        if blocks or budget or max_ctx > self.plain_rows:
+            try:
+                self.ops = cache.CacheOps(**self._ops_args)
+            except HoardError:               # a head layout that only the one-CTA attention takes, up to its positions
+                if blocks or budget:
+                    raise
         self._tree_ops = None
         if blocks:
             self.bounds = torch.zeros(max(1, n_full), cfg.n_head_kv, self.n_cache // blocks.block, 2, hd, dtype=kv_dtype,
@@ -477,7 +493,8 @@ class DecodeModel:
                                     out=att.view(1, c.n_head, hd), n_past_dev=row_dev, stream=s)
         else:
             self._store(q, k, v, q_rot, kc, vc, qn, kn, mode, hx, s, pos)
-            if self.ops:
+            # the split attention for blocks, and beyond the positions that the one-CTA attention takes
+            if self.ops and (self.blocks or (self.max_ctx if pos is None else pos + 1) > self.plain_rows):
                 args = dict(gate=self._gate_view(q), out=att.view(1, c.n_head, hd), n_past_dev=pd, stream=s)
                 rot, k3, v3, n = q_rot.view(1, c.n_head, hd), self._heads(kc), self._heads(vc), pos or 0
                 if self.blocks:

@@ -26,3 +26,13 @@ def test_blocks_that_are_left_out():
 def test_tree_generate_refuses_blocks_that_are_left_out(blocks):
     with pytest.raises(ValueError, match="blocks"):
         driver(blocks=blocks).tree_generate(list(range(90)), 4, depth=3, width=2)
+
+
+def test_positions_of_the_one_cta_attention():
+    """One position more than plain_attention_rows says is refused (before anything is launched)."""
+    one = 4096
+    for hd in (8, 16, 64, 128, 256, 4, 2):
+        n = hx.plain_attention_rows(hd)
+        assert n > 40000 and hx._hx().hoard_hx_attention(one, one, one, 4, 2, hd, n + 1, 0.1, one, 1, None) == -1
+    for hd in (0, 96, 80, 512):
+        assert hx.plain_attention_rows(hd) == 0

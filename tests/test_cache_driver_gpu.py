@@ -82,3 +82,54 @@ def test_tree_generate_is_greedy(cfg, weights):
         got, _ = m.tree_generate(prompt, n_gen, depth=3, width=4)
         m.close()
         assert_greedy(cfg, weights, prompt, got)
+
+
+def test_long_contexts_keep_the_plain_attention_where_it_runs(weights):
+    """The same bits whatever max_ctx is: eager steps up to the positions that the one-CTA attention takes, captured ones up to
+    contexts of as many."""
+    cfg, n_gen = QWEN_S, 12
+    prompt = prompt_of(cfg, 40)
+    runs = []
+    for max_ctx in (60, 46976, 60000):
+        m = make(cfg, weights, max_ctx=max_ctx)
+        assert m.plain_rows == 46976
+        logits = torch.empty(n_gen, cfg.n_vocab, device="cuda:0")
+        tokens = m.generate(prompt, n_gen, logits_out=logits)
+        graphed = m.generate_graphed(prompt, n_gen)
+        runs.append((tokens, logits, graphed, m.logits.clone()))
+        m.close()
+    for tokens, logits, graphed, last in runs[1:]:
+        assert tokens == runs[0][0] and torch.equal(logits, runs[0][1])
+    assert runs[1][2] == runs[0][2] and torch.equal(runs[1][3], runs[0][3])
+    assert_greedy(cfg, weights, prompt, runs[2][2])
+
+
+def test_the_step_where_the_plain_attention_ends(weights):
+    cfg = QWEN_S
+    m = make(cfg, weights, max_ctx=47100)
+    m.kc.normal_(std=0.5), m.vc.normal_(std=0.5)
+    m.seq.fill_(11)
+    for pos in (m.plain_rows - 1, m.plain_rows, 47099):
+        m.step(pos, m.scratch_tok)
+        step = m.logits.clone()
+        tree = m.forward_tree([11], [-1], pos)[0]
+        assert torch.isfinite(step).all() and rel(tree, step) < 2e-2, pos
+    m.close()
+
+
+def test_layouts_that_only_the_plain_attention_takes():
+    """More than 64 query heads per KV head: a long context is served up to the positions of the one-CTA attention."""
+    cfg = hx.ModelConfig("qwen3moe", 1, 512, 256, 2, 8, 16, 4, 256, 2048, 1e6, 1e-6, "head", True)
+    tensors, prompt, runs = hx.seeded_tensors(cfg, seed=5, device=torch.device("cuda", 0)), prompt_of(cfg, 20), []
+    for max_ctx in (40, 60000):
+        m = hx.DecodeModel(cfg, tensors, device=0, max_ctx=max_ctx)
+        assert m.ops is None
+        logits = torch.empty(8, cfg.n_vocab, device="cuda:0")
+        runs.append((m.generate(prompt, 8, logits_out=logits), logits))
+        if max_ctx == 60000:
+            with pytest.raises(hx.HoardError):
+                m.step(m.plain_rows, m.scratch_tok)
+        m.close()
+    assert runs[0][0] == runs[1][0] and torch.equal(runs[0][1], runs[1][1])
+    with pytest.raises(hx.HoardError):
+        hx.DecodeModel(cfg, tensors, device=0, max_ctx=200, budget=hx.CacheBudget(64, n_recent=8))
