@@ -750,7 +750,7 @@ class DecodeModel:
         if len(parents) != m or m > self.max_batch or base < 0 or base + m > self.max_ctx:
             raise ValueError("a tree has a parent for each of its 1..max_batch tokens, inside max_ctx")
         if self._tree_ops is None:
-            self._tree_ops = cache.CacheOps(**self._ops_args, max_tokens=self.max_batch, max_acc_tokens=0)
+            self._tree_ops = cache.CacheOps(**self._ops_args, max_tokens=min(self.max_batch, self.max_ctx), max_acc_tokens=0)
             z = lambda *sh: torch.zeros(*sh, dtype=torch.float32, device=self.dev)
             B = self.max_batch
             self._tq, self._tk, self._tv = z(B, self.nqp), z(B, self.nkv), z(B, self.nkv)

@@ -133,3 +133,17 @@ def test_layouts_that_only_the_plain_attention_takes():
     assert runs[0][0] == runs[1][0] and torch.equal(runs[0][1], runs[1][1])
     with pytest.raises(hx.HoardError):
         hx.DecodeModel(cfg, tensors, device=0, max_ctx=200, budget=hx.CacheBudget(64, n_recent=8))
+
+
+def test_trees_in_a_context_shorter_than_the_largest_batch(weights):
+    cfg = OLMOE_S
+    m = make(cfg, weights, max_ctx=8)
+    prompt = prompt_of(cfg, 3)
+    m.generate(prompt, 1)
+    out = m.forward_tree([5, 6, 7, 8, 9], [-1, 0, 0, 2, -1], 3)
+    chain = m.forward_batch([5, 7, 8], 3)
+    for i, j in ((0, 0), (2, 1), (3, 2)):
+        assert rel(out[i], chain[j]) < 5e-2
+    with pytest.raises(ValueError):
+        m.forward_tree([1] * 6, [-1] * 6, 3)
+    m.close()
