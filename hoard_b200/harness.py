@@ -651,7 +651,7 @@ class DecodeModel:
         if not hasattr(self, "_xb"):
             z = lambda *sh: torch.zeros(*sh, dtype=torch.float32, device=self.dev)
             self._xb, self._x2b, self._curb = z(self.max_batch, H), z(self.max_batch, H), z(self.max_batch, H)
-            self._qb, self._kb, self._vb = z(self.max_batch, self.nq), z(self.max_batch, self.nkv), z(self.max_batch, self.nkv)
+            self._qb, self._kb, self._vb = z(self.max_batch, self.nqp), z(self.max_batch, self.nkv), z(self.max_batch, self.nkv)
             self._attb, self._lgb = z(self.max_batch, self.nq), z(self.max_batch, c.n_vocab)
         xb, x2b, cur = self._xb, self._x2b, self._curb
         for i in range(m):

@@ -147,3 +147,22 @@ def test_trees_in_a_context_shorter_than_the_largest_batch(weights):
     with pytest.raises(ValueError):
         m.forward_tree([1] * 6, [-1] * 6, 3)
     m.close()
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_batches_of_a_gated_attention(hd):
+    """Layers with an output gate and no delta-net between them: a token's q row in a batch holds its gate, and a tree goes
+    through the operators with it."""
+    cfg = dataclasses.replace(QWEN_S, n_head=8, head_dim=hd, attn_gate=True, rope_dim=64)
+    m = hx.DecodeModel(cfg, hx.seeded_tensors(cfg, seed=5, device=torch.device("cuda", 0)), device=0, max_ctx=80, max_batch=6)
+    prompt = prompt_of(cfg, 30)
+    tokens = prompt_of(cfg, 6, seed=8)
+    m.generate(prompt, 1)
+    assert m._q_view(m.q).shape == m._gate_view(m.q).shape == (1, 8, hd)
+    out = m.forward_batch(tokens, 30)
+    steps = m.score(prompt + tokens + [0], 31)
+    assert all(rel(out[i], steps[i]) < 5e-2 for i in range(6))
+    m.generate(prompt, 1)
+    tree = m.forward_tree(tokens, [-1, 0, 1, 2, 3, 4], 30)
+    assert all(rel(tree[i], out[i]) < 5e-2 for i in range(6))
+    m.close()
