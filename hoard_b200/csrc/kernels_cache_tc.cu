@@ -401,16 +401,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
             top = fmaxf(mx, __fmul_rn(top, sc));
             const float f = top > mx ? ex2f(mx - top) : 1.f;
             // weights 2^(s sc - top + P_EXP), their exponents by one multiply-add each. Where the roundings of s sc and of top
-            // may come to more than 2^-4, in the order that makes the largest weight 2^P_EXP exactly
+            // may come to more than 2^-4, s sc - top is formed first, in the order that makes the largest weight 2^P_EXP exactly
             const float base = top == -INFINITY ? 0.f : top;
+            float mul = sc, add = Terms<KT>::P_EXP - base;
             if (__any_sync(0xffffffffu, fabsf(base) > LARGE_SCORE)) {
 #pragma unroll
                 for (int i = 0; i < TK; ++i)
-                    sr[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(sr[i]), sc), base) + Terms<KT>::P_EXP);
-            } else {
-                const float b = Terms<KT>::P_EXP - base;
-#pragma unroll
-                for (int i = 0; i < TK; ++i) sr[i] = __float_as_uint(fmaf(__uint_as_float(sr[i]), sc, b));
+                    sr[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(sr[i]), sc), base));
+                mul = 1.f;
+                add = Terms<KT>::P_EXP;
             }
             mx = top;
             float sum = 0.f;
@@ -419,8 +418,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_cache_attention_tc(const Cach
                 uint32_t w[TN][16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float p0 = ex2f(__uint_as_float(sr[32 * h + 2 * i]));
-                    float p1 = ex2f(__uint_as_float(sr[32 * h + 2 * i + 1]));
+                    float p0 = ex2f(fmaf(__uint_as_float(sr[32 * h + 2 * i]), mul, add));
+                    float p1 = ex2f(fmaf(__uint_as_float(sr[32 * h + 2 * i + 1]), mul, add));
                     sum += p0 + p1;
 #pragma unroll
                     for (int u = 0; u < TN; ++u) w[u][i] = take_term<KT>(p0, p1);
