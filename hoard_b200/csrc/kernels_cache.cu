@@ -713,7 +713,8 @@ template <typename KT> cudaError_t attention_type(const CacheAttn& a, cudaStream
 int cache_tile_dims(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
 // The plan of a call: query rows of a tile (8 or 16), splits of the chunks and who joins them, or the tensor-core form.
-// The choice is by time, from what the parts were measured to take in microseconds (f16; bf16 a tenth more):
+// The choice is by time, from what the parts were measured to take in microseconds, for f16 (bf16 takes a tenth more in either
+// form, which the choice leaves out):
 //
 //   - a CTA's start and end, and a chunk of each of its warps (a CTA has as many in turn as its fullest warp):
 //     tiles of 16 cost more of both and halve the reads of the cache where there are more than 8 rows

@@ -18,8 +18,8 @@
 // The tensor cores truncate as they accumulate, so a tile's O leaves tensor memory after every tile and is added
 // with rounding, sums scaled to a risen maximum in the same multiply-add.
 // The last tile is the tokens' own rows, with their masks. k_cache_combine joins the splits.
-// Bound by power in long calls: 64 tokens of 8 heads x 4 KV heads over 131008 rows are 2 x 137 GFLOP in 225 us, 1.2 PFLOP/s of
-// products, and 270 when repeated (the clock falls to 1.4 GHz). In short ones by what does not depend on the cache's length:
+// Bound by power in long calls: 64 tokens of 8 heads x 4 KV heads over 131008 rows are 2 x 137 GFLOP in 240 us, 1.14 PFLOP/s of
+// products, and 275 when repeated (the clock falls to 1.4 GHz). In short ones by what does not depend on the cache's length:
 // tensor memory, q staged and split, the first tile, the end, 10 us together.
 // Every wait is bounded; a CTA whose wait ran out reports totals of NaN, which reach the output.
 #include "common.cuh"

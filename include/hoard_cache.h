@@ -60,7 +60,8 @@ typedef struct hoard_kv_query {
 
 /* out[t][h] = sum_j p_j V[j], p = softmax over the rows that token t sees of scale * q[t][h] . K[j]: every past
  * row and its visible own rows. A token that sees nothing gets 0; what masked rows hold, infinities and
- * NaN among it, does not reach the result. acc (optional, f32 [n_head_kv][max_rows], m <= max_acc_tokens):
+ * NaN among it, does not reach the result. Of a row that is seen an infinity may come out as NaN. Sums are
+ * f32 and weights at most 1 in them (2^14 over f16): |V| times the rows has to stay below the largest float. acc (optional, f32 [n_head_kv][max_rows], m <= max_acc_tokens):
  * acc[kv][j] += sum of p_j over the tokens and the heads of KV head kv, in a fixed order. */
 int hoard_kv_attention(const hoard_kv_desc* d, const hoard_kv_query* a, float* acc, void* ws, hoard_stream stream);
 
